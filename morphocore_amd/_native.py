@@ -1,4 +1,5 @@
-"""ctypes binding of the C ABI in ``include/morphocore_amd.h`` (``libmorphocore_amd.so``).
+"""ctypes binding of the C ABI in ``include/morphocore_amd.h`` and ``include/morphocore_amd_mixer.h``
+(``libmorphocore_amd.so``).
 
 The library holds the gfx950 kernels; nothing here computes. Every call enqueues work on the
 current HIP stream of the tensors' device, which is what the reference's CUDA launchers do with
@@ -77,6 +78,19 @@ EXPORTS = (
     "mca_probe_smorph_exp_f64",
 )
 
+# Every symbol include/morphocore_amd_mixer.h declares.
+MIXER_EXPORTS = (
+    "mca_pack8",
+    "mca_unpack8",
+    "mca_rms_norm_forward",
+    "mca_rms_norm_backward_workspace_size",
+    "mca_rms_norm_backward",
+    "mca_gated_silu_forward",
+    "mca_gated_silu_backward",
+    "mca_grad_weight8_workspace_size",
+    "mca_grad_weight8",
+)
+
 _lib = None
 
 
@@ -106,6 +120,19 @@ def lib() -> ctypes.CDLL:
     so.mca_version.argtypes = []
     so.mca_last_error.restype = ctypes.c_char_p
     so.mca_last_error.argtypes = []
+    for name, args in (("mca_pack8", [_I, _P, _I64, _P, _P, _I64, _I64, _P]),
+                       ("mca_unpack8", [_I, _P, _P, _P, _I64, _I64, _P]),
+                       ("mca_rms_norm_forward", [_I, _I, _P, _I64, _P, _I64, _P, ctypes.c_float, _P, _P, _P, _P, _P, _I64, _I64, _P]),
+                       ("mca_rms_norm_backward", [_I, _I, _P, _I64, _P, _I64, _P, _I64, _P, _P, _P, _P, _I64, _I64, _P, _SZ, _P]),
+                       ("mca_gated_silu_forward", [_I, _P, _I64, _P, _I64] + [_P] * 7 + [_I64, _I64, _P]),
+                       ("mca_gated_silu_backward", [_I, _P, _I64, _P, _I64, _P, _I64] + [_P] * 6 + [_I64, _I64, _I64, _P]),
+                       ("mca_grad_weight8", [_I, _I, _P, _I64, _P, _P, _P, _I64, _I64, _I64, _P, _SZ, _P])):
+        getattr(so, name).argtypes = args
+        getattr(so, name).restype = _I
+    so.mca_rms_norm_backward_workspace_size.argtypes = [_I64, _I64]
+    so.mca_rms_norm_backward_workspace_size.restype = _SZ
+    so.mca_grad_weight8_workspace_size.argtypes = [_I, _I64, _I64, _I64]
+    so.mca_grad_weight8_workspace_size.restype = _SZ
     so.mca_morpho_indices_bytes.argtypes = [_I] + _GEOM
     so.mca_morpho_indices_bytes.restype = _SZ
     for sfx, real in (("f32", ctypes.c_float), ("f64", ctypes.c_double)):

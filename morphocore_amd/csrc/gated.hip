@@ -1,0 +1,207 @@
+// 8-bit blocks on their own (pack8, unpack8) and the gated activation y = g * sigmoid(g) * u, whose forward
+// writes the 8-bit form of g and u for the backward, and of y for the weight gradient of the layer that
+// reads it:
+//   grad_g = grad_y * u * s * (1 + g * (1 - s)),  grad_u = grad_y * g * s,  s = sigmoid(g).
+//
+// Bound by HBM: one pass, 8 values a lane (16-byte accesses of 16-bit values). A workgroup's 256 lanes are
+// rows x G lanes; G, the power of two at or above the row's units, keeps the lanes of short rows busy, and a
+// row wider than G = 256 takes several workgroups (blockIdx.x), so that one row already fills many CUs.
+#include "block8.hpp"
+#include "launch.hpp"
+#include "mixer.hpp"
+
+namespace mca
+{
+
+struct RowGrid
+{
+    dim3 grid;
+    int lanes_log2;
+};
+
+// Rows beyond the grid are taken in the kernels' loop.
+static RowGrid row_grid(int64_t rows, int cols)
+{
+    const int units = blocks_of(cols) * MX_LANES;
+    int lg = 2;
+    while ((1 << lg) < units && lg < 8) ++lg;
+    const int64_t x = (units + (1 << lg) - 1) >> lg, per = BLOCK >> lg, y = (rows + per - 1) / per;
+    const int64_t most = 65535;
+    return RowGrid{dim3((unsigned)x, (unsigned)(y < most ? y : most)), lg};
+}
+
+// The lane's unit of its row, and the loop over the rows.
+#define MCA_ROW_LOOP(unit, row)                                                                   \
+    const int unit = (int)(blockIdx.x << lanes_log2) + (int)(threadIdx.x & ((1u << lanes_log2) - 1)); \
+    if (unit >= blocks_of(cols) * MX_LANES) return;                                               \
+    const int rows_per = BLOCK >> lanes_log2;                                                     \
+    for (int64_t row = (int64_t)blockIdx.y * rows_per + (threadIdx.x >> lanes_log2); row < rows; row += (int64_t)gridDim.y * rows_per)
+
+template <typename T>
+__global__ __launch_bounds__(BLOCK) void pack8_kernel(const T* __restrict__ x, int64_t xs, uint8_t* __restrict__ codes,
+                                                      uint8_t* __restrict__ scales, int64_t rows, int cols, int lanes_log2)
+{
+    const int nb = blocks_of(cols);
+    MCA_ROW_LOOP(unit, row)
+    {
+        const int c = unit * UNIT, valid = cols - c;
+        float v[UNIT];
+        load_unit(x + row * xs + c, valid, v);
+        store_packed(codes + row * cols, scales + row * nb, unit, valid, v);
+    }
+}
+
+// float16 holds less than the packed values: those beyond its largest saturate.
+template <typename T>
+__device__ __forceinline__ void saturate_unit(float (&v)[UNIT])
+{
+    if constexpr (std::is_same_v<T, _Float16>)
+    {
+#pragma unroll
+        for (int j = 0; j < UNIT; ++j)
+            if (v[j] == v[j]) v[j] = fminf(fmaxf(v[j], -65504.0f), 65504.0f);
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(BLOCK) void unpack8_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
+                                                        T* __restrict__ out, int64_t rows, int cols, int lanes_log2)
+{
+    const int nb = blocks_of(cols);
+    MCA_ROW_LOOP(unit, row)
+    {
+        const int c = unit * UNIT, valid = cols - c;
+        if (valid <= 0) continue;
+        float v[UNIT];
+        unpack_unit(load_codes(codes + row * cols + c, valid), scale_of(scales[row * nb + unit / MX_LANES]), v);
+        saturate_unit<T>(v);
+        store_unit(out + row * cols + c, valid, v);
+    }
+}
+
+// The library's exponential for float32; the hardware's, whose error grows with the argument to a few
+// float32 units in the last place, where the result is rounded to 16 bits.
+template <typename T>
+__device__ __forceinline__ float sigmoid_of(float g)
+{
+    const float e = std::is_same_v<T, float> ? expf(-g) : __expf(-g);
+    return 1.0f / (1.0f + e);
+}
+
+template <typename T>
+__global__ __launch_bounds__(BLOCK) void gated_silu_fwd_kernel(const T* __restrict__ gate, int64_t gs, const T* __restrict__ up, int64_t us,
+                                                               T* __restrict__ y, PackedOut g8, PackedOut u8, PackedOut y8, int64_t rows,
+                                                               int cols, int lanes_log2)
+{
+    const int nb = blocks_of(cols);
+    MCA_ROW_LOOP(unit, row)
+    {
+        const int c = unit * UNIT, valid = cols - c;
+        float g[UNIT], u[UNIT], v[UNIT];
+        load_unit(gate + row * gs + c, valid, g);
+        load_unit(up + row * us + c, valid, u);
+        if (g8.codes) store_packed(g8.codes + row * cols, g8.scales + row * nb, unit, valid, g);
+        if (u8.codes) store_packed(u8.codes + row * cols, u8.scales + row * nb, unit, valid, u);
+#pragma unroll
+        for (int j = 0; j < UNIT; ++j) v[j] = g[j] * sigmoid_of<T>(g[j]) * u[j];
+        if (valid > 0) store_unit(y + row * cols + c, valid, v);
+        if (y8.codes)
+        {
+            round_unit<T>(v);  // the 8-bit form is y's, as stored
+            store_packed(y8.codes + row * cols, y8.scales + row * nb, unit, valid, v);
+        }
+    }
+}
+
+template <typename T, bool PACKED>
+__global__ __launch_bounds__(BLOCK) void gated_silu_bwd_kernel(const T* __restrict__ gy, int64_t gys, const T* __restrict__ gate, int64_t gs,
+                                                               const T* __restrict__ up, int64_t us, PackedOut g8, PackedOut u8,
+                                                               T* __restrict__ gg, T* __restrict__ gu, int64_t grad_s, int64_t rows, int cols,
+                                                               int lanes_log2)
+{
+    const int nb = blocks_of(cols);
+    MCA_ROW_LOOP(unit, row)
+    {
+        const int c = unit * UNIT, valid = cols - c;
+        if (valid <= 0) continue;
+        float d[UNIT], g[UNIT], u[UNIT];
+        load_unit(gy + row * gys + c, valid, d);
+        if constexpr (PACKED)
+        {
+            const int64_t at = row * cols + c, block = row * nb + unit / MX_LANES;
+            unpack_unit(load_codes(g8.codes + at, valid), scale_of(g8.scales[block]), g);
+            unpack_unit(load_codes(u8.codes + at, valid), scale_of(u8.scales[block]), u);
+        }
+        else
+        {
+            load_unit(gate + row * gs + c, valid, g);
+            load_unit(up + row * us + c, valid, u);
+        }
+#pragma unroll
+        for (int j = 0; j < UNIT; ++j)
+        {
+            const float s = sigmoid_of<T>(g[j]);
+            u[j] = d[j] * u[j] * (s * (1.0f + g[j] * (1.0f - s)));
+            g[j] = d[j] * g[j] * s;
+        }
+        store_unit(gg + row * grad_s + c, valid, u);
+        store_unit(gu + row * grad_s + c, valid, g);
+    }
+}
+
+template <typename T>
+hipError_t pack8(const T* x, int64_t x_stride, uint8_t* codes, uint8_t* scales, int64_t rows, int cols, hipStream_t stream)
+{
+    if (rows <= 0 || cols <= 0) return hipSuccess;
+    const RowGrid g = row_grid(rows, cols);
+    pack8_kernel<T><<<g.grid, BLOCK, 0, stream>>>(x, x_stride, codes, scales, rows, cols, g.lanes_log2);
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t unpack8(const uint8_t* codes, const uint8_t* scales, T* out, int64_t rows, int cols, hipStream_t stream)
+{
+    if (rows <= 0 || cols <= 0) return hipSuccess;
+    const RowGrid g = row_grid(rows, cols);
+    unpack8_kernel<T><<<g.grid, BLOCK, 0, stream>>>(codes, scales, out, rows, cols, g.lanes_log2);
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t gated_silu_forward(const T* gate, int64_t g_stride, const T* up, int64_t u_stride, T* y, PackedOut gate8, PackedOut up8,
+                              PackedOut y8, int64_t rows, int cols, hipStream_t stream)
+{
+    if (rows <= 0 || cols <= 0) return hipSuccess;
+    const RowGrid g = row_grid(rows, cols);
+    gated_silu_fwd_kernel<T><<<g.grid, BLOCK, 0, stream>>>(gate, g_stride, up, u_stride, y, gate8, up8, y8, rows, cols, g.lanes_log2);
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t gated_silu_backward(const T* grad_y, int64_t gy_stride, const T* gate, int64_t g_stride, const T* up, int64_t u_stride,
+                               PackedOut gate8, PackedOut up8, T* grad_gate, T* grad_up, int64_t grad_stride, int64_t rows, int cols,
+                               hipStream_t stream)
+{
+    if (rows <= 0 || cols <= 0) return hipSuccess;
+    const RowGrid g = row_grid(rows, cols);
+    if (gate)
+        gated_silu_bwd_kernel<T, false><<<g.grid, BLOCK, 0, stream>>>(grad_y, gy_stride, gate, g_stride, up, u_stride, gate8, up8, grad_gate,
+                                                                      grad_up, grad_stride, rows, cols, g.lanes_log2);
+    else
+        gated_silu_bwd_kernel<T, true><<<g.grid, BLOCK, 0, stream>>>(grad_y, gy_stride, gate, g_stride, up, u_stride, gate8, up8, grad_gate,
+                                                                     grad_up, grad_stride, rows, cols, g.lanes_log2);
+    return hipGetLastError();
+}
+
+#define MCA_GATED(T)                                                                                                                    \
+    template hipError_t pack8<T>(const T*, int64_t, uint8_t*, uint8_t*, int64_t, int, hipStream_t);                                     \
+    template hipError_t unpack8<T>(const uint8_t*, const uint8_t*, T*, int64_t, int, hipStream_t);                                      \
+    template hipError_t gated_silu_forward<T>(const T*, int64_t, const T*, int64_t, T*, PackedOut, PackedOut, PackedOut, int64_t, int,  \
+                                              hipStream_t);                                                                             \
+    template hipError_t gated_silu_backward<T>(const T*, int64_t, const T*, int64_t, const T*, int64_t, PackedOut, PackedOut, T*, T*,   \
+                                               int64_t, int64_t, int, hipStream_t)
+MCA_GATED(float);
+MCA_GATED(_Float16);
+MCA_GATED(__bf16);
+
+}  // namespace mca

@@ -1,0 +1,463 @@
+// Root-mean-square norm of rows, with the residual's addition and the output's 8-bit form:
+//   h = x (+ residual),  rstd = 1 / sqrt(mean(h^2) + eps),  y = h * rstd * w,
+// and its gradients, with n = h * rstd and a = grad_y * w:
+//   grad_x = grad_residual = rstd * (a - n * mean(a * n)) + grad_h,  grad_w = sum over the rows of grad_y * n.
+//
+// Bound by HBM: every operand is read once and every result written once. A row lies in the registers of G
+// lanes, V units each, between its sum and its scaling; G follows the row's width (a few lanes for rows of
+// an image's channels, so that a wave carries several rows; a workgroup for wide ones), so that a lane holds
+// at most 4 units. The forward normalises the float32 sum x + residual, not its rounded h (one rounding
+// fewer); the backward reads h as stored.
+#include "block8.hpp"
+#include "launch.hpp"
+#include "mixer.hpp"
+
+namespace mca
+{
+
+// Rows up to this many units (32768 values) stay in registers; wider ones are read twice.
+constexpr int NORM_MAX_UNITS = 4096;
+// Workgroups of a forward launch: 8 of 256 threads on each of 256 CUs, the rest of the rows in their loop.
+constexpr int NORM_BLOCKS = 2048;
+
+template <int G>
+constexpr int norm_threads()
+{
+    return G > BLOCK ? G : BLOCK;
+}
+
+// The sum over the G lanes of a row, in every one of them. `part` holds one value per wave, for two rows in
+// turn (`turn`), so that one barrier a row suffices.
+template <int G>
+__device__ __forceinline__ float row_sum(float s, float* part, int turn)
+{
+#pragma unroll
+    for (int d = 1; d < (G < WAVE ? G : WAVE); d *= 2) s += __shfl_xor(s, d);
+    if constexpr (G > WAVE)
+    {
+        constexpr int N = G / WAVE;
+        float* p = part + turn * N;
+        if (threadIdx.x % WAVE == 0) p[threadIdx.x / WAVE] = s;
+        __syncthreads();
+        s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) s += p[i];
+    }
+    return s;
+}
+
+template <typename T, typename WT, int G, int V>
+__global__ __launch_bounds__(norm_threads<G>()) void rms_norm_fwd_kernel(const T* __restrict__ x, int64_t xs, const T* __restrict__ r,
+                                                                         int64_t rs, const WT* __restrict__ w, float eps, T* __restrict__ y,
+                                                                         T* __restrict__ h, uint8_t* __restrict__ codes,
+                                                                         uint8_t* __restrict__ scales, float* __restrict__ rstd, int64_t rows,
+                                                                         int cols)
+{
+    constexpr int ROWS = norm_threads<G>() / G;
+    __shared__ float part[2 * (G > WAVE ? G / WAVE : 1)];
+    const int lane = threadIdx.x % G, nb = blocks_of(cols);
+    const float inv = 1.0f / (float)cols;
+    float wv[V][UNIT];
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+    {
+        const int c = (lane + G * k) * UNIT;
+        load_unit(w + c, cols - c, wv[k]);
+    }
+    int turn = 0;
+    for (int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / G; row < rows; row += (int64_t)gridDim.x * ROWS, turn ^= 1)
+    {
+        float v[V][UNIT];
+        float s = 0.0f;
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+        {
+            const int c = (lane + G * k) * UNIT;
+            load_unit(x + row * xs + c, cols - c, v[k]);
+            if (r)
+            {
+                float u[UNIT];
+                load_unit(r + row * rs + c, cols - c, u);
+#pragma unroll
+                for (int j = 0; j < UNIT; ++j) v[k][j] += u[j];
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+#pragma unroll
+            for (int j = 0; j < UNIT; ++j) s += v[k][j] * v[k][j];
+        const float q = 1.0f / sqrtf(row_sum<G>(s, part, turn) * inv + eps);
+        if (rstd && lane == 0) rstd[row] = q;
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+        {
+            const int c = (lane + G * k) * UNIT, valid = cols - c;
+            if (h && valid > 0) store_unit(h + row * cols + c, valid, v[k]);
+#pragma unroll
+            for (int j = 0; j < UNIT; ++j) v[k][j] = v[k][j] * q * wv[k][j];
+            if (y && valid > 0) store_unit(y + row * cols + c, valid, v[k]);
+            if (codes)
+            {
+                round_unit<T>(v[k]);  // the 8-bit form is y's, as stored
+                store_packed(codes + row * cols, scales + row * nb, lane + G * k, valid, v[k]);
+            }
+        }
+    }
+}
+
+// The same for rows of any width, one workgroup a row, the row read once for its sum and again to scale.
+template <typename T, typename WT>
+__global__ __launch_bounds__(1024) void rms_norm_fwd_wide_kernel(const T* __restrict__ x, int64_t xs, const T* __restrict__ r, int64_t rs,
+                                                                 const WT* __restrict__ w, float eps, T* __restrict__ y, T* __restrict__ h,
+                                                                 uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
+                                                                 float* __restrict__ rstd, int64_t rows, int cols)
+{
+    constexpr int G = 1024;
+    __shared__ float part[2 * G / WAVE];
+    const int nb = blocks_of(cols), padded = nb * MX_LANES;
+    int turn = 0;
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x, turn ^= 1)
+    {
+        const T* __restrict__ xr = x + row * xs;
+        const T* __restrict__ rr = r ? r + row * rs : nullptr;
+        auto load = [&](int unit, float(&v)[UNIT]) {
+            const int c = unit * UNIT;
+            load_unit(xr + c, cols - c, v);
+            if (rr)
+            {
+                float u[UNIT];
+                load_unit(rr + c, cols - c, u);
+#pragma unroll
+                for (int j = 0; j < UNIT; ++j) v[j] += u[j];
+            }
+        };
+        float s = 0.0f;
+        for (int unit = threadIdx.x; unit < padded; unit += G)
+        {
+            float v[UNIT];
+            load(unit, v);
+#pragma unroll
+            for (int j = 0; j < UNIT; ++j) s += v[j] * v[j];
+        }
+        const float q = 1.0f / sqrtf(row_sum<G>(s, part, turn) * (1.0f / (float)cols) + eps);
+        if (rstd && threadIdx.x == 0) rstd[row] = q;
+        for (int unit = threadIdx.x; unit < padded; unit += G)  // whole blocks: their lanes stay together
+        {
+            const int c = unit * UNIT, valid = cols - c;
+            float v[UNIT], wv[UNIT];
+            load(unit, v);
+            load_unit(w + c, valid, wv);
+            if (h && valid > 0) store_unit(h + row * cols + c, valid, v);
+#pragma unroll
+            for (int j = 0; j < UNIT; ++j) v[j] = v[j] * q * wv[j];
+            if (y && valid > 0) store_unit(y + row * cols + c, valid, v);
+            if (codes)
+            {
+                round_unit<T>(v);
+                store_packed(codes + row * cols, scales + row * nb, unit, valid, v);
+            }
+        }
+    }
+}
+
+// grad_x, and grad_w's sums over the workgroup's rows: lane sums over its rows in registers, then over the
+// row groups of the workgroup in lane and wave order, into slot blockIdx.x of `part` (a fixed order, the same
+// from run to run).
+template <typename T, typename WT, int G, int V>
+__global__ __launch_bounds__(norm_threads<G>()) void rms_norm_bwd_kernel(const T* __restrict__ gy, int64_t gys, const T* __restrict__ gh,
+                                                                         int64_t ghs, const T* __restrict__ h, int64_t hs,
+                                                                         const WT* __restrict__ w, const float* __restrict__ rstd,
+                                                                         T* __restrict__ gx, float* __restrict__ gw_part, int64_t rows, int cols)
+{
+    constexpr int THREADS = norm_threads<G>(), ROWS = THREADS / G;
+    __shared__ float part[2 * (G > WAVE ? G / WAVE : 1)];
+    const int lane = threadIdx.x % G;
+    const float inv = 1.0f / (float)cols;
+    float wv[V][UNIT], gw[V][UNIT];
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+    {
+        const int c = (lane + G * k) * UNIT;
+        load_unit(w + c, cols - c, wv[k]);
+#pragma unroll
+        for (int j = 0; j < UNIT; ++j) gw[k][j] = 0.0f;
+    }
+    int turn = 0;
+    for (int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / G; row < rows; row += (int64_t)gridDim.x * ROWS, turn ^= 1)
+    {
+        const float q = rstd[row];
+        float n[V][UNIT], a[V][UNIT];
+        float s = 0.0f;
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+        {
+            const int c = (lane + G * k) * UNIT;
+            load_unit(h + row * hs + c, cols - c, n[k]);
+            if (gy)
+            {
+                load_unit(gy + row * gys + c, cols - c, a[k]);
+            }
+            else
+            {
+#pragma unroll
+                for (int j = 0; j < UNIT; ++j) a[k][j] = 0.0f;
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+#pragma unroll
+            for (int j = 0; j < UNIT; ++j)
+            {
+                n[k][j] *= q;
+                gw[k][j] += a[k][j] * n[k][j];
+                a[k][j] *= wv[k][j];
+                s += a[k][j] * n[k][j];
+            }
+        if (!gx) continue;
+        const float m = row_sum<G>(s, part, turn) * inv;
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+        {
+            const int c = (lane + G * k) * UNIT, valid = cols - c;
+#pragma unroll
+            for (int j = 0; j < UNIT; ++j) a[k][j] = q * (a[k][j] - n[k][j] * m);
+            if (gh)
+            {
+                float u[UNIT];
+                load_unit(gh + row * ghs + c, valid, u);
+#pragma unroll
+                for (int j = 0; j < UNIT; ++j) a[k][j] += u[j];
+            }
+            if (valid > 0) store_unit(gx + row * cols + c, valid, a[k]);
+        }
+    }
+    if (!gw_part) return;
+    float* __restrict__ out = gw_part + (int64_t)blockIdx.x * cols;
+    if constexpr (G >= BLOCK)
+    {
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+        {
+            const int c = (lane + G * k) * UNIT;
+            if (c < cols) store_unit(out + c, cols - c, gw[k]);
+        }
+    }
+    else
+    {
+        constexpr int L = G < WAVE ? G : WAVE;  // lanes of a wave that hold distinct columns
+        __shared__ float sums[NWAVES][V][L][UNIT];
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+#pragma unroll
+            for (int j = 0; j < UNIT; ++j)
+            {
+                float t = gw[k][j];
+#pragma unroll
+                for (int d = L; d < WAVE; d *= 2) t += __shfl_xor(t, d);
+                if (threadIdx.x % WAVE < L) sums[threadIdx.x / WAVE][k][threadIdx.x % L][j] = t;
+            }
+        __syncthreads();
+        for (int c = threadIdx.x; c < cols; c += THREADS)
+        {
+            const int unit = c / UNIT, k = unit / G, l = unit % G, j = c % UNIT;
+            out[c] = ((sums[0][k][l][j] + sums[1][k][l][j]) + sums[2][k][l][j]) + sums[3][k][l][j];
+        }
+    }
+}
+
+// grad_x of rows of any width, one workgroup a row, read twice.
+template <typename T, typename WT>
+__global__ __launch_bounds__(1024) void rms_norm_bwd_wide_kernel(const T* __restrict__ gy, int64_t gys, const T* __restrict__ gh, int64_t ghs,
+                                                                 const T* __restrict__ h, int64_t hs, const WT* __restrict__ w,
+                                                                 const float* __restrict__ rstd, T* __restrict__ gx, int64_t rows, int cols)
+{
+    constexpr int G = 1024;
+    __shared__ float part[2 * G / WAVE];
+    const int units = units_of(cols);
+    int turn = 0;
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x, turn ^= 1)
+    {
+        const float q = rstd[row];
+        auto load = [&](int unit, float(&n)[UNIT], float(&a)[UNIT]) {
+            const int c = unit * UNIT;
+            float wv[UNIT];
+            load_unit(h + row * hs + c, cols - c, n);
+            load_unit(gy + row * gys + c, cols - c, a);
+            load_unit(w + c, cols - c, wv);
+#pragma unroll
+            for (int j = 0; j < UNIT; ++j)
+            {
+                n[j] *= q;
+                a[j] *= wv[j];
+            }
+        };
+        float s = 0.0f;
+        if (gy)
+            for (int unit = threadIdx.x; unit < units; unit += G)
+            {
+                float n[UNIT], a[UNIT];
+                load(unit, n, a);
+#pragma unroll
+                for (int j = 0; j < UNIT; ++j) s += a[j] * n[j];
+            }
+        const float m = row_sum<G>(s, part, turn) * (1.0f / (float)cols);
+        for (int unit = threadIdx.x; unit < units; unit += G)
+        {
+            const int c = unit * UNIT;
+            float n[UNIT] = {}, a[UNIT] = {};
+            if (gy) load(unit, n, a);
+#pragma unroll
+            for (int j = 0; j < UNIT; ++j) a[j] = q * (a[j] - n[j] * m);
+            if (gh)
+            {
+                float u[UNIT];
+                load_unit(gh + row * ghs + c, cols - c, u);
+#pragma unroll
+                for (int j = 0; j < UNIT; ++j) a[j] += u[j];
+            }
+            store_unit(gx + row * cols + c, cols - c, a);
+        }
+    }
+}
+
+// grad_w's sums of wide rows: a lane's unit over every gridDim.y-th row, into slot blockIdx.y.
+template <typename T>
+__global__ __launch_bounds__(BLOCK) void rms_norm_gw_wide_kernel(const T* __restrict__ gy, int64_t gys, const T* __restrict__ h, int64_t hs,
+                                                                 const float* __restrict__ rstd, float* __restrict__ gw_part, int64_t rows,
+                                                                 int cols)
+{
+    const int unit = blockIdx.x * BLOCK + threadIdx.x;
+    if (unit >= units_of(cols)) return;
+    const int c = unit * UNIT;
+    float gw[UNIT] = {};
+    for (int64_t row = blockIdx.y; row < rows; row += gridDim.y)
+    {
+        const float q = rstd[row];
+        float n[UNIT], a[UNIT];
+        load_unit(h + row * hs + c, cols - c, n);
+        load_unit(gy + row * gys + c, cols - c, a);
+#pragma unroll
+        for (int j = 0; j < UNIT; ++j) gw[j] += a[j] * (n[j] * q);
+    }
+    store_unit(gw_part + (int64_t)blockIdx.y * cols + c, cols - c, gw);
+}
+
+// f(G, V): lanes a row and units a lane, the narrowest that hold `units`.
+template <typename F>
+static hipError_t norm_shape(int units, F&& f)
+{
+    using std::integral_constant;
+#define MCA_NORM_SHAPE(G, V) \
+    if (units <= (G) * (V)) return f(integral_constant<int, G>(), integral_constant<int, V>())
+    MCA_NORM_SHAPE(4, 1);
+    MCA_NORM_SHAPE(8, 1);
+    MCA_NORM_SHAPE(16, 1);
+    MCA_NORM_SHAPE(32, 1);
+    MCA_NORM_SHAPE(64, 1);
+    MCA_NORM_SHAPE(64, 2);
+    MCA_NORM_SHAPE(64, 3);
+    MCA_NORM_SHAPE(64, 4);
+    MCA_NORM_SHAPE(256, 2);
+    MCA_NORM_SHAPE(256, 3);
+    MCA_NORM_SHAPE(256, 4);
+    MCA_NORM_SHAPE(1024, 2);
+    MCA_NORM_SHAPE(1024, 4);
+#undef MCA_NORM_SHAPE
+    return hipErrorInvalidValue;
+}
+
+static int norm_grid(int64_t rows, int rows_per_block, int most)
+{
+    const int64_t n = (rows + rows_per_block - 1) / rows_per_block;
+    return (int)(n < most ? n : most);
+}
+
+template <typename T, typename WT>
+hipError_t rms_norm_forward(const T* x, int64_t x_stride, const T* residual, int64_t r_stride, const WT* w, float eps, T* y, T* h,
+                            uint8_t* codes, uint8_t* scales, float* rstd, int64_t rows, int cols, hipStream_t stream)
+{
+    if (rows <= 0 || cols <= 0) return hipSuccess;
+    const int units = units_of(cols);
+    if (units > NORM_MAX_UNITS)
+    {
+        rms_norm_fwd_wide_kernel<T, WT><<<norm_grid(rows, 1, NORM_BLOCKS), 1024, 0, stream>>>(x, x_stride, residual, r_stride, w, eps, y, h,
+                                                                                             codes, scales, rstd, rows, cols);
+        return hipGetLastError();
+    }
+    return norm_shape(units, [&](auto g, auto v) {
+        constexpr int G = decltype(g)::value, V = decltype(v)::value;
+        rms_norm_fwd_kernel<T, WT, G, V><<<norm_grid(rows, norm_threads<G>() / G, NORM_BLOCKS), norm_threads<G>(), 0, stream>>>(
+            x, x_stride, residual, r_stride, w, eps, y, h, codes, scales, rstd, rows, cols);
+        return hipGetLastError();
+    });
+}
+
+// Slots of grad_w's partial sums: workgroups of a backward launch. Two workgroups a CU keep enough loads in
+// flight for wide rows, whose slots cost `cols` values each; narrow rows take more.
+static int norm_slots(int64_t rows, int cols)
+{
+    const int units = units_of(cols);
+    if (units > NORM_MAX_UNITS) return norm_grid(rows, 16, 64);
+    const int per = units > 64 * 4 ? 1 : BLOCK / (units > 32 ? 64 : units > 16 ? 32 : units > 8 ? 16 : units > 4 ? 8 : 4);
+    return norm_grid(rows, per, units > 64 ? 512 : 1024);
+}
+
+size_t rms_norm_backward_workspace(int64_t rows, int cols)
+{
+    return rows > 0 && cols > 0 ? align_up((size_t)norm_slots(rows, cols) * (size_t)cols * sizeof(float)) : 0;
+}
+
+template <typename T, typename WT>
+hipError_t rms_norm_backward(const T* grad_y, int64_t gy_stride, const T* grad_h, int64_t gh_stride, const T* h, int64_t h_stride, const WT* w,
+                             const float* rstd, T* grad_x, WT* grad_w, int64_t rows, int cols, void* workspace, hipStream_t stream)
+{
+    if (cols <= 0) return hipSuccess;
+    if (rows <= 0 || !grad_y)
+    {
+        if (grad_w)
+        {
+            const hipError_t err = sum_slots_async<WT>(nullptr, 0, cols, grad_w, stream);
+            if (err != hipSuccess) return err;
+        }
+        if (rows <= 0 || !grad_x) return hipSuccess;
+        grad_w = nullptr;
+    }
+    if (!grad_x && !grad_w) return hipSuccess;
+    const int units = units_of(cols), slots = norm_slots(rows, cols);
+    float* part = grad_w ? (float*)workspace : nullptr;
+    hipError_t err;
+    if (units > NORM_MAX_UNITS)
+    {
+        if (grad_x)
+            rms_norm_bwd_wide_kernel<T, WT><<<norm_grid(rows, 1, NORM_BLOCKS), 1024, 0, stream>>>(grad_y, gy_stride, grad_h, gh_stride, h, h_stride,
+                                                                                                 w, rstd, grad_x, rows, cols);
+        if (part)
+            rms_norm_gw_wide_kernel<T><<<dim3((units + BLOCK - 1) / BLOCK, slots), BLOCK, 0, stream>>>(grad_y, gy_stride, h, h_stride, rstd, part,
+                                                                                                       rows, cols);
+        err = hipGetLastError();
+    }
+    else
+    {
+        err = norm_shape(units, [&](auto g, auto v) {
+            constexpr int G = decltype(g)::value, V = decltype(v)::value;
+            rms_norm_bwd_kernel<T, WT, G, V><<<slots, norm_threads<G>(), 0, stream>>>(grad_y, gy_stride, grad_h, gh_stride, h, h_stride, w, rstd,
+                                                                                      grad_x, part, rows, cols);
+            return hipGetLastError();
+        });
+    }
+    if (err != hipSuccess || !part) return err;
+    return sum_slots_async<WT>(part, slots, cols, grad_w, stream);
+}
+
+#define MCA_NORM(T, WT)                                                                                                                     \
+    template hipError_t rms_norm_forward<T, WT>(const T*, int64_t, const T*, int64_t, const WT*, float, T*, T*, uint8_t*, uint8_t*, float*, \
+                                                int64_t, int, hipStream_t);                                                                 \
+    template hipError_t rms_norm_backward<T, WT>(const T*, int64_t, const T*, int64_t, const T*, int64_t, const WT*, const float*, T*, WT*, \
+                                                 int64_t, int, void*, hipStream_t)
+MCA_NORM(float, float);
+MCA_NORM(_Float16, _Float16);
+MCA_NORM(_Float16, float);
+MCA_NORM(__bf16, __bf16);
+MCA_NORM(__bf16, float);
+
+}  // namespace mca

@@ -1,0 +1,83 @@
+"""Activations kept in 8 bits: the blocks themselves, and a layer whose input is all that it keeps.
+
+No reference counterpart: its layers keep their inputs and outputs as they are for the backward.
+"""
+from typing import NamedTuple
+
+import torch
+
+from ._ops import ops
+
+
+class Packed8(NamedTuple):
+    """A tensor in 8-bit blocks of 32 values along its last dimension.
+
+    codes : float8_e4m3fn, of the tensor's shape.
+    scales : float8_e8m0fnu, [..., ceil(last / 32)], a power of two for each block.
+
+    A value is code * scale, within 1/16 of the original's magnitude or 2^-17 of its block's largest,
+    whichever is more. It is exact in bfloat16 and float32. NaN and infinities become NaN.
+    """
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+
+def pack8(x: torch.Tensor) -> Packed8:
+    """``x`` (float32, float16 or bfloat16, on a HIP device) in 8-bit blocks. Not differentiable.
+
+    Each block's scale 2^e has the smallest e in [-117, 119] with max |v| <= 448 * 2^e; codes are
+    rounded to nearest even.
+    """
+    return Packed8(*ops.pack8(x))
+
+
+def unpack8(packed: Packed8, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The values of ``packed`` (exact in float32 and bfloat16; rounded, and saturated at 65504, in float16)."""
+    return ops.unpack8(packed.codes, packed.scales, dtype)
+
+
+class _Checkpoint8(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, module, state, x, *params):
+        with torch.no_grad():
+            out = module(x)
+        if not isinstance(out, torch.Tensor):
+            raise TypeError(f"checkpoint8 takes a module that returns one tensor, not {type(out).__name__}")
+        ctx.module, ctx.state, ctx.dtype = module, state, x.dtype
+        ctx.save_for_backward(*pack8(x), *params)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        codes, scales, *params = ctx.saved_tensors
+        x = unpack8(Packed8(codes, scales), ctx.dtype).requires_grad_(ctx.needs_input_grad[2])
+        device = x.device
+        devices = [] if ctx.state is None else [device]
+        with torch.random.fork_rng(devices, enabled=ctx.state is not None, device_type="cuda"), torch.enable_grad():
+            if ctx.state is not None:
+                torch.set_rng_state(ctx.state[0])
+                torch.cuda.set_rng_state(ctx.state[1], device)
+            out = ctx.module(x)
+        wanted = [t for t, need in zip([x, *params], ctx.needs_input_grad[2:]) if need]
+        grads = iter(torch.autograd.grad(out, wanted, grad, allow_unused=True))
+        return None, None, *(next(grads) if need else None for need in ctx.needs_input_grad[2:])
+
+
+def checkpoint8(module: torch.nn.Module, x: torch.Tensor) -> torch.Tensor:
+    """``module(x)``, keeping only ``x``, in 8 bits, for the backward, which runs the module again on the
+    values kept and takes the gradients there.
+
+    The output is the module's own. The gradients are those of the module at the kept values (see
+    :class:`Packed8` for how far these are from ``x``). Modules that draw random numbers (dropout, weight noise) draw the same ones again.
+    A module with state that its forward changes (running statistics) changes it twice.
+
+    module : a module of one tensor to one tensor; its parameters' gradients flow as without the checkpoint.
+    x : float32, float16 or bfloat16 on a HIP device (any shape the module takes; blocks run along the last dimension).
+    """
+    params = [p for p in module.parameters() if p.requires_grad]
+    if not torch.is_grad_enabled() or not (x.requires_grad or params):
+        return module(x)
+    # A module in training may draw; its draws are repeated from the generators' states.
+    state = (torch.get_rng_state(), torch.cuda.get_rng_state(x.device)) if module.training and x.is_cuda else None
+    return _Checkpoint8.apply(module, state, x, *params)

@@ -1,0 +1,19 @@
+import torch
+import torch.nn as nn
+
+from ..functional import checkpoint8
+
+
+class Checkpoint8(nn.Module):
+    """A module of one tensor to one tensor (a MorphoStack, an Opening, a Sequential of them) that keeps only
+    its input, in 8 bits, and runs again in the backward (:func:`morphocore_amd.functional.checkpoint8`).
+    No reference counterpart."""
+
+    def __init__(self, module: nn.Module):
+        super().__init__()
+        if not isinstance(module, nn.Module):
+            raise TypeError(f"Checkpoint8 takes a module, not {type(module).__name__}")
+        self.module = module
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return checkpoint8(self.module, x)

@@ -4,10 +4,10 @@
 
 Two shared libraries, both written for gfx950 only:
   * morphocore_amd/libmorphocore_amd.so — the hand-written HIP kernels and their C ABI
-    (include/morphocore_amd.h), compiled by hipcc with --offload-arch=gfx950; it depends only on the
+    (include/morphocore_amd.h, include/morphocore_amd_mixer.h), compiled by hipcc with --offload-arch=gfx950; it depends only on the
     HIP runtime;
   * morphocore_amd/_C*.so — the PyTorch-ROCm extension that registers torch.ops.morphocore.* and its
-    C++ autograd Functions (csrc/torch_ops.cpp, host code compiled against torch's headers), linked
+    C++ autograd Functions (csrc/torch_ops.cpp, csrc/mixer_ops.cpp, host code compiled against torch's headers), linked
     to the kernel library.
 The sources are HIP and C++ only: no CUDA sources, no hipify step, no Triton. Objects are rebuilt when
 a source or a shared header is newer than them (--force rebuilds everything); sources compile in
@@ -32,9 +32,10 @@ ROCM_INCLUDE = "/opt/rocm/include"
 
 # The longest compiles first.
 KERNEL_SOURCES = ["morpho_fwd_f32_dilation.hip", "morpho_fwd_f32_erosion.hip", "morpho_fwd_f16.hip", "morpho_fwd_bf16.hip", "smorph_static.hip",
-                  "morpho_fwd_f64.hip", "morpho_fused.hip", "morpho_bwd.hip", "smorph.hip", "smorph_element.hip", "smorph_rows.hip", "morpho_ident.hip", "morpho_scatter.hip", "morpho_fwd.hip", "util.hip",
-                  "capi.cpp", "stack.cpp"]
-KERNEL_HEADERS = ["common.hpp", "launch.hpp", "morpho_fwd.hpp", "smorph_common.hpp", "smorph_element.hpp", os.path.join("..", "..", "include", "morphocore_amd.h")]
+                  "morpho_fwd_f64.hip", "morpho_fused.hip", "morpho_bwd.hip", "smorph.hip", "smorph_element.hip", "smorph_rows.hip", "morpho_ident.hip", "morpho_scatter.hip", "morpho_fwd.hip", "norm.hip", "weight8.hip", "gated.hip", "util.hip",
+                  "capi.cpp", "stack.cpp", "mixer_api.cpp"]
+KERNEL_HEADERS = ["common.hpp", "launch.hpp", "morpho_fwd.hpp", "smorph_common.hpp", "smorph_element.hpp", "block8.hpp", "mixer.hpp",
+                  os.path.join("..", "..", "include", "morphocore_amd.h"), os.path.join("..", "..", "include", "morphocore_amd_mixer.h")]
 # Packed FP32 instructions stay disabled: only scalar fp32 VALU forms are emitted.
 HIP_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-munsafe-fp-atomics", "-Wall", "-Wno-unused-function",
              "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
@@ -97,7 +98,8 @@ class HipBuildExt(build_ext):
         target = self.get_ext_fullpath(ext.name)
         os.makedirs(os.path.dirname(target), exist_ok=True)
         torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
-        deps = list(ext.sources) + [os.path.join(CSRC, "smorph_element.hpp"), os.path.join(ROOT, "include", "morphocore_amd.h"), KERNEL_LIB]
+        deps = list(ext.sources) + [os.path.join(CSRC, "smorph_element.hpp"), os.path.join(ROOT, "include", "morphocore_amd.h"),
+                                     os.path.join(ROOT, "include", "morphocore_amd_mixer.h"), KERNEL_LIB]
         if not _stale(target, deps, self.force):
             return
         abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
@@ -105,12 +107,15 @@ class HipBuildExt(build_ext):
         includes = cpp_extension.include_paths() + [sysconfig.get_paths()["include"], ROCM_INCLUDE]
         cflags = ["-O2", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
                   "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=_C"]
-        obj = os.path.join(OBJDIR, "torch_ops.cpp.o")
-        _run([cxx] + cflags + [f"-I{p}" for p in includes] + ["-c", ext.sources[0], "-o", obj])
+        objs = [os.path.join(OBJDIR, os.path.basename(src) + ".o") for src in ext.sources]
+        with ThreadPoolExecutor(self._jobs()) as pool:
+            for f in [pool.submit(_run, [cxx] + cflags + [f"-I{p}" for p in includes] + ["-c", src, "-o", obj])
+                      for src, obj in zip(ext.sources, objs)]:
+                f.result()
         libdir = os.path.dirname(KERNEL_LIB)
         # The extension finds libmorphocore_amd.so next to itself; torch's libraries (and the HIP
         # runtime torch loads) are already in the process when it is imported.
-        _run([cxx, "-shared", obj, "-o", target + ".tmp", f"-L{libdir}", "-lmorphocore_amd", "-Wl,-rpath,$ORIGIN", f"-L{torch_lib}",
+        _run([cxx, "-shared"] + objs + ["-o", target + ".tmp", f"-L{libdir}", "-lmorphocore_amd", "-Wl,-rpath,$ORIGIN", f"-L{torch_lib}",
               "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lamdhip64", f"-Wl,-rpath,{torch_lib}"])
         os.replace(target + ".tmp", target)
 
@@ -120,7 +125,7 @@ setup(
     version="0.13.1",
     description="morphocore's dilation / erosion / smorph hot path as HIP kernels for AMD Instinct MI355X (gfx950)",
     packages=["morphocore_amd", "morphocore_amd.functional", "morphocore_amd.nn"],
-    ext_modules=[Extension("morphocore_amd._C", sources=[os.path.join("morphocore_amd", "csrc", "torch_ops.cpp")])],
+    ext_modules=[Extension("morphocore_amd._C", sources=[os.path.join("morphocore_amd", "csrc", src) for src in ("torch_ops.cpp", "mixer_ops.cpp")])],
     cmdclass={"build_ext": HipBuildExt},
     python_requires=">=3.9",
 )

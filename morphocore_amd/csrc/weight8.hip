@@ -1,5 +1,20 @@
 // The weight gradient of a linear layer from its packed input:
 //   grad_weight[n, k] = sum over the rows m of grad_y[m, n] * value(codes[m, k]).
+//
+// A matrix product over the rows on the bfloat16 matrix instructions. A packed value (4 significant bits
+// times a power of two) is exact in bfloat16, and grad_y is split by truncation into as many bfloat16 terms
+// as its significand takes: bfloat16 itself, float16 two, float32 three; every product is then exact and
+// the sums are float32. Three bfloat16 products still run several times as fast as one float32 product.
+//
+// Both operands lie with the summed axis as the slow one, so a wave reads its fragments from LDS with the
+// transposing read (ds_read_b64_tr_b16: 16 lanes read 4 rows of 16 columns and each gets a column). A row
+// of a staged tile is stored in groups of 16 columns (32 bytes), group g of row m at place g ^ (m & 3), so
+// that the 4 rows of such a read lie in different banks. Tiles are double-buffered in LDS: the next rows'
+// loads are issued before the products of the present ones and stored after them. Codes become bfloat16 on
+// the way into LDS, once for the workgroup.
+//
+// Rows are split over workgroups where the output has too few tiles for the 256 CUs; each split writes its
+// float32 sums to a slot, and the slots are added in order (no atomics: the same result every time).
 #include "block8.hpp"
 #include "launch.hpp"
 #include "mixer.hpp"
@@ -7,73 +22,273 @@
 namespace mca
 {
 
-constexpr int TILE_N = 64, TILE_K = 64, TILE_M = 32;
-// Rows a split sums at least: below them the joining of the splits costs more than the products.
-constexpr int SPLIT_ROWS = 256;
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 
+// bfloat16 terms of a grad_y value.
 template <typename T>
-__global__ __launch_bounds__(BLOCK) void grad_weight8_kernel(const T* __restrict__ gy, int64_t gys, const uint8_t* __restrict__ codes,
-                                                             const uint8_t* __restrict__ scales, float* __restrict__ part, int64_t rows,
-                                                             int64_t split_rows, int out, int cols)
+constexpr int planes_of()
 {
-    __shared__ float a[TILE_M][TILE_N], b[TILE_M][TILE_K];
-    const int n0 = blockIdx.x * TILE_N, k0 = blockIdx.y * TILE_K, nb = blocks_of(cols);
-    const int tn = threadIdx.x / 16 * 4, tk = threadIdx.x % 16 * 4;
-    const int64_t m0 = blockIdx.z * split_rows, m1 = m0 + split_rows < rows ? m0 + split_rows : rows;
-    float acc[4][4] = {};
-    for (int64_t m = m0; m < m1; m += TILE_M)
+    return std::is_same_v<T, float> ? 3 : std::is_same_v<T, _Float16> ? 2 : 1;
+}
+
+// N x K outputs of a workgroup, M rows staged at a time, waves along N and K.
+template <int N_, int K_, int M_, int WN_, int WK_>
+struct WeightTile
+{
+    static constexpr int N = N_, K = K_, M = M_, WN = WN_, WK = WK_;
+    static constexpr int THREADS = WN * WK * WAVE;
+    static constexpr int FN = N / WN / 32, FK = K / WK / 32;  // 32 x 32 fragments of a wave
+};
+
+// Byte of column c (a multiple of 8) of row m in a staged tile of C columns.
+template <int C>
+__device__ __forceinline__ int tile_byte(int m, int c)
+{
+    return m * (C * 2) + (((c / 16) ^ (m & 3)) * 32) + (c & 8) * 2;
+}
+
+// A lane's 8 values of the summed axis (rows m0 + 8 (lane / 32) ..) for column c0 + lane % 32.
+template <int C>
+__device__ __forceinline__ bf16x8 read_fragment(const char* tile, int m0, int c0)
+{
+    const int l = threadIdx.x % WAVE, r = (l / 4) & 3;
+    const int group = (c0 / 16 + ((l / 16) & 1)) ^ r;
+    const char* p = tile + (m0 + 8 * (l / 32) + r) * (C * 2) + group * 32 + (l & 3) * 8;
+    typedef __attribute__((address_space(3))) bf16x4* lds4;
+    const bf16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)p);
+    const bf16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(p + 4 * C * 2));
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// The bfloat16 terms of 8 values, each the leading 8 bits of what the ones before leave.
+template <typename T, int P>
+__device__ __forceinline__ void split_unit(const T (&raw)[UNIT], bf16x8 (&term)[P])
+{
+    if constexpr (P == 1)
     {
-        const int r = threadIdx.x / 8, c = threadIdx.x % 8 * UNIT;
-        const bool in = m + r < m1;
-        float v[UNIT];
-        load_unit(gy + (m + r) * gys + n0 + c, in ? out - n0 - c : 0, v);
 #pragma unroll
-        for (int j = 0; j < UNIT; ++j) a[r][c + j] = v[j];
-        const int valid = in ? cols - k0 - c : 0;
-        const uint2 code = load_codes(codes + (m + r) * cols + k0 + c, valid);
-        unpack_unit(code, valid > 0 ? scale_of(scales[(m + r) * nb + (k0 + c) / MX_BLOCK]) : 1.0f, v);
+        for (int j = 0; j < UNIT; ++j) term[0][j] = raw[j];
+    }
+    else
+    {
 #pragma unroll
-        for (int j = 0; j < UNIT; ++j) b[r][c + j] = v[j];
-        __syncthreads();
-        for (int i = 0; i < TILE_M; ++i)
+        for (int j = 0; j < UNIT; ++j)
+        {
+            float v = (float)raw[j];
 #pragma unroll
-            for (int p = 0; p < 4; ++p)
+            for (int i = 0; i < P; ++i)
+            {
+                const uint32_t bits = __float_as_uint(v) & 0xffff0000u;
+                term[i][j] = __builtin_bit_cast(__bf16, (uint16_t)(bits >> 16));
+                // An infinity is its own first term and leaves nothing; a NaN stays one.
+                v = fabsf(v) == __builtin_inff() ? 0.0f : v - __uint_as_float(bits);
+            }
+        }
+    }
+}
+
+// One tile of the sums over rows [m0, m1), m0 = split * split_rows, to out + split * out_rows * cols.
+template <typename T, typename OT, typename L>
+__global__ __launch_bounds__(L::THREADS) void grad_weight8_kernel(const T* __restrict__ gy, int64_t gys, const uint8_t* __restrict__ codes,
+                                                                  const uint8_t* __restrict__ scales, OT* __restrict__ out, int64_t rows,
+                                                                  int64_t split_rows, int out_rows, int cols, int tiles_n, int tiles_k)
+{
+    constexpr int P = planes_of<T>(), THREADS = L::THREADS;
+    constexpr int A_BYTES = L::M * L::N * 2, B_BYTES = L::M * L::K * 2, BUFFER = P * A_BYTES + B_BYTES;
+    constexpr int UA = L::N / UNIT, UB = L::K / UNIT;               // units of a row
+    constexpr int NA = L::M * UA / THREADS, NB = L::M * UB / THREADS;  // units of a thread
+    static_assert(NA * THREADS == L::M * UA && NB * THREADS == L::M * UB);
+    __shared__ __align__(16) char lds[2][BUFFER];
+
+    const int tiles = tiles_n * tiles_k, work = xcd_work_index(blockIdx.x, gridDim.x);
+    const int split = work / tiles, tile = work % tiles;
+    const int n0 = tile / tiles_k * L::N, k0 = tile % tiles_k * L::K, nb = blocks_of(cols);
+    const int64_t m0 = split * split_rows, m1 = m0 + split_rows < rows ? m0 + split_rows : rows;
+    const bool full_cols = n0 + L::N <= out_rows && k0 + L::K <= cols;
+
+    T a[NA][UNIT];
+    uint2 b[NB];
+    uint32_t s[NB];
+    auto load = [&](int64_t m) {
+        const bool full = full_cols && m + L::M <= m1;
 #pragma unroll
-                for (int q = 0; q < 4; ++q) acc[p][q] += a[i][tn + p] * b[i][tk + q];
+        for (int i = 0; i < NA; ++i)
+        {
+            const int u = threadIdx.x + i * THREADS, c = n0 + u % UA * UNIT;
+            const int64_t row = m + u / UA;
+            const T* __restrict__ p = gy + row * gys + c;
+            if (full)
+            {
+                __builtin_memcpy(a[i], p, sizeof(a[i]));
+            }
+            else
+            {
+                const int valid = row < m1 ? out_rows - c : 0;
+                if (valid >= UNIT)
+                {
+                    __builtin_memcpy(a[i], p, sizeof(a[i]));
+                }
+                else
+                {
+#pragma unroll
+                    for (int j = 0; j < UNIT; ++j) a[i][j] = j < valid ? p[j] : T(0);
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+        {
+            const int u = threadIdx.x + i * THREADS, c = k0 + u % UB * UNIT;
+            const int64_t row = m + u / UB;
+            const int valid = full ? UNIT : row < m1 ? cols - c : 0;
+            b[i] = load_codes(codes + row * cols + c, valid);
+            s[i] = valid > 0 ? scales[row * nb + c / MX_BLOCK] : 127;
+        }
+    };
+    auto store = [&](char* buffer) {
+#pragma unroll
+        for (int i = 0; i < NA; ++i)
+        {
+            const int u = threadIdx.x + i * THREADS;
+            bf16x8 term[P];
+            split_unit<T, P>(a[i], term);
+#pragma unroll
+            for (int q = 0; q < P; ++q) *(bf16x8*)(buffer + q * A_BYTES + tile_byte<L::N>(u / UA, u % UA * UNIT)) = term[q];
+        }
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+        {
+            const int u = threadIdx.x + i * THREADS;
+            const float scale = scale_of(s[i]);
+            typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+            const bf16x2 v0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b[i].x, scale, false);
+            const bf16x2 v1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b[i].x, scale, true);
+            const bf16x2 v2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b[i].y, scale, false);
+            const bf16x2 v3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b[i].y, scale, true);
+            const bf16x8 v = {v0[0], v0[1], v1[0], v1[1], v2[0], v2[1], v3[0], v3[1]};
+            *(bf16x8*)(buffer + P * A_BYTES + tile_byte<L::K>(u / UB, u % UB * UNIT)) = v;
+        }
+    };
+
+    const int wave = threadIdx.x / WAVE, wn = wave / L::WK * (L::N / L::WN), wk = wave % L::WK * (L::K / L::WK);
+    // The first terms' sums; float32's further terms have sums of their own, so that the rounding of the large
+    // ones does not swallow them.
+    constexpr int SUMS = P == 3 ? 2 : 1;
+    f32x16 acc[SUMS][L::FN][L::FK] = {};
+    load(m0);
+    store(lds[0]);
+    __syncthreads();
+    int turn = 0;
+    for (int64_t m = m0; m < m1; m += L::M, turn ^= 1)
+    {
+        const bool more = m + L::M < m1;
+        if (more) load(m + L::M);
+        const char* buffer = lds[turn];
+#pragma unroll
+        for (int i = 0; i < L::M; i += 16)
+        {
+            bf16x8 fb[L::FK];
+#pragma unroll
+            for (int k = 0; k < L::FK; ++k) fb[k] = read_fragment<L::K>(buffer + P * A_BYTES, i, wk + 32 * k);
+#pragma unroll
+            for (int q = P - 1; q >= 0; --q)  // small terms first
+            {
+                bf16x8 fa[L::FN];
+#pragma unroll
+                for (int n = 0; n < L::FN; ++n) fa[n] = read_fragment<L::N>(buffer + q * A_BYTES, i, wn + 32 * n);
+#pragma unroll
+                for (int n = 0; n < L::FN; ++n)
+#pragma unroll
+                    for (int k = 0; k < L::FK; ++k) acc[q ? SUMS - 1 : 0][n][k] =
+                            __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[n], fb[k], acc[q ? SUMS - 1 : 0][n][k], 0, 0, 0);
+            }
+        }
+        if (more) store(lds[turn ^ 1]);
         __syncthreads();
     }
-    float* __restrict__ o = part + (int64_t)blockIdx.z * out * cols;
+
+    // A lane holds column lane % 32 and rows 8 (r / 4) + 4 (lane / 32) + r % 4 of a fragment.
+    const int l = threadIdx.x % WAVE;
+    OT* __restrict__ o = out + (int64_t)split * out_rows * cols;
 #pragma unroll
-    for (int p = 0; p < 4; ++p)
+    for (int n = 0; n < L::FN; ++n)
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-            if (n0 + tn + p < out && k0 + tk + q < cols) o[(int64_t)(n0 + tn + p) * cols + k0 + tk + q] = acc[p][q];
+        for (int k = 0; k < L::FK; ++k)
+        {
+            const int col = k0 + wk + 32 * k + l % 32;
+            if (col >= cols) continue;
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+            {
+                const int row = n0 + wn + 32 * n + 8 * (r / 4) + 4 * (l / 32) + r % 4;
+                float v = acc[0][n][k][r];
+                if constexpr (SUMS == 2) v += acc[1][n][k][r];
+                if (row < out_rows) o[(int64_t)row * cols + col] = (OT)v;
+            }
+        }
 }
+
+using WideTile = WeightTile<256, 256, 64, 2, 4>;
+using MiddleTile = WeightTile<128, 128, 32, 2, 2>;
+using SmallTile = WeightTile<64, 64, 64, 2, 2>;
 
 struct WeightPlan
 {
-    dim3 grid;
+    int tile;  // 0 wide, 1 middle, 2 small
+    int tiles_n, tiles_k, splits;
     int64_t split_rows;
-    int splits;
 };
 
-static WeightPlan weight_plan(int64_t rows, int out, int cols)
+// Rows a split sums at least: below them the joining of the splits costs more than the products.
+constexpr int SPLIT_ROWS = 512;
+
+static WeightPlan weight_plan(int planes, int64_t rows, int out, int cols)
 {
-    const int64_t tiles = (int64_t)((out + TILE_N - 1) / TILE_N) * ((cols + TILE_K - 1) / TILE_K);
-    int64_t splits = 1024 / tiles, most = (rows + SPLIT_ROWS - 1) / SPLIT_ROWS;
+    WeightPlan p{};
+    int side = 64, step = 64;
+    p.tile = 2;
+    if (out > 64 || cols > 64) p.tile = 1, side = 128, step = 32;
+    if (planes == 1 && out > 128 && cols > 128)
+    {
+        const int64_t wide = (int64_t)((out + 255) / 256) * ((cols + 255) / 256) * ((rows + SPLIT_ROWS - 1) / SPLIT_ROWS);
+        if (wide >= 256) p.tile = 0, side = 256, step = 64;
+    }
+    p.tiles_n = (out + side - 1) / side;
+    p.tiles_k = (cols + side - 1) / side;
+    const int64_t tiles = (int64_t)p.tiles_n * p.tiles_k;
+    const int64_t wanted = p.tile == 0 ? 256 : 512;
+    int64_t splits = wanted / tiles, most = (rows + SPLIT_ROWS - 1) / SPLIT_ROWS;
     splits = splits < 1 ? 1 : splits;
     splits = splits < most ? splits : most;
-    int64_t per = (rows + splits - 1) / splits;
-    per = (per + TILE_M - 1) / TILE_M * TILE_M;
-    splits = (rows + per - 1) / per;
-    return WeightPlan{dim3((out + TILE_N - 1) / TILE_N, (cols + TILE_K - 1) / TILE_K, (unsigned)splits), per, (int)splits};
+    p.split_rows = ((rows + splits - 1) / splits + step - 1) / step * step;
+    p.splits = (int)((rows + p.split_rows - 1) / p.split_rows);
+    return p;
 }
 
 template <typename T>
 size_t grad_weight8_workspace(int64_t rows, int out, int cols)
 {
     if (rows <= 0 || out <= 0 || cols <= 0) return 0;
-    return align_up((size_t)weight_plan(rows, out, cols).splits * out * cols * sizeof(float));
+    const WeightPlan p = weight_plan(planes_of<T>(), rows, out, cols);
+    return p.splits > 1 ? align_up((size_t)p.splits * out * cols * sizeof(float)) : 0;
+}
+
+template <typename T, typename OT>
+static hipError_t weight_launch(const WeightPlan& p, const T* gy, int64_t gys, const uint8_t* codes, const uint8_t* scales, OT* out, int64_t rows,
+                                int out_rows, int cols, hipStream_t stream)
+{
+    const unsigned grid = (unsigned)((int64_t)p.tiles_n * p.tiles_k * p.splits);
+    auto run = [&](auto tile) {
+        using L = decltype(tile);
+        grad_weight8_kernel<T, OT, L><<<grid, L::THREADS, 0, stream>>>(gy, gys, codes, scales, out, rows, p.split_rows, out_rows, cols, p.tiles_n,
+                                                                       p.tiles_k);
+        return hipGetLastError();
+    };
+    if constexpr (planes_of<T>() == 1)
+        if (p.tile == 0) return run(WideTile());
+    return p.tile == 1 ? run(MiddleTile()) : run(SmallTile());
 }
 
 template <typename T, typename OT>
@@ -82,9 +297,10 @@ hipError_t grad_weight8(const T* grad_y, int64_t gy_stride, const uint8_t* codes
 {
     if (out <= 0 || cols <= 0) return hipSuccess;
     if (rows <= 0) return sum_slots_async<OT>(nullptr, 0, (int64_t)out * cols, grad_weight, stream);
-    const WeightPlan p = weight_plan(rows, out, cols);
-    grad_weight8_kernel<T><<<p.grid, BLOCK, 0, stream>>>(grad_y, gy_stride, codes, scales, (float*)workspace, rows, p.split_rows, out, cols);
-    const hipError_t err = hipGetLastError();
+    const WeightPlan p = weight_plan(planes_of<T>(), rows, out, cols);
+    if ((int64_t)p.tiles_n * p.tiles_k * p.splits > 0x7fffffff) return hipErrorInvalidValue;
+    if (p.splits == 1) return weight_launch<T, OT>(p, grad_y, gy_stride, codes, scales, grad_weight, rows, out, cols, stream);
+    const hipError_t err = weight_launch<T, float>(p, grad_y, gy_stride, codes, scales, (float*)workspace, rows, out, cols, stream);
     if (err != hipSuccess) return err;
     return sum_slots_async<OT>((const float*)workspace, p.splits, (int64_t)out * cols, grad_weight, stream);
 }
@@ -121,6 +337,7 @@ __global__ __launch_bounds__(BLOCK) void sum_slots_kernel(const float* __restric
         for (int k = 0; k < 4; ++k) sums[q][g][k] = s[k];
         __syncthreads();
         if (q != 0) return;
+#pragma unroll 4
         for (int i = 1; i < Q; ++i)
 #pragma unroll
             for (int k = 0; k < 4; ++k) s[k] += sums[i][g][k];

@@ -30,75 +30,160 @@ constexpr float LARGEST = 0x1.cp127f;
 inline __host__ __device__ int units_of(int cols) { return (int)(((int64_t)cols + UNIT - 1) / UNIT); }
 inline __host__ __device__ int blocks_of(int cols) { return (int)(((int64_t)cols + MX_BLOCK - 1) / MX_BLOCK); }
 
-// The `valid` (at least 8: all) first of 8 values at p, the others 0. p is aligned to T only: global
-// accesses of gfx950 take any alignment, so rows of odd widths load as wide as others.
+// A unit as stored: 8 values in consecutive dwords (two 16-bit values each), which keeps a unit that waits in
+// registers as small as it is in memory.
 template <typename T>
-__device__ __forceinline__ void load_unit(const T* __restrict__ p, int valid, float (&v)[UNIT])
+struct RawUnit
 {
-    T raw[UNIT];
+    static constexpr int DWORDS = UNIT * (int)sizeof(T) / 4;
+    uint32_t d[DWORDS];
+
+    __device__ __forceinline__ float operator[](int j) const
+    {
+        if constexpr (sizeof(T) == 4)
+            return __uint_as_float(d[j]);
+        else if constexpr (std::is_same_v<T, __bf16>)
+            return __uint_as_float(j % 2 ? d[j / 2] & 0xffff0000u : d[j / 2] << 16);
+        else
+            return (float)__builtin_bit_cast(_Float16, (uint16_t)(d[j / 2] >> (16 * (j % 2))));
+    }
+
+    // Rounded to nearest even.
+    __device__ __forceinline__ void set(const float (&v)[UNIT])
+    {
+#pragma unroll
+        for (int i = 0; i < DWORDS; ++i)
+        {
+            if constexpr (sizeof(T) == 4)
+            {
+                d[i] = __float_as_uint(v[i]);
+            }
+            else
+            {
+                typedef float f2 __attribute__((ext_vector_type(2)));
+                typedef T t2 __attribute__((ext_vector_type(2)));
+                const f2 pair = {v[2 * i], v[2 * i + 1]};
+                d[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(pair, t2));
+            }
+        }
+    }
+
+    // n values down, zeros above.
+    __device__ __forceinline__ void shift(int n)
+    {
+        constexpr int PER = 4 / (int)sizeof(T);  // values of a dword
+#pragma unroll
+        for (int s = 4; s >= PER; s /= 2)
+            if (n & s)
+            {
+#pragma unroll
+                for (int i = 0; i < DWORDS; ++i) d[i] = i + s / PER < DWORDS ? d[i + s / PER] : 0;
+            }
+        if constexpr (PER == 2)
+            if (n & 1)
+            {
+#pragma unroll
+                for (int i = 0; i < DWORDS; ++i) d[i] = d[i] >> 16 | (i + 1 < DWORDS ? d[i + 1] << 16 : 0);
+            }
+    }
+};
+
+// The 8 values from column c of a row on, p the first of them, `valid` = the columns from c to the row's end:
+// those beyond it are 0. p is aligned to T only: global accesses of gfx950 take any alignment, so rows of
+// odd widths load as wide as others. A row's last, partial unit is read as the row's last 8 values, which
+// are then moved down (a row of fewer than 8 is read value by value).
+template <typename T>
+__device__ __forceinline__ void load_raw(const T* __restrict__ p, int c, int valid, RawUnit<T>& raw)
+{
     if (valid >= UNIT)
     {
-        __builtin_memcpy(raw, p, sizeof(raw));
+        __builtin_memcpy(raw.d, p, sizeof(raw.d));
+        return;
     }
-    else
+#pragma unroll
+    for (int i = 0; i < RawUnit<T>::DWORDS; ++i) raw.d[i] = 0;
+    if (valid <= 0) return;
+    if (c > 0)
     {
-#pragma unroll
-        for (int j = 0; j < UNIT; ++j) raw[j] = j < valid ? p[j] : T(0);
+        __builtin_memcpy(raw.d, p - (UNIT - valid), sizeof(raw.d));
+        raw.shift(UNIT - valid);
+        return;
     }
 #pragma unroll
-    for (int j = 0; j < UNIT; ++j) v[j] = (float)raw[j];
+    for (int j = 0; j < UNIT - 1; ++j)
+        if (j < valid)
+        {
+            if constexpr (sizeof(T) == 4)
+                raw.d[j] = __builtin_bit_cast(uint32_t, p[j]);
+            else
+                raw.d[j / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, p[j]) << (16 * (j % 2));
+        }
+}
+
+template <typename T>
+__device__ __forceinline__ void load_unit(const T* __restrict__ p, int c, int valid, float (&v)[UNIT])
+{
+    RawUnit<T> raw;
+    load_raw(p, c, valid, raw);
+#pragma unroll
+    for (int j = 0; j < UNIT; ++j) v[j] = raw[j];
 }
 
 template <typename T>
 __device__ __forceinline__ void store_unit(T* __restrict__ p, int valid, const float (&v)[UNIT])
 {
-    T raw[UNIT];
-#pragma unroll
-    for (int j = 0; j < UNIT; ++j) raw[j] = (T)v[j];
+    RawUnit<T> raw;
+    raw.set(v);
     if (valid >= UNIT)
     {
-        __builtin_memcpy(p, raw, sizeof(raw));
+        __builtin_memcpy(p, raw.d, sizeof(raw.d));
+        return;
     }
-    else
+    // The rest of a row in pieces of 4, 2 and 1 values.
+    if (valid <= 0) return;
+    if (valid & 4)
     {
-#pragma unroll
-        for (int j = 0; j < UNIT; ++j)
-            if (j < valid) p[j] = raw[j];
+        __builtin_memcpy(p, raw.d, 4 * sizeof(T));
+        raw.shift(4);
     }
+    if (valid & 2)
+    {
+        __builtin_memcpy(p + (valid & 4), raw.d, 2 * sizeof(T));
+        raw.shift(2);
+    }
+    if (valid & 1) __builtin_memcpy(p + (valid & 6), raw.d, sizeof(T));
 }
 
 // v rounded to T and back: what a reader of the stored value sees.
 template <typename T>
 __device__ __forceinline__ void round_unit(float (&v)[UNIT])
 {
+    RawUnit<T> raw;
+    raw.set(v);
 #pragma unroll
-    for (int j = 0; j < UNIT; ++j) v[j] = (float)(T)v[j];
+    for (int j = 0; j < UNIT; ++j) v[j] = raw[j];
 }
 
-__device__ __forceinline__ uint32_t load_codes4(const uint8_t* __restrict__ p, int valid)
+// The same of codes.
+__device__ __forceinline__ uint2 load_codes(const uint8_t* __restrict__ p, int c, int valid)
 {
-    uint32_t c = 0;
-    if (valid >= 4)
-    {
-        __builtin_memcpy(&c, p, 4);
-    }
-    else
-    {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (j < valid) c |= (uint32_t)p[j] << (8 * j);
-    }
-    return c;
-}
-
-__device__ __forceinline__ uint2 load_codes(const uint8_t* __restrict__ p, int valid)
-{
-    uint2 c;
+    uint64_t q = 0;
     if (valid >= UNIT)
-        __builtin_memcpy(&c, p, sizeof(c));
+    {
+        __builtin_memcpy(&q, p, sizeof(q));
+    }
+    else if (valid > 0 && c > 0)
+    {
+        __builtin_memcpy(&q, p - (UNIT - valid), sizeof(q));
+        q >>= 8 * (UNIT - valid);
+    }
     else
-        c = make_uint2(load_codes4(p, valid), load_codes4(p + 4, valid - 4));
-    return c;
+    {
+#pragma unroll
+        for (int j = 0; j < UNIT - 1; ++j)
+            if (j < valid) q |= (uint64_t)p[j] << (8 * j);
+    }
+    return make_uint2((uint32_t)q, (uint32_t)(q >> 32));
 }
 
 __device__ __forceinline__ void store_codes(uint8_t* __restrict__ p, int valid, uint2 c)
@@ -106,13 +191,20 @@ __device__ __forceinline__ void store_codes(uint8_t* __restrict__ p, int valid, 
     if (valid >= UNIT)
     {
         __builtin_memcpy(p, &c, sizeof(c));
+        return;
     }
-    else
+    uint32_t w = c.x;
+    if (valid & 4)
     {
-#pragma unroll
-        for (int j = 0; j < UNIT; ++j)
-            if (j < valid) p[j] = (uint8_t)((j < 4 ? c.x : c.y) >> (8 * (j % 4)));
+        __builtin_memcpy(p, &w, 4);
+        w = c.y;
     }
+    if (valid & 2)
+    {
+        __builtin_memcpy(p + (valid & 4), &w, 2);
+        w >>= 16;
+    }
+    if (valid & 1) p[valid & 6] = (uint8_t)w;
 }
 
 __device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }

@@ -46,7 +46,7 @@ __global__ __launch_bounds__(BLOCK) void pack8_kernel(const T* __restrict__ x, i
     {
         const int c = unit * UNIT, valid = cols - c;
         float v[UNIT];
-        load_unit(x + row * xs + c, valid, v);
+        load_unit(x + row * xs + c, c, valid, v);
         store_packed(codes + row * cols, scales + row * nb, unit, valid, v);
     }
 }
@@ -73,7 +73,7 @@ __global__ __launch_bounds__(BLOCK) void unpack8_kernel(const uint8_t* __restric
         const int c = unit * UNIT, valid = cols - c;
         if (valid <= 0) continue;
         float v[UNIT];
-        unpack_unit(load_codes(codes + row * cols + c, valid), scale_of(scales[row * nb + unit / MX_LANES]), v);
+        unpack_unit(load_codes(codes + row * cols + c, c, valid), scale_of(scales[row * nb + unit / MX_LANES]), v);
         saturate_unit<T>(v);
         store_unit(out + row * cols + c, valid, v);
     }
@@ -98,13 +98,13 @@ __global__ __launch_bounds__(BLOCK) void gated_silu_fwd_kernel(const T* __restri
     {
         const int c = unit * UNIT, valid = cols - c;
         float g[UNIT], u[UNIT], v[UNIT];
-        load_unit(gate + row * gs + c, valid, g);
-        load_unit(up + row * us + c, valid, u);
+        load_unit(gate + row * gs + c, c, valid, g);
+        load_unit(up + row * us + c, c, valid, u);
         if (g8.codes) store_packed(g8.codes + row * cols, g8.scales + row * nb, unit, valid, g);
         if (u8.codes) store_packed(u8.codes + row * cols, u8.scales + row * nb, unit, valid, u);
 #pragma unroll
         for (int j = 0; j < UNIT; ++j) v[j] = g[j] * sigmoid_of<T>(g[j]) * u[j];
-        if (valid > 0) store_unit(y + row * cols + c, valid, v);
+        store_unit(y + row * cols + c, valid, v);
         if (y8.codes)
         {
             round_unit<T>(v);  // the 8-bit form is y's, as stored
@@ -125,17 +125,17 @@ __global__ __launch_bounds__(BLOCK) void gated_silu_bwd_kernel(const T* __restri
         const int c = unit * UNIT, valid = cols - c;
         if (valid <= 0) continue;
         float d[UNIT], g[UNIT], u[UNIT];
-        load_unit(gy + row * gys + c, valid, d);
+        load_unit(gy + row * gys + c, c, valid, d);
         if constexpr (PACKED)
         {
             const int64_t at = row * cols + c, block = row * nb + unit / MX_LANES;
-            unpack_unit(load_codes(g8.codes + at, valid), scale_of(g8.scales[block]), g);
-            unpack_unit(load_codes(u8.codes + at, valid), scale_of(u8.scales[block]), u);
+            unpack_unit(load_codes(g8.codes + at, c, valid), scale_of(g8.scales[block]), g);
+            unpack_unit(load_codes(u8.codes + at, c, valid), scale_of(u8.scales[block]), u);
         }
         else
         {
-            load_unit(gate + row * gs + c, valid, g);
-            load_unit(up + row * us + c, valid, u);
+            load_unit(gate + row * gs + c, c, valid, g);
+            load_unit(up + row * us + c, c, valid, u);
         }
 #pragma unroll
         for (int j = 0; j < UNIT; ++j)

@@ -15,8 +15,8 @@
 namespace mca
 {
 
-// Rows up to this many units (32768 values) stay in registers; wider ones are read twice.
-constexpr int NORM_MAX_UNITS = 4096;
+// Rows up to this many units (16384 values) stay in registers; wider ones are read twice.
+constexpr int NORM_MAX_UNITS = 2048;
 // Workgroups of a forward launch: 8 of 256 threads on each of 256 CUs, the rest of the rows in their loop.
 constexpr int NORM_BLOCKS = 2048;
 
@@ -26,13 +26,48 @@ constexpr int norm_threads()
     return G > BLOCK ? G : BLOCK;
 }
 
+// The workgroup's row of a lane, in a scalar register where a wave has only one.
+template <int G>
+__device__ __forceinline__ int row_of_lane()
+{
+    if constexpr (G >= BLOCK) return 0;
+    if constexpr (G == WAVE) return __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+    return threadIdx.x / G;
+}
+
+template <int CTRL>
+__device__ __forceinline__ float dpp_add(float s)
+{
+    return s + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(s), CTRL, 0xf, 0xf, true));
+}
+
+// The sum over G consecutive lanes (a power of two up to the wave), in every one of them, on the vector unit.
+template <int G>
+__device__ __forceinline__ float lane_sum(float s)
+{
+    if constexpr (G > 1) s = dpp_add<0xb1>(s);   // lane ^ 1
+    if constexpr (G > 2) s = dpp_add<0x4e>(s);   // lane ^ 2
+    if constexpr (G > 4) s = dpp_add<0x141>(s);  // the other 4 of 8 (mirrored)
+    if constexpr (G > 8) s = dpp_add<0x140>(s);  // the other 8 of 16 (mirrored)
+    if constexpr (G > 16)
+    {
+        const auto t = __builtin_amdgcn_permlane16_swap(__float_as_uint(s), __float_as_uint(s), false, false);
+        s = __uint_as_float(t[0]) + __uint_as_float(t[1]);
+    }
+    if constexpr (G > 32)
+    {
+        const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(s), __float_as_uint(s), false, false);
+        s = __uint_as_float(t[0]) + __uint_as_float(t[1]);
+    }
+    return s;
+}
+
 // The sum over the G lanes of a row, in every one of them. `part` holds one value per wave, for two rows in
 // turn (`turn`), so that one barrier a row suffices.
 template <int G>
 __device__ __forceinline__ float row_sum(float s, float* part, int turn)
 {
-#pragma unroll
-    for (int d = 1; d < (G < WAVE ? G : WAVE); d *= 2) s += __shfl_xor(s, d);
+    s = lane_sum<(G < WAVE ? G : WAVE)>(s);
     if constexpr (G > WAVE)
     {
         constexpr int N = G / WAVE;
@@ -46,6 +81,25 @@ __device__ __forceinline__ float row_sum(float s, float* part, int turn)
     return s;
 }
 
+// A lane's values of a row as stored.
+template <typename T, int G, int V>
+__device__ __forceinline__ void load_row(const T* __restrict__ row, int cols, RawUnit<T> (&raw)[V])
+{
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+    {
+        const int c = (threadIdx.x % G + G * k) * UNIT;
+        load_raw(row + c, c, cols - c, raw[k]);
+    }
+}
+
+// Whether a kernel of `arrays` rows of V units loads the next row while it works on one: where their registers allow it.
+template <typename T, int V>
+constexpr bool loads_ahead(int arrays)
+{
+    return arrays * V * (int)sizeof(T) <= 24;
+}
+
 template <typename T, typename WT, int G, int V>
 __global__ __launch_bounds__(norm_threads<G>()) void rms_norm_fwd_kernel(const T* __restrict__ x, int64_t xs, const T* __restrict__ r,
                                                                          int64_t rs, const WT* __restrict__ w, float eps, T* __restrict__ y,
@@ -54,48 +108,45 @@ __global__ __launch_bounds__(norm_threads<G>()) void rms_norm_fwd_kernel(const T
                                                                          int cols)
 {
     constexpr int ROWS = norm_threads<G>() / G;
+    constexpr bool AHEAD = loads_ahead<T, V>(2);
     __shared__ float part[2 * (G > WAVE ? G / WAVE : 1)];
     const int lane = threadIdx.x % G, nb = blocks_of(cols);
     const float inv = 1.0f / (float)cols;
-    float wv[V][UNIT];
-#pragma unroll
-    for (int k = 0; k < V; ++k)
+    const int64_t step = (int64_t)gridDim.x * ROWS;
+    int64_t row = (int64_t)blockIdx.x * ROWS + row_of_lane<G>();
+    RawUnit<T> rx[V], rr[V];
+    auto load = [&](int64_t at) {
+        load_row<T, G, V>(x + at * xs, cols, rx);
+        if (r) load_row<T, G, V>(r + at * rs, cols, rr);
+    };
+    if (AHEAD && row < rows) load(row);
+    RawUnit<WT> wv[V];
+    load_row<WT, G, V>(w, cols, wv);
+    for (int turn = 0; row < rows; row += step, turn ^= 1)
     {
-        const int c = (lane + G * k) * UNIT;
-        load_unit(w + c, cols - c, wv[k]);
-    }
-    int turn = 0;
-    for (int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / G; row < rows; row += (int64_t)gridDim.x * ROWS, turn ^= 1)
-    {
+        if (!AHEAD) load(row);
         float v[V][UNIT];
         float s = 0.0f;
 #pragma unroll
         for (int k = 0; k < V; ++k)
-        {
-            const int c = (lane + G * k) * UNIT;
-            load_unit(x + row * xs + c, cols - c, v[k]);
-            if (r)
+#pragma unroll
+            for (int j = 0; j < UNIT; ++j)
             {
-                float u[UNIT];
-                load_unit(r + row * rs + c, cols - c, u);
-#pragma unroll
-                for (int j = 0; j < UNIT; ++j) v[k][j] += u[j];
+                v[k][j] = rx[k][j];
+                if (r) v[k][j] += rr[k][j];
+                s += v[k][j] * v[k][j];
             }
-        }
-#pragma unroll
-        for (int k = 0; k < V; ++k)
-#pragma unroll
-            for (int j = 0; j < UNIT; ++j) s += v[k][j] * v[k][j];
+        if (AHEAD && row + step < rows) load(row + step);
         const float q = 1.0f / sqrtf(row_sum<G>(s, part, turn) * inv + eps);
         if (rstd && lane == 0) rstd[row] = q;
 #pragma unroll
         for (int k = 0; k < V; ++k)
         {
             const int c = (lane + G * k) * UNIT, valid = cols - c;
-            if (h && valid > 0) store_unit(h + row * cols + c, valid, v[k]);
+            if (h) store_unit(h + row * cols + c, valid, v[k]);
 #pragma unroll
             for (int j = 0; j < UNIT; ++j) v[k][j] = v[k][j] * q * wv[k][j];
-            if (y && valid > 0) store_unit(y + row * cols + c, valid, v[k]);
+            if (y) store_unit(y + row * cols + c, valid, v[k]);
             if (codes)
             {
                 round_unit<T>(v[k]);  // the 8-bit form is y's, as stored
@@ -122,11 +173,11 @@ __global__ __launch_bounds__(1024) void rms_norm_fwd_wide_kernel(const T* __rest
         const T* __restrict__ rr = r ? r + row * rs : nullptr;
         auto load = [&](int unit, float(&v)[UNIT]) {
             const int c = unit * UNIT;
-            load_unit(xr + c, cols - c, v);
+            load_unit(xr + c, c, cols - c, v);
             if (rr)
             {
                 float u[UNIT];
-                load_unit(rr + c, cols - c, u);
+                load_unit(rr + c, c, cols - c, u);
 #pragma unroll
                 for (int j = 0; j < UNIT; ++j) v[j] += u[j];
             }
@@ -146,11 +197,11 @@ __global__ __launch_bounds__(1024) void rms_norm_fwd_wide_kernel(const T* __rest
             const int c = unit * UNIT, valid = cols - c;
             float v[UNIT], wv[UNIT];
             load(unit, v);
-            load_unit(w + c, valid, wv);
-            if (h && valid > 0) store_unit(h + row * cols + c, valid, v);
+            load_unit(w + c, c, valid, wv);
+            if (h) store_unit(h + row * cols + c, valid, v);
 #pragma unroll
             for (int j = 0; j < UNIT; ++j) v[j] = v[j] * q * wv[j];
-            if (y && valid > 0) store_unit(y + row * cols + c, valid, v);
+            if (y) store_unit(y + row * cols + c, valid, v);
             if (codes)
             {
                 round_unit<T>(v);
@@ -170,65 +221,54 @@ __global__ __launch_bounds__(norm_threads<G>()) void rms_norm_bwd_kernel(const T
                                                                          T* __restrict__ gx, float* __restrict__ gw_part, int64_t rows, int cols)
 {
     constexpr int THREADS = norm_threads<G>(), ROWS = THREADS / G;
+    constexpr bool AHEAD = loads_ahead<T, V>(3);
     __shared__ float part[2 * (G > WAVE ? G / WAVE : 1)];
     const int lane = threadIdx.x % G;
     const float inv = 1.0f / (float)cols;
-    float wv[V][UNIT], gw[V][UNIT];
-#pragma unroll
-    for (int k = 0; k < V; ++k)
+    const int64_t step = (int64_t)gridDim.x * ROWS;
+    int64_t row = (int64_t)blockIdx.x * ROWS + row_of_lane<G>();
+    RawUnit<T> rh[V], ry[V], rg[V];
+    float rq = 0.0f;
+    auto load = [&](int64_t at) {
+        load_row<T, G, V>(h + at * hs, cols, rh);
+        if (gy) load_row<T, G, V>(gy + at * gys, cols, ry);
+        if (gh && gx) load_row<T, G, V>(gh + at * ghs, cols, rg);
+        rq = rstd[at];
+    };
+    if (AHEAD && row < rows) load(row);
+    RawUnit<WT> wv[V];
+    load_row<WT, G, V>(w, cols, wv);
+    float gw[V][UNIT] = {};
+    for (int turn = 0; row < rows; row += step, turn ^= 1)
     {
-        const int c = (lane + G * k) * UNIT;
-        load_unit(w + c, cols - c, wv[k]);
-#pragma unroll
-        for (int j = 0; j < UNIT; ++j) gw[k][j] = 0.0f;
-    }
-    int turn = 0;
-    for (int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / G; row < rows; row += (int64_t)gridDim.x * ROWS, turn ^= 1)
-    {
-        const float q = rstd[row];
+        if (!AHEAD) load(row);
+        const float q = rq;
         float n[V][UNIT], a[V][UNIT];
         float s = 0.0f;
-#pragma unroll
-        for (int k = 0; k < V; ++k)
-        {
-            const int c = (lane + G * k) * UNIT;
-            load_unit(h + row * hs + c, cols - c, n[k]);
-            if (gy)
-            {
-                load_unit(gy + row * gys + c, cols - c, a[k]);
-            }
-            else
-            {
-#pragma unroll
-                for (int j = 0; j < UNIT; ++j) a[k][j] = 0.0f;
-            }
-        }
 #pragma unroll
         for (int k = 0; k < V; ++k)
 #pragma unroll
             for (int j = 0; j < UNIT; ++j)
             {
-                n[k][j] *= q;
-                gw[k][j] += a[k][j] * n[k][j];
-                a[k][j] *= wv[k][j];
+                const float g = gy ? ry[k][j] : 0.0f;
+                n[k][j] = rh[k][j] * q;
+                gw[k][j] += g * n[k][j];
+                a[k][j] = g * wv[k][j];
                 s += a[k][j] * n[k][j];
+                // What of grad_x needs no row sum; the rest is n's share of it.
+                a[k][j] *= q;
+                if (gh && gx) a[k][j] += rg[k][j];
             }
+        if (AHEAD && row + step < rows) load(row + step);
         if (!gx) continue;
-        const float m = row_sum<G>(s, part, turn) * inv;
+        const float m = row_sum<G>(s, part, turn) * inv * q;
 #pragma unroll
         for (int k = 0; k < V; ++k)
         {
-            const int c = (lane + G * k) * UNIT, valid = cols - c;
+            const int c = (lane + G * k) * UNIT;
 #pragma unroll
-            for (int j = 0; j < UNIT; ++j) a[k][j] = q * (a[k][j] - n[k][j] * m);
-            if (gh)
-            {
-                float u[UNIT];
-                load_unit(gh + row * ghs + c, valid, u);
-#pragma unroll
-                for (int j = 0; j < UNIT; ++j) a[k][j] += u[j];
-            }
-            if (valid > 0) store_unit(gx + row * cols + c, valid, a[k]);
+            for (int j = 0; j < UNIT; ++j) a[k][j] -= n[k][j] * m;
+            store_unit(gx + row * cols + c, cols - c, a[k]);
         }
     }
     if (!gw_part) return;
@@ -239,7 +279,7 @@ __global__ __launch_bounds__(norm_threads<G>()) void rms_norm_bwd_kernel(const T
         for (int k = 0; k < V; ++k)
         {
             const int c = (lane + G * k) * UNIT;
-            if (c < cols) store_unit(out + c, cols - c, gw[k]);
+            store_unit(out + c, cols - c, gw[k]);
         }
     }
     else
@@ -281,9 +321,9 @@ __global__ __launch_bounds__(1024) void rms_norm_bwd_wide_kernel(const T* __rest
         auto load = [&](int unit, float(&n)[UNIT], float(&a)[UNIT]) {
             const int c = unit * UNIT;
             float wv[UNIT];
-            load_unit(h + row * hs + c, cols - c, n);
-            load_unit(gy + row * gys + c, cols - c, a);
-            load_unit(w + c, cols - c, wv);
+            load_unit(h + row * hs + c, c, cols - c, n);
+            load_unit(gy + row * gys + c, c, cols - c, a);
+            load_unit(w + c, c, cols - c, wv);
 #pragma unroll
             for (int j = 0; j < UNIT; ++j)
             {
@@ -311,7 +351,7 @@ __global__ __launch_bounds__(1024) void rms_norm_bwd_wide_kernel(const T* __rest
             if (gh)
             {
                 float u[UNIT];
-                load_unit(gh + row * ghs + c, cols - c, u);
+                load_unit(gh + row * ghs + c, c, cols - c, u);
 #pragma unroll
                 for (int j = 0; j < UNIT; ++j) a[j] += u[j];
             }
@@ -334,8 +374,8 @@ __global__ __launch_bounds__(BLOCK) void rms_norm_gw_wide_kernel(const T* __rest
     {
         const float q = rstd[row];
         float n[UNIT], a[UNIT];
-        load_unit(h + row * hs + c, cols - c, n);
-        load_unit(gy + row * gys + c, cols - c, a);
+        load_unit(h + row * hs + c, c, cols - c, n);
+        load_unit(gy + row * gys + c, c, cols - c, a);
 #pragma unroll
         for (int j = 0; j < UNIT; ++j) gw[j] += a[j] * (n[j] * q);
     }
@@ -360,8 +400,8 @@ static hipError_t norm_shape(int units, F&& f)
     MCA_NORM_SHAPE(256, 2);
     MCA_NORM_SHAPE(256, 3);
     MCA_NORM_SHAPE(256, 4);
-    MCA_NORM_SHAPE(1024, 2);
-    MCA_NORM_SHAPE(1024, 4);
+    MCA_NORM_SHAPE(512, 3);
+    MCA_NORM_SHAPE(512, 4);
 #undef MCA_NORM_SHAPE
     return hipErrorInvalidValue;
 }

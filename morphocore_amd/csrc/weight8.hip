@@ -64,19 +64,18 @@ __device__ __forceinline__ bf16x8 read_fragment(const char* tile, int m0, int c0
 
 // The bfloat16 terms of 8 values, each the leading 8 bits of what the ones before leave.
 template <typename T, int P>
-__device__ __forceinline__ void split_unit(const T (&raw)[UNIT], bf16x8 (&term)[P])
+__device__ __forceinline__ void split_unit(const RawUnit<T>& raw, bf16x8 (&term)[P])
 {
     if constexpr (P == 1)
     {
-#pragma unroll
-        for (int j = 0; j < UNIT; ++j) term[0][j] = raw[j];
+        term[0] = __builtin_bit_cast(bf16x8, raw);
     }
     else
     {
 #pragma unroll
         for (int j = 0; j < UNIT; ++j)
         {
-            float v = (float)raw[j];
+            float v = raw[j];
 #pragma unroll
             for (int i = 0; i < P; ++i)
             {
@@ -108,42 +107,41 @@ __global__ __launch_bounds__(L::THREADS) void grad_weight8_kernel(const T* __res
     const int64_t m0 = split * split_rows, m1 = m0 + split_rows < rows ? m0 + split_rows : rows;
     const bool full_cols = n0 + L::N <= out_rows && k0 + L::K <= cols;
 
-    T a[NA][UNIT];
+    RawUnit<T> a[NA];
     uint2 b[NB];
     uint32_t s[NB];
     auto load = [&](int64_t m) {
-        const bool full = full_cols && m + L::M <= m1;
+        if (full_cols && m + L::M <= m1)
+        {
+#pragma unroll
+            for (int i = 0; i < NA; ++i)
+            {
+                const int u = threadIdx.x + i * THREADS;
+                __builtin_memcpy(a[i].d, gy + (m + u / UA) * gys + n0 + u % UA * UNIT, sizeof(a[i].d));
+            }
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+            {
+                const int u = threadIdx.x + i * THREADS, c = k0 + u % UB * UNIT;
+                __builtin_memcpy(&b[i], codes + (m + u / UB) * cols + c, sizeof(b[i]));
+                s[i] = scales[(m + u / UB) * nb + c / MX_BLOCK];
+            }
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < NA; ++i)
         {
             const int u = threadIdx.x + i * THREADS, c = n0 + u % UA * UNIT;
             const int64_t row = m + u / UA;
-            const T* __restrict__ p = gy + row * gys + c;
-            if (full)
-            {
-                __builtin_memcpy(a[i], p, sizeof(a[i]));
-            }
-            else
-            {
-                const int valid = row < m1 ? out_rows - c : 0;
-                if (valid >= UNIT)
-                {
-                    __builtin_memcpy(a[i], p, sizeof(a[i]));
-                }
-                else
-                {
-#pragma unroll
-                    for (int j = 0; j < UNIT; ++j) a[i][j] = j < valid ? p[j] : T(0);
-                }
-            }
+            load_raw(gy + row * gys + c, c, row < m1 ? out_rows - c : 0, a[i]);
         }
 #pragma unroll
         for (int i = 0; i < NB; ++i)
         {
             const int u = threadIdx.x + i * THREADS, c = k0 + u % UB * UNIT;
             const int64_t row = m + u / UB;
-            const int valid = full ? UNIT : row < m1 ? cols - c : 0;
-            b[i] = load_codes(codes + row * cols + c, valid);
+            const int valid = row < m1 ? cols - c : 0;
+            b[i] = load_codes(codes + row * cols + c, c, valid);
             s[i] = valid > 0 ? scales[row * nb + c / MX_BLOCK] : 127;
         }
     };
@@ -305,42 +303,52 @@ hipError_t grad_weight8(const T* grad_y, int64_t gy_stride, const uint8_t* codes
     return sum_slots_async<OT>((const float*)workspace, p.splits, (int64_t)out * cols, grad_weight, stream);
 }
 
-// Q threads a group of 4 columns, each summing every Q-th slot; their sums are added in thread order.
+// Q threads a group of 4 columns, each summing every Q-th slot, 8 loads in flight; their sums are added in
+// thread order.
 template <typename OT, int Q>
 __global__ __launch_bounds__(BLOCK) void sum_slots_kernel(const float* __restrict__ part, int nslots, int64_t n, OT* __restrict__ out)
 {
-    constexpr int GROUPS = BLOCK / Q;
+    constexpr int GROUPS = BLOCK / Q, U = 8;
     __shared__ Acc sums[Q][GROUPS][4];
     const int g = threadIdx.x % GROUPS, q = threadIdx.x / GROUPS;
     const int64_t j = ((int64_t)blockIdx.x * GROUPS + g) * 4;
     Acc s[4] = {};
     if (j < n)
-        for (int b = q; b < nslots; b += Q)
+        for (int b = q; b < nslots; b += U * Q)
         {
-            const float* __restrict__ p = part + (int64_t)b * n + j;
-            float v[4];
-            if (j + 4 <= n)
-            {
-                __builtin_memcpy(v, p, sizeof(v));
-            }
-            else
-            {
+            float v[U][4];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) v[k] = j + k < n ? p[k] : 0.0f;
+            for (int u = 0; u < U; ++u)
+            {
+                const float* __restrict__ p = part + (int64_t)min(b + u * Q, nslots - 1) * n + j;
+                if (j + 4 <= n)
+                {
+                    __builtin_memcpy(v[u], p, sizeof(v[u]));
+                }
+                else
+                {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) v[u][k] = j + k < n ? p[k] : 0.0f;
+                }
             }
 #pragma unroll
-            for (int k = 0; k < 4; ++k) s[k] += (Acc)v[k];
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) s[k] += b + u * Q < nslots ? (Acc)v[u][k] : Acc(0);
         }
     if constexpr (Q > 1)
     {
 #pragma unroll
         for (int k = 0; k < 4; ++k) sums[q][g][k] = s[k];
         __syncthreads();
-        if (q != 0) return;
-#pragma unroll 4
-        for (int i = 1; i < Q; ++i)
+        // A thread a column.
+        const int64_t c = (int64_t)blockIdx.x * GROUPS * 4 + threadIdx.x;
+        if (threadIdx.x >= GROUPS * 4 || c >= n) return;
+        Acc t = Acc(0);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) s[k] += sums[i][g][k];
+        for (int i = 0; i < Q; ++i) t += sums[i][threadIdx.x / 4][threadIdx.x % 4];
+        out[c] = (OT)t;
+        return;
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k)
@@ -351,10 +359,13 @@ template <typename OT>
 hipError_t sum_slots_async(const float* part, int nslots, int64_t n, OT* out, hipStream_t stream)
 {
     if (n <= 0) return hipSuccess;
+    auto blocks = [&](int columns) { return (unsigned)((n + columns - 1) / columns); };
     if (nslots <= 16)
-        sum_slots_kernel<OT, 1><<<(unsigned)((n + 4 * BLOCK - 1) / (4 * BLOCK)), BLOCK, 0, stream>>>(part, nslots, n, out);
+        sum_slots_kernel<OT, 1><<<blocks(4 * BLOCK), BLOCK, 0, stream>>>(part, nslots, n, out);
+    else if (nslots <= 256)
+        sum_slots_kernel<OT, 16><<<blocks(64), BLOCK, 0, stream>>>(part, nslots, n, out);
     else
-        sum_slots_kernel<OT, 32><<<(unsigned)((n + 31) / 32), BLOCK, 0, stream>>>(part, nslots, n, out);
+        sum_slots_kernel<OT, 64><<<blocks(16), BLOCK, 0, stream>>>(part, nslots, n, out);
     return hipGetLastError();
 }
 

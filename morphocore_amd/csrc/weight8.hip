@@ -8,8 +8,8 @@
 //
 // Both operands lie with the summed axis as the slow one, so a wave reads its fragments from LDS with the
 // transposing read (ds_read_b64_tr_b16: 16 lanes read 4 rows of 16 columns and each gets a column). A row
-// of a staged tile is stored in groups of 16 columns (32 bytes), group g of row m at place g ^ (m & 3), so
-// that the 4 rows of such a read lie in different banks. Tiles are double-buffered in LDS: the next rows'
+// of a staged tile is stored in groups of 16 columns (32 bytes), whose order changes from row to row so that
+// the 4 rows of two neighbouring groups, which 32 lanes read at once, lie in different banks. Tiles are double-buffered in LDS: the next rows'
 // loads are issued before the products of the present ones and stored after them. Codes become bfloat16 on
 // the way into LDS, once for the workgroup.
 //
@@ -33,20 +33,27 @@ constexpr int planes_of()
     return std::is_same_v<T, float> ? 3 : std::is_same_v<T, _Float16> ? 2 : 1;
 }
 
-// N x K outputs of a workgroup, M rows staged at a time, waves along N and K.
-template <int N_, int K_, int M_, int WN_, int WK_>
+// N x K outputs of a workgroup, M rows staged at a time, D steps of loads in flight, waves along N and K.
+template <int N_, int K_, int M_, int D_, int WN_, int WK_>
 struct WeightTile
 {
-    static constexpr int N = N_, K = K_, M = M_, WN = WN_, WK = WK_;
+    static constexpr int N = N_, K = K_, M = M_, D = D_, WN = WN_, WK = WK_;
     static constexpr int THREADS = WN * WK * WAVE;
     static constexpr int FN = N / WN / 32, FK = K / WK / 32;  // 32 x 32 fragments of a wave
 };
+
+// The place of column group g (of 16) in row m of a staged tile of C columns.
+template <int C>
+__device__ __forceinline__ int group_place(int g, int m)
+{
+    return C >= 128 ? g ^ (2 * (m & 3)) : g ^ (m & 2);
+}
 
 // Byte of column c (a multiple of 8) of row m in a staged tile of C columns.
 template <int C>
 __device__ __forceinline__ int tile_byte(int m, int c)
 {
-    return m * (C * 2) + (((c / 16) ^ (m & 3)) * 32) + (c & 8) * 2;
+    return m * (C * 2) + group_place<C>(c / 16, m) * 32 + (c & 8) * 2;
 }
 
 // A lane's 8 values of the summed axis (rows m0 + 8 (lane / 32) ..) for column c0 + lane % 32.
@@ -54,7 +61,7 @@ template <int C>
 __device__ __forceinline__ bf16x8 read_fragment(const char* tile, int m0, int c0)
 {
     const int l = threadIdx.x % WAVE, r = (l / 4) & 3;
-    const int group = (c0 / 16 + ((l / 16) & 1)) ^ r;
+    const int group = group_place<C>(c0 / 16 + ((l / 16) & 1), r);
     const char* p = tile + (m0 + 8 * (l / 32) + r) * (C * 2) + group * 32 + (l & 3) * 8;
     typedef __attribute__((address_space(3))) bf16x4* lds4;
     const bf16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)p);
@@ -89,7 +96,14 @@ __device__ __forceinline__ void split_unit(const RawUnit<T>& raw, bf16x8 (&term)
 }
 
 // One tile of the sums over rows [m0, m1), m0 = split * split_rows, to out + split * out_rows * cols.
-template <typename T, typename OT, typename L>
+//
+// Every load is made, of an address within the arrays: rows past m1 read row m1 - 1 (grad_y's then count
+// as 0; a value of that row that is not finite has already made its column so), and the last tile of an
+// axis is moved back to end with it, its repeated outputs left to the tile before. What no tile covers
+// whole (fewer columns than a tile's, packed columns that are no multiple of 8) reads the row's last 8
+// values for a partial unit and moves them down; columns past the end hold anything, since they only
+// reach outputs that are not stored. ANY: arrays of fewer than 8 columns, read value by value.
+template <typename T, typename OT, typename L, bool ANY>
 __global__ __launch_bounds__(L::THREADS) void grad_weight8_kernel(const T* __restrict__ gy, int64_t gys, const uint8_t* __restrict__ codes,
                                                                   const uint8_t* __restrict__ scales, OT* __restrict__ out, int64_t rows,
                                                                   int64_t split_rows, int out_rows, int cols, int tiles_n, int tiles_k)
@@ -103,55 +117,81 @@ __global__ __launch_bounds__(L::THREADS) void grad_weight8_kernel(const T* __res
 
     const int tiles = tiles_n * tiles_k, work = xcd_work_index(blockIdx.x, gridDim.x);
     const int split = work / tiles, tile = work % tiles;
-    const int n0 = tile / tiles_k * L::N, k0 = tile % tiles_k * L::K, nb = blocks_of(cols);
-    const int64_t m0 = split * split_rows, m1 = m0 + split_rows < rows ? m0 + split_rows : rows;
-    const bool full_cols = n0 + L::N <= out_rows && k0 + L::K <= cols;
+    const int first_n = tile / tiles_k * L::N, first_k = tile % tiles_k * L::K, nb = blocks_of(cols);
+    const int n0 = max(0, min(first_n, out_rows - L::N)), k0 = max(0, min(first_k, units_of(cols) * UNIT - L::K));
+    const int64_t m0 = split * split_rows;
+    const int mrows = (int)((m0 + split_rows < rows ? m0 + split_rows : rows) - m0);
+    const T* __restrict__ gy0 = gy + m0 * gys;
+    const uint8_t* __restrict__ codes0 = codes + m0 * cols;
+    const uint8_t* __restrict__ scales0 = scales + m0 * nb;
+    const bool part_n = out_rows < L::N, part_k = k0 + L::K > cols;
 
-    RawUnit<T> a[NA];
-    uint2 b[NB];
-    uint32_t s[NB];
-    auto load = [&](int64_t m) {
-        if (full_cols && m + L::M <= m1)
+    struct Stage
+    {
+        RawUnit<T> a[NA];
+        uint2 b[NB];
+        uint32_t s[NB];
+    };
+    // Whole steps: a thread's units lie in one column, STEP_A (STEP_B) rows apart.
+    constexpr int STEP_A = THREADS / UA, STEP_B = THREADS / UB;
+    static_assert(STEP_A * UA == THREADS && STEP_B * UB == THREADS);
+    const T* __restrict__ pa = gy0 + (int64_t)(threadIdx.x / UA) * gys + min(n0 + (int)threadIdx.x % UA * UNIT, out_rows - UNIT);
+    const int col_b = k0 + (int)threadIdx.x % UB * UNIT;
+    const uint8_t* __restrict__ pb = codes0 + (int64_t)(threadIdx.x / UB) * cols + min(col_b, cols - UNIT);
+    const uint8_t* __restrict__ ps = scales0 + (int64_t)(threadIdx.x / UB) * nb + min(col_b / MX_BLOCK, nb - 1);
+    auto load = [&](auto whole, int m, Stage& st) {
+        if (decltype(whole)::value || (!ANY && m + L::M <= mrows))
         {
+            const T* __restrict__ a = pa + m * gys;
+            const uint8_t* __restrict__ b = pb + (int64_t)m * cols;
+            const uint8_t* __restrict__ s = ps + (int64_t)m * nb;
 #pragma unroll
-            for (int i = 0; i < NA; ++i)
-            {
-                const int u = threadIdx.x + i * THREADS;
-                __builtin_memcpy(a[i].d, gy + (m + u / UA) * gys + n0 + u % UA * UNIT, sizeof(a[i].d));
-            }
+            for (int i = 0; i < NA; ++i) __builtin_memcpy(st.a[i].d, a + (int64_t)(i * STEP_A) * gys, sizeof(st.a[i].d));
 #pragma unroll
             for (int i = 0; i < NB; ++i)
             {
-                const int u = threadIdx.x + i * THREADS, c = k0 + u % UB * UNIT;
-                __builtin_memcpy(&b[i], codes + (m + u / UB) * cols + c, sizeof(b[i]));
-                s[i] = scales[(m + u / UB) * nb + c / MX_BLOCK];
+                __builtin_memcpy(&st.b[i], b + (int64_t)(i * STEP_B) * cols, sizeof(st.b[i]));
+                st.s[i] = s[(int64_t)(i * STEP_B) * nb];
             }
             return;
         }
 #pragma unroll
         for (int i = 0; i < NA; ++i)
         {
-            const int u = threadIdx.x + i * THREADS, c = n0 + u % UA * UNIT;
-            const int64_t row = m + u / UA;
-            load_raw(gy + row * gys + c, c, row < m1 ? out_rows - c : 0, a[i]);
+            const int u = threadIdx.x + i * THREADS, c = n0 + u % UA * UNIT, row = min(m + u / UA, mrows - 1);
+            if constexpr (ANY)
+                load_raw(gy0 + row * gys + c, c, out_rows - c, st.a[i]);
+            else
+                __builtin_memcpy(st.a[i].d, gy0 + row * gys + min(c, out_rows - UNIT), sizeof(st.a[i].d));
         }
 #pragma unroll
         for (int i = 0; i < NB; ++i)
         {
             const int u = threadIdx.x + i * THREADS, c = k0 + u % UB * UNIT;
-            const int64_t row = m + u / UB;
-            const int valid = row < m1 ? cols - c : 0;
-            b[i] = load_codes(codes + row * cols + c, c, valid);
-            s[i] = valid > 0 ? scales[row * nb + c / MX_BLOCK] : 127;
+            const int64_t row = min(m + u / UB, mrows - 1);
+            if constexpr (ANY)
+                st.b[i] = load_codes(codes0 + row * cols + c, c, cols - c);
+            else
+                __builtin_memcpy(&st.b[i], codes0 + row * cols + min(c, cols - UNIT), sizeof(st.b[i]));
+            st.s[i] = scales0[row * nb + min(c / MX_BLOCK, nb - 1)];
         }
     };
-    auto store = [&](char* buffer) {
+    // whole: rows and columns are all there.
+    auto store = [&](auto whole, int m, Stage& st, char* buffer) {
+        constexpr bool WHOLE = decltype(whole)::value;
 #pragma unroll
         for (int i = 0; i < NA; ++i)
         {
             const int u = threadIdx.x + i * THREADS;
+            RawUnit<T>& raw = st.a[i];
+            if (!WHOLE && !ANY && part_n) raw.shift(min(max(n0 + u % UA * UNIT - (out_rows - UNIT), 0), UNIT - 1));
+            if (!WHOLE && m + L::M > mrows)
+            {
+#pragma unroll
+                for (int j = 0; j < RawUnit<T>::DWORDS; ++j) raw.d[j] = m + u / UA < mrows ? raw.d[j] : 0;
+            }
             bf16x8 term[P];
-            split_unit<T, P>(a[i], term);
+            split_unit<T, P>(raw, term);
 #pragma unroll
             for (int q = 0; q < P; ++q) *(bf16x8*)(buffer + q * A_BYTES + tile_byte<L::N>(u / UA, u % UA * UNIT)) = term[q];
         }
@@ -159,12 +199,14 @@ __global__ __launch_bounds__(L::THREADS) void grad_weight8_kernel(const T* __res
         for (int i = 0; i < NB; ++i)
         {
             const int u = threadIdx.x + i * THREADS;
-            const float scale = scale_of(s[i]);
+            const float scale = scale_of(st.s[i]);
+            uint64_t q = (uint64_t)st.b[i].y << 32 | st.b[i].x;
+            if (!WHOLE && !ANY && part_k) q >>= 8 * min(max(k0 + u % UB * UNIT - (cols - UNIT), 0), UNIT - 1);
             typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-            const bf16x2 v0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b[i].x, scale, false);
-            const bf16x2 v1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b[i].x, scale, true);
-            const bf16x2 v2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b[i].y, scale, false);
-            const bf16x2 v3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b[i].y, scale, true);
+            const bf16x2 v0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)q, scale, false);
+            const bf16x2 v1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)q, scale, true);
+            const bf16x2 v2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)(q >> 32), scale, false);
+            const bf16x2 v3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)(q >> 32), scale, true);
             const bf16x8 v = {v0[0], v0[1], v1[0], v1[1], v2[0], v2[1], v3[0], v3[1]};
             *(bf16x8*)(buffer + P * A_BYTES + tile_byte<L::K>(u / UB, u % UB * UNIT)) = v;
         }
@@ -175,36 +217,76 @@ __global__ __launch_bounds__(L::THREADS) void grad_weight8_kernel(const T* __res
     // ones does not swallow them.
     constexpr int SUMS = P == 3 ? 2 : 1;
     f32x16 acc[SUMS][L::FN][L::FK] = {};
-    load(m0);
-    store(lds[0]);
-    __syncthreads();
-    int turn = 0;
-    for (int64_t m = m0; m < m1; m += L::M, turn ^= 1)
-    {
-        const bool more = m + L::M < m1;
-        if (more) load(m + L::M);
-        const char* buffer = lds[turn];
+    auto products = [&](const char* buffer) {
+        // The fragments of the next 16 rows (and the next term) are read while the present ones are multiplied.
+        constexpr int S = L::M / 16 * P;  // sets of A fragments, small terms first
+        bf16x8 fa[2][L::FN], fb[2][L::FK];
+        auto read = [&](int t) {
+            const int i = t / P * 16, q = P - 1 - t % P;
+            if (t % P == 0)
 #pragma unroll
-        for (int i = 0; i < L::M; i += 16)
+                for (int k = 0; k < L::FK; ++k) fb[t / P % 2][k] = read_fragment<L::K>(buffer + P * A_BYTES, i, wk + 32 * k);
+#pragma unroll
+            for (int n = 0; n < L::FN; ++n) fa[t % 2][n] = read_fragment<L::N>(buffer + q * A_BYTES, i, wn + 32 * n);
+        };
+        read(0);
+#pragma unroll
+        for (int t = 0; t < S; ++t)
         {
-            bf16x8 fb[L::FK];
+            if (t + 1 < S) read(t + 1);
+            const int sum = t % P < P - 1 ? SUMS - 1 : 0;
 #pragma unroll
-            for (int k = 0; k < L::FK; ++k) fb[k] = read_fragment<L::K>(buffer + P * A_BYTES, i, wk + 32 * k);
+            for (int n = 0; n < L::FN; ++n)
 #pragma unroll
-            for (int q = P - 1; q >= 0; --q)  // small terms first
+                for (int k = 0; k < L::FK; ++k)
+                    acc[sum][n][k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[t % 2][n], fb[t / P % 2][k], acc[sum][n][k], 0, 0, 0);
+            // Two reads to a product, so that neither unit waits for the other's burst.
+            if (t + 1 < S)
             {
-                bf16x8 fa[L::FN];
 #pragma unroll
-                for (int n = 0; n < L::FN; ++n) fa[n] = read_fragment<L::N>(buffer + q * A_BYTES, i, wn + 32 * n);
-#pragma unroll
-                for (int n = 0; n < L::FN; ++n)
-#pragma unroll
-                    for (int k = 0; k < L::FK; ++k) acc[q ? SUMS - 1 : 0][n][k] =
-                            __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[n], fb[k], acc[q ? SUMS - 1 : 0][n][k], 0, 0, 0);
+                for (int g = 0; g < L::FN * L::FK; ++g)
+                {
+                    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                }
             }
         }
-        if (more) store(lds[turn ^ 1]);
-        __syncthreads();
+    };
+    // Before step m (in lds[turn]): step m + M is in st[d + 1], for the other buffer when the products are done,
+    // and st[d], which step m has left, is free for step m + D M.
+    using Whole = std::true_type;
+    using Any = std::false_type;
+    Stage st[L::D];
+#pragma unroll
+    for (int d = 0; d < L::D; ++d) load(Any(), d * L::M, st[d]);
+    store(Any(), 0, st[0], lds[0]);
+    __syncthreads();
+    int turn = 0, m = 0;
+    if (!ANY && !part_n && !part_k)
+        while (m + 2 * L::D * L::M <= mrows)  // no branch between the loads, products and stores of a step
+        {
+#pragma unroll
+            for (int d = 0; d < L::D; ++d, m += L::M, turn ^= 1)
+            {
+                load(Whole(), m + L::D * L::M, st[d]);
+                __builtin_amdgcn_sched_barrier(0);  // the loads first: the compiler would move them to their use
+                products(lds[turn]);
+                store(Whole(), m + L::M, st[(d + 1) % L::D], lds[turn ^ 1]);
+                __syncthreads();
+            }
+        }
+    while (m < mrows)
+    {
+#pragma unroll
+        for (int d = 0; d < L::D; ++d, turn ^= 1)
+        {
+            if (m + L::D * L::M < mrows) load(Any(), m + L::D * L::M, st[d]);
+            products(lds[turn]);
+            m += L::M;
+            if (m >= mrows) break;
+            store(Any(), m, st[(d + 1) % L::D], lds[turn ^ 1]);
+            __syncthreads();
+        }
     }
 
     // A lane holds column lane % 32 and rows 8 (r / 4) + 4 (lane / 32) + r % 4 of a fragment.
@@ -216,21 +298,21 @@ __global__ __launch_bounds__(L::THREADS) void grad_weight8_kernel(const T* __res
         for (int k = 0; k < L::FK; ++k)
         {
             const int col = k0 + wk + 32 * k + l % 32;
-            if (col >= cols) continue;
+            if (col < first_k || col >= cols) continue;
 #pragma unroll
             for (int r = 0; r < 16; ++r)
             {
                 const int row = n0 + wn + 32 * n + 8 * (r / 4) + 4 * (l / 32) + r % 4;
                 float v = acc[0][n][k][r];
                 if constexpr (SUMS == 2) v += acc[1][n][k][r];
-                if (row < out_rows) o[(int64_t)row * cols + col] = (OT)v;
+                if (row >= first_n && row < out_rows) o[(int64_t)row * cols + col] = (OT)v;
             }
         }
 }
 
-using WideTile = WeightTile<256, 256, 64, 2, 4>;
-using MiddleTile = WeightTile<128, 128, 32, 2, 2>;
-using SmallTile = WeightTile<64, 64, 64, 2, 2>;
+using WideTile = WeightTile<256, 256, 32, 2, 2, 4>;
+using MiddleTile = WeightTile<128, 128, 32, 3, 2, 2>;
+using SmallTile = WeightTile<64, 64, 64, 2, 2, 2>;
 
 struct WeightPlan
 {
@@ -241,17 +323,19 @@ struct WeightPlan
 
 // Rows a split sums at least: below them the joining of the splits costs more than the products.
 constexpr int SPLIT_ROWS = 512;
+// And at most, since a split counts its rows in 32 bits.
+constexpr int64_t SPLIT_MOST = 1 << 30;
 
 static WeightPlan weight_plan(int planes, int64_t rows, int out, int cols)
 {
     WeightPlan p{};
     int side = 64, step = 64;
     p.tile = 2;
-    if (out > 64 || cols > 64) p.tile = 1, side = 128, step = 32;
+    if ((out > 64 || cols > 64) && out >= UNIT && cols >= UNIT) p.tile = 1, side = 128, step = 32;
     if (planes == 1 && out > 128 && cols > 128)
     {
         const int64_t wide = (int64_t)((out + 255) / 256) * ((cols + 255) / 256) * ((rows + SPLIT_ROWS - 1) / SPLIT_ROWS);
-        if (wide >= 256) p.tile = 0, side = 256, step = 64;
+        if (wide >= 256) p.tile = 0, side = 256, step = 32;
     }
     p.tiles_n = (out + side - 1) / side;
     p.tiles_k = (cols + side - 1) / side;
@@ -261,6 +345,7 @@ static WeightPlan weight_plan(int planes, int64_t rows, int out, int cols)
     splits = splits < 1 ? 1 : splits;
     splits = splits < most ? splits : most;
     p.split_rows = ((rows + splits - 1) / splits + step - 1) / step * step;
+    if (p.split_rows > SPLIT_MOST) p.split_rows = SPLIT_MOST;
     p.splits = (int)((rows + p.split_rows - 1) / p.split_rows);
     return p;
 }
@@ -278,15 +363,16 @@ static hipError_t weight_launch(const WeightPlan& p, const T* gy, int64_t gys, c
                                 int out_rows, int cols, hipStream_t stream)
 {
     const unsigned grid = (unsigned)((int64_t)p.tiles_n * p.tiles_k * p.splits);
-    auto run = [&](auto tile) {
+    auto run = [&](auto tile, auto any) {
         using L = decltype(tile);
-        grad_weight8_kernel<T, OT, L><<<grid, L::THREADS, 0, stream>>>(gy, gys, codes, scales, out, rows, p.split_rows, out_rows, cols, p.tiles_n,
-                                                                       p.tiles_k);
+        grad_weight8_kernel<T, OT, L, decltype(any)::value>
+            <<<grid, L::THREADS, 0, stream>>>(gy, gys, codes, scales, out, rows, p.split_rows, out_rows, cols, p.tiles_n, p.tiles_k);
         return hipGetLastError();
     };
+    if (out_rows < UNIT || cols < UNIT) return run(SmallTile(), std::true_type());
     if constexpr (planes_of<T>() == 1)
-        if (p.tile == 0) return run(WideTile());
-    return p.tile == 1 ? run(MiddleTile()) : run(SmallTile());
+        if (p.tile == 0) return run(WideTile(), std::false_type());
+    return p.tile == 1 ? run(MiddleTile(), std::false_type()) : run(SmallTile(), std::false_type());
 }
 
 template <typename T, typename OT>

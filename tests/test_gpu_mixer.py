@@ -306,7 +306,7 @@ def test_gated_slices():
 # ------------------------------------------------------------------------------------------------
 
 WEIGHTS = [(1, 1, 1), (1, 64, 64), (31, 5, 33), (32, 64, 32), (100, 64, 64), (257, 100, 31), (300, 33, 257), (511, 129, 130), (1000, 256, 300),
-           (5003, 70, 65), (8200, 1000, 1030), (33000, 300, 500), (4096, 128, 512), (777, 513, 40), (64, 300, 1000), (20000, 16, 24)]
+           (5003, 70, 65), (8200, 1000, 1030), (33000, 300, 500), (4096, 128, 512), (777, 513, 40), (64, 300, 1000), (20000, 16, 24), (300, 9, 301), (300, 301, 9), (50, 8, 8), (70, 7, 200), (70, 200, 7), (9, 200, 250)]
 
 
 @pytest.mark.parametrize("rows,out,cols", WEIGHTS)

@@ -17,8 +17,8 @@ namespace mca
 
 // Rows up to this many units (16384 values) stay in registers; wider ones are read twice.
 constexpr int NORM_MAX_UNITS = 2048;
-// Workgroups of a forward launch: 8 of 256 threads on each of 256 CUs, the rest of the rows in their loop.
-constexpr int NORM_BLOCKS = 2048;
+// Workgroups of a forward launch; the rest of the rows in their loop, which reads the weight once.
+constexpr int NORM_BLOCKS = 4096;
 
 template <int G>
 constexpr int norm_threads()
@@ -93,13 +93,6 @@ __device__ __forceinline__ void load_row(const T* __restrict__ row, int cols, Ra
     }
 }
 
-// Whether a kernel of `arrays` rows of V units loads the next row while it works on one: where their registers allow it.
-template <typename T, int V>
-constexpr bool loads_ahead(int arrays)
-{
-    return arrays * V * (int)sizeof(T) <= 24;
-}
-
 template <typename T, typename WT, int G, int V>
 __global__ __launch_bounds__(norm_threads<G>()) void rms_norm_fwd_kernel(const T* __restrict__ x, int64_t xs, const T* __restrict__ r,
                                                                          int64_t rs, const WT* __restrict__ w, float eps, T* __restrict__ y,
@@ -108,23 +101,17 @@ __global__ __launch_bounds__(norm_threads<G>()) void rms_norm_fwd_kernel(const T
                                                                          int cols)
 {
     constexpr int ROWS = norm_threads<G>() / G;
-    constexpr bool AHEAD = loads_ahead<T, V>(2);
     __shared__ float part[2 * (G > WAVE ? G / WAVE : 1)];
     const int lane = threadIdx.x % G, nb = blocks_of(cols);
     const float inv = 1.0f / (float)cols;
-    const int64_t step = (int64_t)gridDim.x * ROWS;
-    int64_t row = (int64_t)blockIdx.x * ROWS + row_of_lane<G>();
-    RawUnit<T> rx[V], rr[V];
-    auto load = [&](int64_t at) {
-        load_row<T, G, V>(x + at * xs, cols, rx);
-        if (r) load_row<T, G, V>(r + at * rs, cols, rr);
-    };
-    if (AHEAD && row < rows) load(row);
     RawUnit<WT> wv[V];
     load_row<WT, G, V>(w, cols, wv);
-    for (int turn = 0; row < rows; row += step, turn ^= 1)
+    int turn = 0;
+    for (int64_t row = (int64_t)blockIdx.x * ROWS + row_of_lane<G>(); row < rows; row += (int64_t)gridDim.x * ROWS, turn ^= 1)
     {
-        if (!AHEAD) load(row);
+        RawUnit<T> rx[V], rr[V];
+        load_row<T, G, V>(x + row * xs, cols, rx);
+        if (r) load_row<T, G, V>(r + row * rs, cols, rr);
         float v[V][UNIT];
         float s = 0.0f;
 #pragma unroll
@@ -136,7 +123,6 @@ __global__ __launch_bounds__(norm_threads<G>()) void rms_norm_fwd_kernel(const T
                 if (r) v[k][j] += rr[k][j];
                 s += v[k][j] * v[k][j];
             }
-        if (AHEAD && row + step < rows) load(row + step);
         const float q = 1.0f / sqrtf(row_sum<G>(s, part, turn) * inv + eps);
         if (rstd && lane == 0) rstd[row] = q;
 #pragma unroll
@@ -221,28 +207,20 @@ __global__ __launch_bounds__(norm_threads<G>()) void rms_norm_bwd_kernel(const T
                                                                          T* __restrict__ gx, float* __restrict__ gw_part, int64_t rows, int cols)
 {
     constexpr int THREADS = norm_threads<G>(), ROWS = THREADS / G;
-    constexpr bool AHEAD = loads_ahead<T, V>(3);
     __shared__ float part[2 * (G > WAVE ? G / WAVE : 1)];
     const int lane = threadIdx.x % G;
     const float inv = 1.0f / (float)cols;
-    const int64_t step = (int64_t)gridDim.x * ROWS;
-    int64_t row = (int64_t)blockIdx.x * ROWS + row_of_lane<G>();
-    RawUnit<T> rh[V], ry[V], rg[V];
-    float rq = 0.0f;
-    auto load = [&](int64_t at) {
-        load_row<T, G, V>(h + at * hs, cols, rh);
-        if (gy) load_row<T, G, V>(gy + at * gys, cols, ry);
-        if (gh && gx) load_row<T, G, V>(gh + at * ghs, cols, rg);
-        rq = rstd[at];
-    };
-    if (AHEAD && row < rows) load(row);
     RawUnit<WT> wv[V];
     load_row<WT, G, V>(w, cols, wv);
     float gw[V][UNIT] = {};
-    for (int turn = 0; row < rows; row += step, turn ^= 1)
+    int turn = 0;
+    for (int64_t row = (int64_t)blockIdx.x * ROWS + row_of_lane<G>(); row < rows; row += (int64_t)gridDim.x * ROWS, turn ^= 1)
     {
-        if (!AHEAD) load(row);
-        const float q = rq;
+        RawUnit<T> rh[V], ry[V], rg[V];
+        load_row<T, G, V>(h + row * hs, cols, rh);
+        if (gy) load_row<T, G, V>(gy + row * gys, cols, ry);
+        if (gh && gx) load_row<T, G, V>(gh + row * ghs, cols, rg);
+        const float q = rstd[row];
         float n[V][UNIT], a[V][UNIT];
         float s = 0.0f;
 #pragma unroll
@@ -259,7 +237,6 @@ __global__ __launch_bounds__(norm_threads<G>()) void rms_norm_bwd_kernel(const T
                 a[k][j] *= q;
                 if (gh && gx) a[k][j] += rg[k][j];
             }
-        if (AHEAD && row + step < rows) load(row + step);
         if (!gx) continue;
         const float m = row_sum<G>(s, part, turn) * inv * q;
 #pragma unroll
@@ -432,14 +409,21 @@ hipError_t rms_norm_forward(const T* x, int64_t x_stride, const T* residual, int
     });
 }
 
-// Slots of grad_w's partial sums: workgroups of a backward launch. Two workgroups a CU keep enough loads in
-// flight for wide rows, whose slots cost `cols` values each; narrow rows take more.
+// Slots of grad_w's partial sums, one a workgroup of the backward: the workgroups that the 256 CUs hold at once by
+// their registers (units a lane: 1, 2, 3 or more). Fewer leave loads unissued, more leave a last round half
+// empty and make more slots to add (8192 x 4096 bfloat16: 58 us with 1024, 70 with 512; 2048 x 8192: 48 with
+// 1024, 39 with 512; both with the slots' sum).
 static int norm_slots(int64_t rows, int cols)
 {
     const int units = units_of(cols);
     if (units > NORM_MAX_UNITS) return norm_grid(rows, 16, 64);
-    const int per = units > 64 * 4 ? 1 : BLOCK / (units > 32 ? 64 : units > 16 ? 32 : units > 8 ? 16 : units > 4 ? 8 : 4);
-    return norm_grid(rows, per, units > 64 ? 512 : 1024);
+    int slots = 0;
+    (void)norm_shape(units, [&](auto g, auto v) {
+        constexpr int G = decltype(g)::value, V = decltype(v)::value;
+        slots = norm_grid(rows, norm_threads<G>() / G, G > BLOCK ? 256 : V >= 3 ? 512 : V == 1 && G == WAVE ? 1536 : 1024);
+        return hipSuccess;
+    });
+    return slots;
 }
 
 size_t rms_norm_backward_workspace(int64_t rows, int cols)

@@ -328,10 +328,29 @@ Gated gated_rows(const Tensor& gate, const Tensor& up)
     return g;
 }
 
+// gate's and up's 8-bit form in one buffer, which the backward alone reads: gate's codes, up's, gate's scales, up's.
+struct Kept
+{
+    Tensor buffer;
+    int64_t values, blocks;
+
+    uint8_t* at(int64_t offset) const { return buffer.defined() ? (uint8_t*)buffer.data_ptr() + offset : nullptr; }
+    uint8_t* gate_codes() const { return at(0); }
+    uint8_t* up_codes() const { return at(values); }
+    uint8_t* gate_scales() const { return at(2 * values); }
+    uint8_t* up_scales() const { return at(2 * values + blocks); }
+};
+
+Kept kept_of(int64_t rows, int64_t cols)
+{
+    return Kept{Tensor(), rows * cols, rows * ((cols + PACK_BLOCK - 1) / PACK_BLOCK)};
+}
+
 struct GatedOut
 {
     Tensor y;
-    Packed gate, up, packed;
+    Kept kept;
+    Packed packed;
 };
 
 GatedOut gated_forward(const Tensor& gate, const Tensor& up, bool keep8, bool pack)
@@ -340,14 +359,12 @@ GatedOut gated_forward(const Tensor& gate, const Tensor& up, bool keep8, bool pa
     const Gated g = gated_rows(gate, up);
     GatedOut o;
     o.y = torch::empty(g.shape, gate.options());
-    if (keep8)
-    {
-        o.gate = new_packed(g.shape, gate);
-        o.up = new_packed(g.shape, gate);
-    }
+    o.kept = kept_of(g.gate.rows, g.cols);
+    if (keep8) o.kept.buffer = torch::empty({2 * (o.kept.values + o.kept.blocks)}, gate.options().dtype(torch::kUInt8));
     if (pack) o.packed = new_packed(g.shape, gate);
-    check_rc(mca_gated_silu_forward(type_code("gated_silu", gate), g.gate.data(), g.gate.stride, g.up, g.up_stride, o.y.data_ptr(), o.gate.c(),
-                                    o.gate.s(), o.up.c(), o.up.s(), o.packed.c(), o.packed.s(), g.gate.rows, g.cols, stream_of(gate)));
+    check_rc(mca_gated_silu_forward(type_code("gated_silu", gate), g.gate.data(), g.gate.stride, g.up, g.up_stride, o.y.data_ptr(),
+                                    o.kept.gate_codes(), o.kept.gate_scales(), o.kept.up_codes(), o.kept.up_scales(), o.packed.c(), o.packed.s(),
+                                    g.gate.rows, g.cols, stream_of(gate)));
     return o;
 }
 
@@ -367,7 +384,7 @@ public:
             ctx->save_for_backward({gate, u});
             return {o.y};
         }
-        ctx->save_for_backward({o.gate.codes, o.gate.scales, o.up.codes, o.up.scales});
+        ctx->save_for_backward({o.kept.buffer});
         ctx->mark_non_differentiable({o.packed.codes, o.packed.scales});
         return {o.y, o.packed.codes, o.packed.scales};
     }
@@ -387,14 +404,14 @@ public:
         Tensor gg = torch::empty(shape, gy.options()), gu = joint ? Tensor() : torch::empty(shape, gy.options());
         void* gu_data = joint ? (void*)((char*)gg.data_ptr() + cols * gy.element_size()) : gu.data_ptr();
         Gated in{};
-        Packed p[2];
+        Kept kept = kept_of(g.rows, cols);
         if (eight)
-            p[0] = Packed{saved[0], saved[1]}, p[1] = Packed{saved[2], saved[3]};
+            kept.buffer = saved[0];
         else
             in = gated_rows(saved[0], saved[1]);
         check_rc(mca_gated_silu_backward(type_code("gated_silu", gy), g.data(), g.stride, eight ? nullptr : in.gate.data(),
-                                         eight ? 0 : in.gate.stride, eight ? nullptr : in.up, eight ? 0 : in.up_stride, p[0].c(), p[0].s(),
-                                         p[1].c(), p[1].s(), gg.data_ptr(), gu_data, shape.back(), g.rows, cols, stream_of(gy)));
+                                         eight ? 0 : in.gate.stride, eight ? nullptr : in.up, eight ? 0 : in.up_stride, kept.gate_codes(),
+                                         kept.gate_scales(), kept.up_codes(), kept.up_scales(), gg.data_ptr(), gu_data, shape.back(), g.rows, cols, stream_of(gy)));
         return {ctx->needs_input_grad(0) ? gg : Tensor(), !joint && ctx->needs_input_grad(1) ? gu : Tensor(), Tensor()};
     }
 };

@@ -124,7 +124,7 @@ __global__ __launch_bounds__(L::THREADS) void grad_weight8_kernel(const T* __res
     const T* __restrict__ gy0 = gy + m0 * gys;
     const uint8_t* __restrict__ codes0 = codes + m0 * cols;
     const uint8_t* __restrict__ scales0 = scales + m0 * nb;
-    const bool part_n = out_rows < L::N, part_k = k0 + L::K > cols;
+    const bool part_n = out_rows < L::N && out_rows % UNIT;
 
     struct Stage
     {
@@ -138,6 +138,7 @@ __global__ __launch_bounds__(L::THREADS) void grad_weight8_kernel(const T* __res
     const T* __restrict__ pa = gy0 + (int64_t)(threadIdx.x / UA) * gys + min(n0 + (int)threadIdx.x % UA * UNIT, out_rows - UNIT);
     const int col_b = k0 + (int)threadIdx.x % UB * UNIT;
     const uint8_t* __restrict__ pb = codes0 + (int64_t)(threadIdx.x / UB) * cols + min(col_b, cols - UNIT);
+    const int down_b = 8 * min(max(col_b - (cols - UNIT), 0), UNIT - 1);
     const uint8_t* __restrict__ ps = scales0 + (int64_t)(threadIdx.x / UB) * nb + min(col_b / MX_BLOCK, nb - 1);
     auto load = [&](auto whole, int m, Stage& st) {
         if (decltype(whole)::value || (!ANY && m + L::M <= mrows))
@@ -201,7 +202,7 @@ __global__ __launch_bounds__(L::THREADS) void grad_weight8_kernel(const T* __res
             const int u = threadIdx.x + i * THREADS;
             const float scale = scale_of(st.s[i]);
             uint64_t q = (uint64_t)st.b[i].y << 32 | st.b[i].x;
-            if (!WHOLE && !ANY && part_k) q >>= 8 * min(max(k0 + u % UB * UNIT - (cols - UNIT), 0), UNIT - 1);
+            if constexpr (!ANY) q >>= down_b;
             typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
             const bf16x2 v0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)q, scale, false);
             const bf16x2 v1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)q, scale, true);
@@ -262,7 +263,7 @@ __global__ __launch_bounds__(L::THREADS) void grad_weight8_kernel(const T* __res
     store(Any(), 0, st[0], lds[0]);
     __syncthreads();
     int turn = 0, m = 0;
-    if (!ANY && !part_n && !part_k)
+    if (!ANY && !part_n)
         while (m + 2 * L::D * L::M <= mrows)  // no branch between the loads, products and stores of a step
         {
 #pragma unroll

@@ -88,8 +88,14 @@ __device__ __forceinline__ void split_unit(const RawUnit<T>& raw, bf16x8 (&term)
             {
                 const uint32_t bits = __float_as_uint(v) & 0xffff0000u;
                 term[i][j] = __builtin_bit_cast(__bf16, (uint16_t)(bits >> 16));
-                // An infinity is its own first term and leaves nothing; a NaN stays one.
-                v = fabsf(v) == __builtin_inff() ? 0.0f : v - __uint_as_float(bits);
+                if (i + 1 == P) break;
+                const float rest = v - __uint_as_float(bits);
+                // An infinity is its own first term; what it leaves must be no NaN. (Of float16 the rest is at most 65504, and
+                // for the NaN that an infinity leaves the median is -65504, which the infinite products swallow.)
+                if constexpr (std::is_same_v<T, _Float16>)
+                    v = __builtin_amdgcn_fmed3f(rest, -65504.0f, 65504.0f);
+                else
+                    v = i == 0 && fabsf(v) == __builtin_inff() ? 0.0f : rest;
             }
         }
     }
@@ -331,7 +337,7 @@ struct TileCost
     double alone, shared;
 };
 constexpr TileCost TILE_COST[3][3] = {
-    {{256, 32, 1, 28.0, 28.0}, {128, 32, 2, 15.0, 9.5}, {64, 64, 4, 7.0, 4.6}},    // bfloat16
+    {{256, 32, 1, 28.0, 28.0}, {128, 32, 2, 15.0, 10.5}, {64, 64, 4, 7.0, 4.6}},    // bfloat16
     {{}, {128, 32, 2, 30.0, 17.0}, {64, 64, 3, 13.0, 7.6}},                        // float16
     {{}, {128, 32, 1, 30.0, 30.0}, {64, 64, 2, 17.0, 11.0}},                       // float32
 };

@@ -504,3 +504,48 @@ def test_checkpoint8_of_a_morphological_stack():
     want = torch.autograd.grad(stack(kept), [kept, *stack.parameters()], gy)
     # The stack's own gradient sums may differ in their order from run to run.
     assert all((a - b).norm() <= 1e-5 * b.norm() for a, b in zip(got, want))
+
+
+# ------------------------------------------------------------------------------------------------
+# Offsets past 32 bits
+# ------------------------------------------------------------------------------------------------
+
+def test_rows_past_32_bit_offsets():
+    """Arrays of more than 2^32 elements: the last rows are worked on as the same rows of a small array."""
+    rows, cols, tail = (1 << 26) + 5, 72, 300
+    x = torch.zeros(rows, cols, dtype=torch.bfloat16, device=DEV)
+    x[-tail:] = randn(1, tail, cols, dtype=torch.bfloat16)
+    small = x[-tail:].clone()
+    print("pack8 / unpack8", flush=True)
+    p, q = F.pack8(x), F.pack8(small)
+    assert torch.equal(p.codes[-tail:].view(torch.uint8), q.codes.view(torch.uint8))
+    assert torch.equal(p.scales[-tail:].view(torch.uint8), q.scales.view(torch.uint8))
+    assert torch.equal(F.unpack8(p, torch.bfloat16)[-tail:], F.unpack8(q, torch.bfloat16))
+    print("grad_weight8", flush=True)
+    # All other rows are zeros, so the sums are the small array's; the order differs.
+    g64, x64 = np64(small[:, :64]), O.unpack(q.codes.view(torch.uint8).cpu().numpy(), q.scales.view(torch.uint8).cpu().numpy())
+    got = F.grad_weight8(x[:, :64], p, torch.float32)
+    near(got, g64.T @ x64, (2 * np.sqrt(tail) + 16) * f32 * (np.abs(g64).T @ np.abs(x64)), torch.float32, "gw")
+    print("gated", flush=True)
+    assert torch.equal(F.gated_silu(x)[-tail:], F.gated_silu(small))
+    del p
+    print("rms_norm", flush=True)
+    w = torch.ones(cols, dtype=torch.bfloat16, device=DEV)
+    assert torch.equal(F.rms_norm(x, w)[-tail:], F.rms_norm(small, w))
+    del x
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_example_trains(dtype):
+    """The example's network, through every operator: its loss falls to less than half."""
+    import importlib.util
+    import os
+
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "train_mixer.py")
+    spec = importlib.util.spec_from_file_location("train_mixer", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    losses, kept = example.train(steps=40, size=32, batch=2, channels=16, dtype=dtype)
+    assert all(np.isfinite(losses)) and kept > 0
+    assert np.mean(losses[-5:]) < 0.5 * losses[0]

@@ -3,9 +3,10 @@
 // reads it:
 //   grad_g = grad_y * u * s * (1 + g * (1 - s)),  grad_u = grad_y * g * s,  s = sigmoid(g).
 //
-// Bound by HBM: one pass, 8 values a lane (16-byte accesses of 16-bit values). A workgroup's 256 lanes are
-// rows x G lanes; G, the power of two at or above the row's units, keeps the lanes of short rows busy, and a
-// row wider than G = 256 takes several workgroups (blockIdx.x), so that one row already fills many CUs.
+// Bound by HBM: one pass, 8 values a lane (16-byte accesses of 16-bit values). A workgroup's 256 lanes take as
+// many whole rows as they hold, a lane a unit (a multiple of 4 lanes a row, so that a block's lanes stay
+// together); a row of more than 256 units takes several workgroups (blockIdx.x), so that one row already
+// fills many CUs.
 #include "block8.hpp"
 #include "launch.hpp"
 #include "mixer.hpp"
@@ -16,30 +17,29 @@ namespace mca
 struct RowGrid
 {
     dim3 grid;
-    int lanes_log2;
+    int lanes;
+    int magic;  // ceil(2^16 / lanes): t / lanes = t * magic >> 16 for t < 256
 };
 
 // Rows beyond the grid are taken in the kernels' loop.
 static RowGrid row_grid(int64_t rows, int cols)
 {
-    const int units = blocks_of(cols) * MX_LANES;
-    int lg = 2;
-    while ((1 << lg) < units && lg < 8) ++lg;
-    const int64_t x = (units + (1 << lg) - 1) >> lg, per = BLOCK >> lg, y = (rows + per - 1) / per;
-    const int64_t most = 65535;
-    return RowGrid{dim3((unsigned)x, (unsigned)(y < most ? y : most)), lg};
+    const int units = blocks_of(cols) * MX_LANES, chunks = (units + BLOCK - 1) / BLOCK;
+    const int lanes = ((units + chunks - 1) / chunks + MX_LANES - 1) / MX_LANES * MX_LANES;
+    const int64_t per = BLOCK / lanes, y = (rows + per - 1) / per, most = 65535;
+    return RowGrid{dim3((unsigned)chunks, (unsigned)(y < most ? y : most)), lanes, (65535 + lanes) / lanes};
 }
 
 // The lane's unit of its row, and the loop over the rows.
-#define MCA_ROW_LOOP(unit, row)                                                                   \
-    const int unit = (int)(blockIdx.x << lanes_log2) + (int)(threadIdx.x & ((1u << lanes_log2) - 1)); \
-    if (unit >= blocks_of(cols) * MX_LANES) return;                                               \
-    const int rows_per = BLOCK >> lanes_log2;                                                     \
-    for (int64_t row = (int64_t)blockIdx.y * rows_per + (threadIdx.x >> lanes_log2); row < rows; row += (int64_t)gridDim.y * rows_per)
+#define MCA_ROW_LOOP(unit, row)                                                             \
+    const int own_row = (int)threadIdx.x * magic >> 16, rows_per = BLOCK * magic >> 16;     \
+    const int unit = (int)blockIdx.x * lanes + (int)threadIdx.x - own_row * lanes;          \
+    if (unit >= blocks_of(cols) * MX_LANES || own_row >= rows_per) return;                  \
+    for (int64_t row = (int64_t)blockIdx.y * rows_per + own_row; row < rows; row += (int64_t)gridDim.y * rows_per)
 
 template <typename T>
 __global__ __launch_bounds__(BLOCK) void pack8_kernel(const T* __restrict__ x, int64_t xs, uint8_t* __restrict__ codes,
-                                                      uint8_t* __restrict__ scales, int64_t rows, int cols, int lanes_log2)
+                                                      uint8_t* __restrict__ scales, int64_t rows, int cols, int lanes, int magic)
 {
     const int nb = blocks_of(cols);
     MCA_ROW_LOOP(unit, row)
@@ -65,7 +65,7 @@ __device__ __forceinline__ void saturate_unit(float (&v)[UNIT])
 
 template <typename T>
 __global__ __launch_bounds__(BLOCK) void unpack8_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
-                                                        T* __restrict__ out, int64_t rows, int cols, int lanes_log2)
+                                                        T* __restrict__ out, int64_t rows, int cols, int lanes, int magic)
 {
     const int nb = blocks_of(cols);
     MCA_ROW_LOOP(unit, row)
@@ -91,7 +91,7 @@ __device__ __forceinline__ float sigmoid_of(float g)
 template <typename T>
 __global__ __launch_bounds__(BLOCK) void gated_silu_fwd_kernel(const T* __restrict__ gate, int64_t gs, const T* __restrict__ up, int64_t us,
                                                                T* __restrict__ y, PackedOut g8, PackedOut u8, PackedOut y8, int64_t rows,
-                                                               int cols, int lanes_log2)
+                                                               int cols, int lanes, int magic)
 {
     const int nb = blocks_of(cols);
     MCA_ROW_LOOP(unit, row)
@@ -117,7 +117,7 @@ template <typename T, bool PACKED>
 __global__ __launch_bounds__(BLOCK) void gated_silu_bwd_kernel(const T* __restrict__ gy, int64_t gys, const T* __restrict__ gate, int64_t gs,
                                                                const T* __restrict__ up, int64_t us, PackedOut g8, PackedOut u8,
                                                                T* __restrict__ gg, T* __restrict__ gu, int64_t grad_s, int64_t rows, int cols,
-                                                               int lanes_log2)
+                                                               int lanes, int magic)
 {
     const int nb = blocks_of(cols);
     MCA_ROW_LOOP(unit, row)
@@ -154,7 +154,7 @@ hipError_t pack8(const T* x, int64_t x_stride, uint8_t* codes, uint8_t* scales, 
 {
     if (rows <= 0 || cols <= 0) return hipSuccess;
     const RowGrid g = row_grid(rows, cols);
-    pack8_kernel<T><<<g.grid, BLOCK, 0, stream>>>(x, x_stride, codes, scales, rows, cols, g.lanes_log2);
+    pack8_kernel<T><<<g.grid, BLOCK, 0, stream>>>(x, x_stride, codes, scales, rows, cols, g.lanes, g.magic);
     return hipGetLastError();
 }
 
@@ -163,7 +163,7 @@ hipError_t unpack8(const uint8_t* codes, const uint8_t* scales, T* out, int64_t 
 {
     if (rows <= 0 || cols <= 0) return hipSuccess;
     const RowGrid g = row_grid(rows, cols);
-    unpack8_kernel<T><<<g.grid, BLOCK, 0, stream>>>(codes, scales, out, rows, cols, g.lanes_log2);
+    unpack8_kernel<T><<<g.grid, BLOCK, 0, stream>>>(codes, scales, out, rows, cols, g.lanes, g.magic);
     return hipGetLastError();
 }
 
@@ -173,7 +173,7 @@ hipError_t gated_silu_forward(const T* gate, int64_t g_stride, const T* up, int6
 {
     if (rows <= 0 || cols <= 0) return hipSuccess;
     const RowGrid g = row_grid(rows, cols);
-    gated_silu_fwd_kernel<T><<<g.grid, BLOCK, 0, stream>>>(gate, g_stride, up, u_stride, y, gate8, up8, y8, rows, cols, g.lanes_log2);
+    gated_silu_fwd_kernel<T><<<g.grid, BLOCK, 0, stream>>>(gate, g_stride, up, u_stride, y, gate8, up8, y8, rows, cols, g.lanes, g.magic);
     return hipGetLastError();
 }
 
@@ -186,10 +186,10 @@ hipError_t gated_silu_backward(const T* grad_y, int64_t gy_stride, const T* gate
     const RowGrid g = row_grid(rows, cols);
     if (gate)
         gated_silu_bwd_kernel<T, false><<<g.grid, BLOCK, 0, stream>>>(grad_y, gy_stride, gate, g_stride, up, u_stride, gate8, up8, grad_gate,
-                                                                      grad_up, grad_stride, rows, cols, g.lanes_log2);
+                                                                      grad_up, grad_stride, rows, cols, g.lanes, g.magic);
     else
         gated_silu_bwd_kernel<T, true><<<g.grid, BLOCK, 0, stream>>>(grad_y, gy_stride, gate, g_stride, up, u_stride, gate8, up8, grad_gate,
-                                                                     grad_up, grad_stride, rows, cols, g.lanes_log2);
+                                                                     grad_up, grad_stride, rows, cols, g.lanes, g.magic);
     return hipGetLastError();
 }
 

@@ -20,17 +20,20 @@ constexpr int NORM_MAX_UNITS = 2048;
 // Workgroups of a forward launch; the rest of the rows in their loop, which reads the weight once.
 constexpr int NORM_BLOCKS = 4096;
 
+constexpr int NUM_CU = 256;
+
+// A workgroup has one row of more than a wave, or the rows of 4 waves.
 template <int G>
 constexpr int norm_threads()
 {
-    return G > BLOCK ? G : BLOCK;
+    return G > WAVE ? G : BLOCK;
 }
 
 // The workgroup's row of a lane, in a scalar register where a wave has only one.
 template <int G>
 __device__ __forceinline__ int row_of_lane()
 {
-    if constexpr (G >= BLOCK) return 0;
+    if constexpr (G > WAVE) return 0;
     if constexpr (G == WAVE) return __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
     return threadIdx.x / G;
 }
@@ -250,7 +253,7 @@ __global__ __launch_bounds__(norm_threads<G>()) void rms_norm_bwd_kernel(const T
     }
     if (!gw_part) return;
     float* __restrict__ out = gw_part + (int64_t)blockIdx.x * cols;
-    if constexpr (G >= BLOCK)
+    if constexpr (G > WAVE)
     {
 #pragma unroll
         for (int k = 0; k < V; ++k)
@@ -359,26 +362,32 @@ __global__ __launch_bounds__(BLOCK) void rms_norm_gw_wide_kernel(const T* __rest
     store_unit(gw_part + (int64_t)blockIdx.y * cols + c, cols - c, gw);
 }
 
-// f(G, V): lanes a row and units a lane, the narrowest that hold `units`.
+// f(G, V): lanes a row and units a lane for rows of `units`. One unit a lane leaves registers for the most waves and
+// is the fastest where it wastes few lanes (16384 x 2000 bfloat16: forward 53 us, 67 with 64 lanes of 4 units;
+// 4096 x 8000: 59 and 55 us forward and backward, 74 and 79 with 256 lanes of 4); between the powers of
+// two the shape with fewer idle lanes (12000 x 2500: forward 64 us with 256 x 2, 77 with 384 x 1; 3000 x 11000:
+// 66 with 512 x 3, 75 with 768 x 2).
 template <typename F>
 static hipError_t norm_shape(int units, F&& f)
 {
     using std::integral_constant;
-#define MCA_NORM_SHAPE(G, V) \
-    if (units <= (G) * (V)) return f(integral_constant<int, G>(), integral_constant<int, V>())
-    MCA_NORM_SHAPE(4, 1);
-    MCA_NORM_SHAPE(8, 1);
-    MCA_NORM_SHAPE(16, 1);
-    MCA_NORM_SHAPE(32, 1);
-    MCA_NORM_SHAPE(64, 1);
-    MCA_NORM_SHAPE(64, 2);
-    MCA_NORM_SHAPE(64, 3);
-    MCA_NORM_SHAPE(64, 4);
-    MCA_NORM_SHAPE(256, 2);
-    MCA_NORM_SHAPE(256, 3);
-    MCA_NORM_SHAPE(256, 4);
-    MCA_NORM_SHAPE(512, 3);
-    MCA_NORM_SHAPE(512, 4);
+#define MCA_NORM_SHAPE(MOST, G, V)                                     \
+    static_assert((MOST) <= (G) * (V));                                \
+    if (units <= (MOST)) return f(integral_constant<int, G>(), integral_constant<int, V>())
+    MCA_NORM_SHAPE(4, 4, 1);
+    MCA_NORM_SHAPE(8, 8, 1);
+    MCA_NORM_SHAPE(16, 16, 1);
+    MCA_NORM_SHAPE(32, 32, 1);
+    MCA_NORM_SHAPE(64, 64, 1);
+    MCA_NORM_SHAPE(128, 64, 2);
+    MCA_NORM_SHAPE(192, 192, 1);
+    MCA_NORM_SHAPE(256, 256, 1);
+    MCA_NORM_SHAPE(384, 256, 2);
+    MCA_NORM_SHAPE(512, 512, 1);
+    MCA_NORM_SHAPE(768, 768, 1);
+    MCA_NORM_SHAPE(1024, 1024, 1);
+    MCA_NORM_SHAPE(1536, 512, 3);
+    MCA_NORM_SHAPE(NORM_MAX_UNITS, 1024, 2);
 #undef MCA_NORM_SHAPE
     return hipErrorInvalidValue;
 }
@@ -403,16 +412,17 @@ hipError_t rms_norm_forward(const T* x, int64_t x_stride, const T* residual, int
     }
     return norm_shape(units, [&](auto g, auto v) {
         constexpr int G = decltype(g)::value, V = decltype(v)::value;
-        rms_norm_fwd_kernel<T, WT, G, V><<<norm_grid(rows, norm_threads<G>() / G, NORM_BLOCKS), norm_threads<G>(), 0, stream>>>(
+        rms_norm_fwd_kernel<T, WT, G, V><<<norm_grid(rows, norm_threads<G>() / G, NORM_BLOCKS * BLOCK / norm_threads<G>()), norm_threads<G>(), 0, stream>>>(
             x, x_stride, residual, r_stride, w, eps, y, h, codes, scales, rstd, rows, cols);
         return hipGetLastError();
     });
 }
 
-// Slots of grad_w's partial sums, one a workgroup of the backward: the workgroups that the 256 CUs hold at once by
-// their registers (units a lane: 1, 2, 3 or more). Fewer leave loads unissued, more leave a last round half
-// empty and make more slots to add (8192 x 4096 bfloat16: 58 us with 1024, 70 with 512; 2048 x 8192: 48 with
-// 1024, 39 with 512; both with the slots' sum).
+// Slots of grad_w's partial sums, one a workgroup of the backward: about as many threads as the 256 CUs hold at once by
+// their registers. Fewer leave loads unissued, more leave a last round half empty and make more slots to
+// add (8192 x 4096 bfloat16, 256 lanes of 2 units: 58 us with 1024 workgroups, 70 with 512; 2048 x 8192, 256 lanes of
+// 4: 48 with 1024, 39 with 512; both with the slots' sum). A workgroup takes two rows at least where that leaves two
+// workgroups for every CU.
 static int norm_slots(int64_t rows, int cols)
 {
     const int units = units_of(cols);
@@ -420,7 +430,9 @@ static int norm_slots(int64_t rows, int cols)
     int slots = 0;
     (void)norm_shape(units, [&](auto g, auto v) {
         constexpr int G = decltype(g)::value, V = decltype(v)::value;
-        slots = norm_grid(rows, norm_threads<G>() / G, G > BLOCK ? 256 : V >= 3 ? 512 : V == 1 && G == WAVE ? 1536 : 1024);
+        constexpr int THREADS = norm_threads<G>();
+        const int most = (V >= 3 ? 512 : V == 1 && G == WAVE ? 1536 : 1024) * BLOCK / THREADS, two = norm_grid(rows, 2 * THREADS / G, most);
+        slots = two > 2 * NUM_CU ? two : norm_grid(rows, THREADS / G, most < 2 * NUM_CU ? most : 2 * NUM_CU);
         return hipSuccess;
     });
     return slots;

@@ -420,56 +420,58 @@ hipError_t grad_weight8(const T* grad_y, int64_t gy_stride, const uint8_t* codes
     return sum_slots_async<OT>((const float*)workspace, p.splits, (int64_t)out * cols, grad_weight, stream);
 }
 
-// Q threads a group of 4 columns, each summing every Q-th slot, 8 loads in flight; their sums are added in
-// thread order.
+// Q threads a group of 4 columns, each summing every Q-th slot, 8 loads in flight without a branch between them: the
+// last group is moved back to end with the columns and leaves those before its own to its neighbour. The threads'
+// sums are added in thread order.
 template <typename OT, int Q>
 __global__ __launch_bounds__(BLOCK) void sum_slots_kernel(const float* __restrict__ part, int nslots, int64_t n, OT* __restrict__ out)
 {
-    constexpr int GROUPS = BLOCK / Q, U = 8;
-    __shared__ Acc sums[Q][GROUPS][4];
+    constexpr int GROUPS = BLOCK / Q, COLS = GROUPS * 4, U = Q > 1 ? 8 : 4;
+    __shared__ Acc sums[Q * COLS], four[Q / 4 * COLS + 1];
     const int g = threadIdx.x % GROUPS, q = threadIdx.x / GROUPS;
-    const int64_t j = ((int64_t)blockIdx.x * GROUPS + g) * 4;
+    const int64_t own = ((int64_t)blockIdx.x * GROUPS + g) * 4, j = own + 4 <= n ? own : n < 4 ? 0 : n - 4;
     Acc s[4] = {};
-    if (j < n)
-        for (int b = q; b < nslots; b += U * Q)
+    for (int b = q; b < nslots; b += U * Q)
+    {
+        float v[U][4];
+        if (n >= 4)
         {
-            float v[U][4];
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-            {
-                const float* __restrict__ p = part + (int64_t)min(b + u * Q, nslots - 1) * n + j;
-                if (j + 4 <= n)
-                {
-                    __builtin_memcpy(v[u], p, sizeof(v[u]));
-                }
-                else
-                {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) v[u][k] = j + k < n ? p[k] : 0.0f;
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) s[k] += b + u * Q < nslots ? (Acc)v[u][k] : Acc(0);
+            for (int u = 0; u < U; ++u) __builtin_memcpy(v[u], part + (int64_t)min(b + u * Q, nslots - 1) * n + j, sizeof(v[u]));
         }
+        else
+        {
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[u][k] = part[(int64_t)min(b + u * Q, nslots - 1) * n + min(k, (int)n - 1)];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s[k] += b + u * Q < nslots ? (Acc)v[u][k] : Acc(0);
+    }
     if constexpr (Q > 1)
     {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) sums[q][g][k] = s[k];
+        for (int k = 0; k < 4; ++k) sums[q * COLS + g * 4 + k] = s[k];
+        __syncthreads();
+        const int tc = threadIdx.x % COLS, tq = threadIdx.x / COLS;
+        four[tq * COLS + tc] = ((sums[4 * tq * COLS + tc] + sums[(4 * tq + 1) * COLS + tc]) + sums[(4 * tq + 2) * COLS + tc]) +
+                               sums[(4 * tq + 3) * COLS + tc];
         __syncthreads();
         // A thread a column.
-        const int64_t c = (int64_t)blockIdx.x * GROUPS * 4 + threadIdx.x;
-        if (threadIdx.x >= GROUPS * 4 || c >= n) return;
+        const int64_t first = (int64_t)blockIdx.x * COLS + tc / 4 * 4, c = (first + 4 <= n ? first : n < 4 ? 0 : n - 4) + tc % 4;
+        if (tq != 0 || c < first || c >= n) return;
         Acc t = Acc(0);
 #pragma unroll
-        for (int i = 0; i < Q; ++i) t += sums[i][threadIdx.x / 4][threadIdx.x % 4];
+        for (int i = 0; i < Q / 4; ++i) t += four[i * COLS + tc];
         out[c] = (OT)t;
         return;
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-        if (j + k < n) out[j + k] = (OT)s[k];
+        if (j + k >= own && j + k < n) out[j + k] = (OT)s[k];
 }
 
 template <typename OT>
@@ -481,6 +483,8 @@ hipError_t sum_slots_async(const float* part, int nslots, int64_t n, OT* out, hi
         sum_slots_kernel<OT, 1><<<blocks(4 * BLOCK), BLOCK, 0, stream>>>(part, nslots, n, out);
     else if (nslots <= 256)
         sum_slots_kernel<OT, 16><<<blocks(64), BLOCK, 0, stream>>>(part, nslots, n, out);
+    else if (n <= 1024)
+        sum_slots_kernel<OT, 256><<<blocks(4), BLOCK, 0, stream>>>(part, nslots, n, out);
     else
         sum_slots_kernel<OT, 64><<<blocks(16), BLOCK, 0, stream>>>(part, nslots, n, out);
     return hipGetLastError();

@@ -318,7 +318,7 @@ __global__ __launch_bounds__(L::THREADS) void grad_weight8_kernel(const T* __res
 }
 
 using WideTile = WeightTile<256, 256, 32, 2, 2, 4>;
-using MiddleTile = WeightTile<128, 128, 32, 3, 2, 2>;
+using MiddleTile = WeightTile<128, 128, 32, 2, 4, 2>;
 using SmallTile = WeightTile<64, 64, 64, 2, 2, 2>;
 
 struct WeightPlan
@@ -330,16 +330,16 @@ struct WeightPlan
 
 // What a row of a workgroup's sums takes, in ns: of one workgroup alone on its CU, and of each of several (at most
 // per_cu). Measured over shapes from 64 x 64 to 4096 x 4096; the small tiles' rates are per output lower
-// (small to wide: 300, 880 and 1170 TFLOP/s of bfloat16 products).
+// (small to wide: 450, 980 and 1170 TFLOP/s of bfloat16 products).
 struct TileCost
 {
     int side, step, per_cu;
     double alone, shared;
 };
 constexpr TileCost TILE_COST[3][3] = {
-    {{256, 32, 1, 28.0, 28.0}, {128, 32, 2, 15.0, 10.5}, {64, 64, 4, 7.0, 4.6}},    // bfloat16
-    {{}, {128, 32, 2, 30.0, 17.0}, {64, 64, 3, 13.0, 7.6}},                        // float16
-    {{}, {128, 32, 1, 30.0, 30.0}, {64, 64, 2, 17.0, 11.0}},                       // float32
+    {{256, 32, 1, 28.0, 28.0}, {128, 32, 2, 13.0, 8.5}, {64, 64, 4, 7.0, 4.6}},    // bfloat16
+    {{}, {128, 32, 2, 32.0, 15.0}, {64, 64, 3, 13.0, 7.6}},                        // float16
+    {{}, {128, 32, 1, 22.0, 22.0}, {64, 64, 2, 17.0, 11.0}},                       // float32
 };
 constexpr int NUM_CU = 256;
 // Bytes of slots written and read a ns, rows a split sums at least, and at most (a split counts its rows in 32 bits).
@@ -347,9 +347,9 @@ constexpr double SLOT_RATE = 3200.0;
 constexpr int64_t SPLIT_ROWS = 48, SPLIT_MOST = 1 << 30;
 
 // The tile and the number of splits of the least estimated time: rounds of workgroups over the CUs, and the
-// slots' way to memory and back. The estimate picks within 3% of the best of all on average over 34
+// slots' way to memory and back. The estimate picks within 1% of the best of all on average over 34
 // measured shapes; one rule of thumb (the largest tile, splits up to two workgroups a CU) was 35% off
-// (2048 x 2048 x 2048 bfloat16: 52 us against 31 with middle tiles unsplit; 16384 x 512 x 512: 40 against 27 with small ones).
+// (2048 x 2048 x 2048 bfloat16: 52 us against 27 with middle tiles unsplit; 16384 x 512 x 512: 40 against 27 with small ones).
 static WeightPlan weight_plan(int planes, int64_t rows, int out, int cols)
 {
     WeightPlan best{};
@@ -426,7 +426,7 @@ hipError_t grad_weight8(const T* grad_y, int64_t gy_stride, const uint8_t* codes
 template <typename OT, int Q>
 __global__ __launch_bounds__(BLOCK) void sum_slots_kernel(const float* __restrict__ part, int nslots, int64_t n, OT* __restrict__ out)
 {
-    constexpr int GROUPS = BLOCK / Q, COLS = GROUPS * 4, U = Q > 1 ? 8 : 4;
+    constexpr int GROUPS = BLOCK / Q, COLS = GROUPS * 4, U = Q > 1 ? 8 : 2;
     __shared__ Acc sums[Q * COLS], four[Q / 4 * COLS + 1];
     const int g = threadIdx.x % GROUPS, q = threadIdx.x / GROUPS;
     const int64_t own = ((int64_t)blockIdx.x * GROUPS + g) * 4, j = own + 4 <= n ? own : n < 4 ? 0 : n - 4;

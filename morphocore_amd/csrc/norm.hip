@@ -131,7 +131,7 @@ __global__ __launch_bounds__(norm_threads<G>()) void rms_norm_fwd_kernel(const T
                                                                          int64_t rs, const WT* __restrict__ w, float eps, T* __restrict__ y,
                                                                          T* __restrict__ h, uint8_t* __restrict__ codes,
                                                                          uint8_t* __restrict__ scales, float* __restrict__ rstd, int64_t rows,
-                                                                         int cols)
+                                                                         int cols, bool streaming)
 {
     constexpr int ROWS = norm_threads<G>() / G;
     __shared__ float part[2 * (G > WAVE ? G / WAVE : 1)];
@@ -162,10 +162,10 @@ __global__ __launch_bounds__(norm_threads<G>()) void rms_norm_fwd_kernel(const T
         for (int k = 0; k < V; ++k)
         {
             const int c = (lane + G * k) * UNIT, valid = cols - c;
-            if (h) store_unit(h + row * cols + c, valid, v[k]);
+            if (h) store_unit(h + row * cols + c, valid, v[k], streaming);
 #pragma unroll
             for (int j = 0; j < UNIT; ++j) v[k][j] = scaled(v[k][j], q, wv[k][j]);
-            if (y) store_unit(y + row * cols + c, valid, v[k]);
+            if (y) store_unit(y + row * cols + c, valid, v[k], streaming);
             if (codes)
             {
                 round_unit<T>(v[k]);  // the 8-bit form is y's, as stored
@@ -180,7 +180,7 @@ template <typename T, typename WT>
 __global__ __launch_bounds__(1024) void rms_norm_fwd_wide_kernel(const T* __restrict__ x, int64_t xs, const T* __restrict__ r, int64_t rs,
                                                                  const WT* __restrict__ w, float eps, T* __restrict__ y, T* __restrict__ h,
                                                                  uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
-                                                                 float* __restrict__ rstd, int64_t rows, int cols)
+                                                                 float* __restrict__ rstd, int64_t rows, int cols, bool streaming)
 {
     constexpr int G = 1024;
     __shared__ float part[2 * G / WAVE];
@@ -217,10 +217,10 @@ __global__ __launch_bounds__(1024) void rms_norm_fwd_wide_kernel(const T* __rest
             float v[UNIT], wv[UNIT];
             load(unit, v);
             load_unit(w + c, c, valid, wv);
-            if (h) store_unit(h + row * cols + c, valid, v);
+            if (h) store_unit(h + row * cols + c, valid, v, streaming);
 #pragma unroll
             for (int j = 0; j < UNIT; ++j) v[j] = scaled(v[j], q, wv[j]);
-            if (y) store_unit(y + row * cols + c, valid, v);
+            if (y) store_unit(y + row * cols + c, valid, v, streaming);
             if (codes)
             {
                 round_unit<T>(v);
@@ -237,7 +237,8 @@ template <typename T, typename WT, int G, int V>
 __global__ __launch_bounds__(norm_threads<G>()) void rms_norm_bwd_kernel(const T* __restrict__ gy, int64_t gys, const T* __restrict__ gh,
                                                                          int64_t ghs, const T* __restrict__ h, int64_t hs,
                                                                          const WT* __restrict__ w, const float* __restrict__ rstd,
-                                                                         T* __restrict__ gx, float* __restrict__ gw_part, int64_t rows, int cols)
+                                                                         T* __restrict__ gx, float* __restrict__ gw_part, int64_t rows, int cols,
+                                                                         bool streaming)
 {
     constexpr int THREADS = norm_threads<G>(), ROWS = THREADS / G;
     __shared__ float part[2 * (G > WAVE ? G / WAVE : 1)];
@@ -278,7 +279,7 @@ __global__ __launch_bounds__(norm_threads<G>()) void rms_norm_bwd_kernel(const T
             const int c = (lane + G * k) * UNIT;
 #pragma unroll
             for (int j = 0; j < UNIT; ++j) a[k][j] -= n[k][j] * m;
-            store_unit(gx + row * cols + c, cols - c, a[k]);
+            store_unit(gx + row * cols + c, cols - c, a[k], streaming);
         }
     }
     if (!gw_part) return;
@@ -319,7 +320,7 @@ __global__ __launch_bounds__(norm_threads<G>()) void rms_norm_bwd_kernel(const T
 template <typename T, typename WT>
 __global__ __launch_bounds__(1024) void rms_norm_bwd_wide_kernel(const T* __restrict__ gy, int64_t gys, const T* __restrict__ gh, int64_t ghs,
                                                                  const T* __restrict__ h, int64_t hs, const WT* __restrict__ w,
-                                                                 const float* __restrict__ rstd, T* __restrict__ gx, int64_t rows, int cols)
+                                                                 const float* __restrict__ rstd, T* __restrict__ gx, int64_t rows, int cols, bool streaming)
 {
     constexpr int G = 1024;
     __shared__ float part[2 * G / WAVE];
@@ -365,7 +366,7 @@ __global__ __launch_bounds__(1024) void rms_norm_bwd_wide_kernel(const T* __rest
 #pragma unroll
                 for (int j = 0; j < UNIT; ++j) a[j] += u[j];
             }
-            store_unit(gx + row * cols + c, cols - c, a);
+            store_unit(gx + row * cols + c, cols - c, a, streaming);
         }
     }
 }
@@ -434,16 +435,19 @@ hipError_t rms_norm_forward(const T* x, int64_t x_stride, const T* residual, int
 {
     if (rows <= 0 || cols <= 0) return hipSuccess;
     const int units = units_of(cols);
+    // (A lane's 8 float32 values are two stores, which past the caches write half lines: a norm alone, 524288 x 64, takes
+    // 50 us for 42; with the residual, 106 for 121.)
+    const bool streaming = (sizeof(T) == 2 || residual) && streams((double)rows * cols * (sizeof(T) * (1.0 + !!residual + !!y + !!h) + !!codes));
     if (units > NORM_MAX_UNITS)
     {
         rms_norm_fwd_wide_kernel<T, WT><<<norm_grid(rows, 1, NORM_BLOCKS), 1024, 0, stream>>>(x, x_stride, residual, r_stride, w, eps, y, h,
-                                                                                             codes, scales, rstd, rows, cols);
+                                                                                             codes, scales, rstd, rows, cols, streaming);
         return hipGetLastError();
     }
     return norm_shape(units, [&](auto g, auto v) {
         constexpr int G = decltype(g)::value, V = decltype(v)::value;
         rms_norm_fwd_kernel<T, WT, G, V><<<norm_grid(rows, norm_threads<G>() / G, NORM_BLOCKS * BLOCK / norm_threads<G>()), norm_threads<G>(), 0, stream>>>(
-            x, x_stride, residual, r_stride, w, eps, y, h, codes, scales, rstd, rows, cols);
+            x, x_stride, residual, r_stride, w, eps, y, h, codes, scales, rstd, rows, cols, streaming);
         return hipGetLastError();
     });
 }
@@ -491,12 +495,13 @@ hipError_t rms_norm_backward(const T* grad_y, int64_t gy_stride, const T* grad_h
     if (!grad_x && !grad_w) return hipSuccess;
     const int units = units_of(cols), slots = norm_slots(rows, cols);
     float* part = grad_w ? (float*)workspace : nullptr;
+    const bool streaming = streams((double)rows * cols * sizeof(T) * (1.0 + !!grad_y + !!grad_h + !!grad_x));
     hipError_t err;
     if (units > NORM_MAX_UNITS)
     {
         if (grad_x)
             rms_norm_bwd_wide_kernel<T, WT><<<norm_grid(rows, 1, NORM_BLOCKS), 1024, 0, stream>>>(grad_y, gy_stride, grad_h, gh_stride, h, h_stride,
-                                                                                                 w, rstd, grad_x, rows, cols);
+                                                                                                 w, rstd, grad_x, rows, cols, streaming);
         if (part)
             rms_norm_gw_wide_kernel<T><<<dim3((units + BLOCK - 1) / BLOCK, slots), BLOCK, 0, stream>>>(grad_y, gy_stride, h, h_stride, rstd, part,
                                                                                                        rows, cols);
@@ -507,7 +512,7 @@ hipError_t rms_norm_backward(const T* grad_y, int64_t gy_stride, const T* grad_h
         err = norm_shape(units, [&](auto g, auto v) {
             constexpr int G = decltype(g)::value, V = decltype(v)::value;
             rms_norm_bwd_kernel<T, WT, G, V><<<slots, norm_threads<G>(), 0, stream>>>(grad_y, gy_stride, grad_h, gh_stride, h, h_stride, w, rstd,
-                                                                                      grad_x, part, rows, cols);
+                                                                                      grad_x, part, rows, cols, streaming);
             return hipGetLastError();
         });
     }

@@ -140,7 +140,7 @@ def test_empty(shape):
 # ------------------------------------------------------------------------------------------------
 
 NORMS = [(1, 1), (3, 5), (2, 32), (17, 33), (130, 64), (9, 120), (33, 250), (7, 500), (5, 777), (6, 1024), (3, 1237), (4, 2048), (3, 2500), (2, 4096),
-         (2, 5001), (3, 8192), (2, 12289), (1, 20000), (2, 32801), (2100, 40), (700, 130)]
+         (2, 5001), (3, 8192), (2, 11000), (2, 12289), (1, 20000), (2, 32801), (2100, 40), (700, 130)]
 
 
 def check_norm(dtype, wdtype, rows, cols, residual, gy_on=True, gh_on=True, scale=1.0):
@@ -192,6 +192,21 @@ def test_norm(dtype, rows, cols):
 def test_norm_with_one_gradient_missing(cols):
     check_norm(torch.bfloat16, torch.bfloat16, 5, cols, True, gy_on=False)
     check_norm(torch.float32, torch.float32, 5, cols, True, gh_on=False)
+
+
+def test_only_the_gradients_asked_for():
+    x, r, w = randn(1, 9, 200).requires_grad_(), randn(2, 9, 200).requires_grad_(), randn(3, 200).requires_grad_()
+    gy, gh = randn(4, 9, 200), randn(5, 9, 200)
+    def grads(a, b, c):
+        return torch.autograd.grad(F.rms_norm(a, b, c), [t for t in (a, b, c) if t.requires_grad], [gy, gh])
+    gx, gw, gr = grads(x, w, r)
+    assert torch.equal(grads(x, w.detach(), r.detach())[0], gx) and torch.equal(grads(x.detach(), w.detach(), r)[0], gr)
+    assert torch.equal(grads(x.detach(), w, r.detach())[0], gw)
+    u = randn(6, 9, 200).requires_grad_()
+    for f in (F.gated_silu, lambda *t: F.gated_silu8(*t).y):
+        gg, gu = torch.autograd.grad(f(x, u), [x, u], gy)
+        assert torch.equal(torch.autograd.grad(f(x, u.detach()), x, gy)[0], gg)
+        assert torch.equal(torch.autograd.grad(f(x.detach(), u), u, gy)[0], gu)
 
 
 def test_norm_of_expanded_and_strided_rows():
@@ -507,8 +522,26 @@ def test_checkpoint8_of_a_morphological_stack():
 
 
 # ------------------------------------------------------------------------------------------------
-# Offsets past 32 bits
+# Launches beyond the last-level cache, offsets past 32 bits
 # ------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype,rows,cols", [(torch.bfloat16, 41000, 1001), (torch.float32, 300000, 88), (torch.float16, 2500, 17000)])
+def test_large_launches_give_the_rows_of_small_ones(dtype, rows, cols):
+    """More than 256 MB, whose results are stored past the caches: every row as the same row of a short array."""
+    x, r = randn(1, 1000, cols, dtype=dtype).repeat(rows // 1000 + 1, 1)[:rows], randn(2, 1000, cols, dtype=dtype).repeat(rows // 1000 + 1, 1)[:rows]
+    w = (1 + 0.1 * randn(3, cols)).to(dtype)
+
+    def step(x, r):
+        x, r = x.clone().requires_grad_(), r.clone().requires_grad_()
+        y, packed, h = F.rms_norm8(x, w, r)
+        gx, = torch.autograd.grad([y, h], x, [r.detach(), x.detach()])
+        z, packed2 = F.gated_silu8(x, r)
+        g, u = torch.autograd.grad(z, [x, r], y.detach())
+        return [y, h, F.unpack8(packed, dtype), gx, z, F.unpack8(packed2, dtype), g, u]
+
+    for large, small in zip(step(x, r), step(x[:1000], r[:1000])):
+        assert torch.equal(large[:1000], small) and torch.equal(large[-500:], small[torch.arange(rows - 500, rows, device=DEV) % 1000])
+
 
 def test_rows_past_32_bit_offsets():
     """Arrays of more than 2^32 elements: the last rows are worked on as the same rows of a small array."""

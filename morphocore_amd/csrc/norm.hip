@@ -435,9 +435,9 @@ hipError_t rms_norm_forward(const T* x, int64_t x_stride, const T* residual, int
 {
     if (rows <= 0 || cols <= 0) return hipSuccess;
     const int units = units_of(cols);
-    // (A lane's 8 float32 values are two stores, which past the caches write half lines: a norm alone, 524288 x 64, takes
-    // 50 us for 42; with the residual, 106 for 121.)
-    const bool streaming = (sizeof(T) == 2 || residual) && streams((double)rows * cols * (sizeof(T) * (1.0 + !!residual + !!y + !!h) + !!codes));
+    // (A norm alone in float32, two stores a lane, is up to 8 us slower of 42 at 524288 x 64; its training step, whose
+    // backward then finds x in the cache, takes 123 us for 137.)
+    const bool streaming = streams((double)rows * cols * (sizeof(T) * (1.0 + !!residual + !!y + !!h) + !!codes));
     if (units > NORM_MAX_UNITS)
     {
         rms_norm_fwd_wide_kernel<T, WT><<<norm_grid(rows, 1, NORM_BLOCKS), 1024, 0, stream>>>(x, x_stride, residual, r_stride, w, eps, y, h,

@@ -486,6 +486,13 @@ Tensor grad_weight8(const Tensor& grad_output, const Tensor& codes, const Tensor
     return weight_gradient(grad_output.detach(), p, out);
 }
 
+// The plain product in the operands' type, under autocast too: what the backward runs, which autocast does not reach.
+Tensor plain_product(const Tensor& x, const Tensor& weight)
+{
+    const c10::impl::ExcludeDispatchKeyGuard guard(c10::DispatchKey::AutocastCUDA);
+    return at::linear(x, weight);
+}
+
 class Linear8Function : public torch::autograd::Function<Linear8Function>
 {
 public:
@@ -497,7 +504,7 @@ public:
         ctx->set_materialize_grads(false);
         ctx->save_for_backward({x.requires_grad() ? weight : Tensor(), p.codes, p.scales});
         ctx->saved_data["type"] = (int64_t)weight.scalar_type();
-        return at::linear(x, weight);
+        return plain_product(x, weight);
     }
 
     static tensor_list backward(AutogradContext* ctx, tensor_list grads)
@@ -529,7 +536,7 @@ Tensor linear8(const Tensor& input, const Tensor& weight, const OptTensor& codes
         packed_arg("linear8", *codes, *scales);
         check_device("linear8", input, {*codes});
     }
-    if (!records({input, weight})) return at::linear(input, weight);
+    if (!records({input, weight})) return plain_product(input, weight);
     return Linear8Function::apply(input, weight, codes, scales);
 }
 

@@ -3,8 +3,8 @@
 //
 // A matrix product over the rows on the bfloat16 matrix instructions. A packed value (4 significant bits
 // times a power of two) is exact in bfloat16, and grad_y is split by truncation into as many bfloat16 terms
-// as its significand takes: bfloat16 itself, float16 two, float32 three; every product is then exact and
-// the sums are float32. Three bfloat16 products still run several times as fast as one float32 product.
+// as its significand takes: bfloat16 itself, float16 two, float32 three; every product is then exact (but for
+// what a float32 value below 2^-110 has under bfloat16's smallest, 2^-133) and the sums are float32. Three bfloat16 products still run several times as fast as one float32 product.
 //
 // Both operands lie with the summed axis as the slow one, so a wave reads its fragments from LDS with the
 // transposing read (ds_read_b64_tr_b16: 16 lanes read 4 rows of 16 columns and each gets a column). A row

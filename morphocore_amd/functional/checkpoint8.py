@@ -44,6 +44,7 @@ class _Checkpoint8(torch.autograd.Function):
         if not isinstance(out, torch.Tensor):
             raise TypeError(f"checkpoint8 takes a module that returns one tensor, not {type(out).__name__}")
         ctx.module, ctx.state, ctx.dtype = module, state, x.dtype
+        ctx.autocast = dict(enabled=torch.is_autocast_enabled("cuda"), dtype=torch.get_autocast_dtype("cuda"))
         ctx.save_for_backward(*pack8(x), *params)
         return out
 
@@ -54,11 +55,14 @@ class _Checkpoint8(torch.autograd.Function):
         x = unpack8(Packed8(codes, scales), ctx.dtype).requires_grad_(ctx.needs_input_grad[2])
         device = x.device
         devices = [] if ctx.state is None else [device]
-        with torch.random.fork_rng(devices, enabled=ctx.state is not None, device_type="cuda"), torch.enable_grad():
+        with torch.random.fork_rng(devices, enabled=ctx.state is not None, device_type="cuda"), torch.enable_grad(), \
+                torch.autocast("cuda", **ctx.autocast):
             if ctx.state is not None:
                 torch.set_rng_state(ctx.state[0])
                 torch.cuda.set_rng_state(ctx.state[1], device)
             out = ctx.module(x)
+        if not out.requires_grad:  # the output depends on none of them
+            return (None,) * len(ctx.needs_input_grad)
         wanted = [t for t, need in zip([x, *params], ctx.needs_input_grad[2:]) if need]
         grads = iter(torch.autograd.grad(out, wanted, grad, allow_unused=True))
         return None, None, *(next(grads) if need else None for need in ctx.needs_input_grad[2:])

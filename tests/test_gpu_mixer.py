@@ -348,6 +348,15 @@ def test_weight_gradient_keeps_every_bit_of_its_operands(dtype):
     assert np.array_equal(F.grad_weight8(gy, packed, torch.float32).cpu().numpy(), want)
 
 
+def test_weight_gradient_of_subnormal_values():
+    """bfloat16 and float16 gradients down to their smallest values, float32 ones to 2^-133."""
+    packed = F.pack8(torch.full((1, 40), 2.0**60, device=DEV))
+    for dtype, e in ((torch.bfloat16, -131), (torch.float16, -22), (torch.float32, -109), (torch.float32, -124)):
+        gy = (1 + torch.rand(1, 50, generator=torch.Generator().manual_seed(1), dtype=torch.float64)).mul(2.0**e).to(dtype).to(DEV)
+        far = np.abs(np64(F.grad_weight8(gy, packed, torch.float32)) / 2.0**60 - np64(gy).T)
+        assert far.max() <= (2.0**-133 if e == -124 else 0.0)
+
+
 def test_weight_gradient_of_strided_and_expanded_gradients():
     packed = F.pack8(randn(1, 4, 50, 96))
     wide = randn(2, 4, 50, 200)
@@ -466,6 +475,38 @@ def test_checkpoint8():
     net.eval()
     gb, = torch.autograd.grad(F.checkpoint8(net, x.detach()), net[0].bias, gy)
     assert torch.equal(gb, torch.autograd.grad(net(F.unpack8(F.pack8(x))), net[0].bias, gy)[0])
+
+
+def test_autocast():
+    """Operators keep their operands' type under autocast; a checkpointed module runs again under the forward's."""
+    import morphocore_amd.nn as nn
+
+    x, w = randn(1, 8, 96).requires_grad_(), randn(2, 40, 96).requires_grad_()
+    mixer, net = nn.ChannelMixer(96, 64).to(DEV), torch.nn.Linear(96, 33).to(DEV)
+    want = mixer(x)[0]
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        assert F.linear8(x, w).dtype == torch.float32
+        assert torch.equal(mixer(x)[0], want)
+        out = F.checkpoint8(net, x)
+    assert out.dtype == torch.bfloat16
+    kept = F.unpack8(F.pack8(x)).requires_grad_()
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        plain = net(kept)
+    gy = randn(3, 8, 33, dtype=torch.bfloat16)
+    for a, b in zip(torch.autograd.grad(out, [x, net.weight], gy), torch.autograd.grad(plain, [kept, net.weight], gy)):
+        assert torch.equal(a, b)
+
+
+def test_checkpoint8_of_modules_that_pass_or_drop_their_input():
+    x = randn(1, 4, 32).requires_grad_()
+    assert torch.equal(torch.autograd.grad(F.checkpoint8(torch.nn.Identity(), x), x, x.detach())[0], x)
+
+    class Constant(torch.nn.Module):
+        def forward(self, t):
+            return torch.ones_like(t)
+
+    out = F.checkpoint8(Constant(), x)
+    assert torch.autograd.grad(out, x, x.detach(), allow_unused=True)[0] is None
 
 
 # ------------------------------------------------------------------------------------------------

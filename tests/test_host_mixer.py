@@ -74,7 +74,10 @@ def test_abi_refuses_types_sizes_and_strides():
     refused(lib.mca_gated_silu_backward(0, P, 8, None, 8, None, 8, P, P, P, None, P, P, 8, 4, 8, None), "packed form")
     refused(lib.mca_gated_silu_backward(0, P, 8, P, 8, P, 8, None, None, None, None, P, P, 7, 4, 8, None), "grad_stride")
     refused(lib.mca_grad_weight8(0, 1, P, 8, P, P, P, 4, 8, 8, P, 1 << 20, None), "weight_dtype")
-    refused(lib.mca_grad_weight8(0, 0, P, 8, P, P, P, 4, 8, 8, P, 1, None), "Workspace too small")
+    need = lib.mca_grad_weight8_workspace_size(0, 100000, 64, 64)  # rows in splits
+    assert need > 0
+    refused(lib.mca_grad_weight8(0, 0, P, 64, P, P, P, 100000, 64, 64, P, need - 1, None), "Workspace too small")
+    refused(lib.mca_grad_weight8(0, 0, P, 64, P, P, P, 100000, 64, 64, None, need, None), "Workspace too small")
     refused(lib.mca_grad_weight8(0, 0, P, 8, P, P, None, 4, 8, 8, P, 1 << 20, None), "must not be null")
 
 

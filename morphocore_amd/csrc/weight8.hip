@@ -4,7 +4,8 @@
 // A matrix product over the rows on the bfloat16 matrix instructions. A packed value (4 significant bits
 // times a power of two) is exact in bfloat16, and grad_y is split by truncation into as many bfloat16 terms
 // as its significand takes: bfloat16 itself, float16 two, float32 three; every product is then exact (but for
-// what a float32 value below 2^-110 has under bfloat16's smallest, 2^-133) and the sums are float32. Three bfloat16 products still run several times as fast as one float32 product.
+// what a float32 value below 2^-110 has under bfloat16's smallest, 2^-133) and the sums are float32. Three bfloat16
+// products still run several times as fast as one float32 product.
 //
 // Both operands lie with the summed axis as the slow one, so a wave reads its fragments from LDS with the
 // transposing read (ds_read_b64_tr_b16: 16 lanes read 4 rows of 16 columns and each gets a column). A row
@@ -16,10 +17,10 @@
 // Rows are split over workgroups where the output has too few tiles for the 256 CUs; each split writes its
 // float32 sums to a slot, and the slots are added in order (no atomics: the same result every time).
 //
-// Measured: 8192 x 4096 x 4096 (rows, out, columns) bfloat16 237 us, 1158 TFLOP/s, where the library's bfloat16
+// Measured: 8192 x 4096 x 4096 (rows, out, columns) bfloat16 234 us, 1172 TFLOP/s, where the library's bfloat16
 // product of 8192^3, the fastest measured, runs at 1202 and its product of these operands unpacked takes 287 us;
-// float16 4096 x 8192 x 1024 139 us (988 TFLOP/s of bfloat16 products), float32 205 us (1005). 524288 x 64 x 64 float32
-// 36 us (4.5 TB/s), bound by HBM. Tiles in between are bound by latency: 5003 x 1111 x 777 float16 39 us.
+// float16 452 us (1216 TFLOP/s of bfloat16 products), float32 667 us (1237). 524288 x 64 x 64 float32 36 us
+// (4.5 TB/s), bound by HBM. Tiles in between are bound by latency: 5003 x 1111 x 777 float16 36 us.
 #include "block8.hpp"
 #include "launch.hpp"
 #include "mixer.hpp"
@@ -323,28 +324,32 @@ __global__ __launch_bounds__(L::THREADS) void grad_weight8_kernel(const T* __res
 }
 
 using WideTile = WeightTile<256, 256, 32, 2, 2, 4>;
+using TallTile = WeightTile<128, 256, 32, 2, 2, 4>;
 using MiddleTile = WeightTile<128, 128, 32, 2, 4, 2>;
 using SmallTile = WeightTile<64, 64, 64, 2, 2, 2>;
 
 struct WeightPlan
 {
-    int tile;  // 0 wide, 1 middle, 2 small
+    int tile;  // 0 wide, 1 tall, 2 middle, 3 small
     int tiles_n, tiles_k, splits;
     int64_t split_rows;
 };
 
 // What a row of a workgroup's sums takes, in ns: of one workgroup alone on its CU, and of each of several (at most
-// per_cu). Measured over shapes from 64 x 64 to 4096 x 4096; the small tiles' rates are per output lower
-// (small to wide: 450, 980 and 1170 TFLOP/s of bfloat16 products).
+// per_cu). Measured over shapes from 64 x 64 to 4096 x 4096. Larger tiles read and convert less for a product:
+// 8192 x 4096 x 4096 takes 234 us of bfloat16 with wide tiles, 292 with tall and 339 with middle ones; 452 of float16 with
+// tall and 534 with middle ones; 667 against 834 of float32, whose conversion costs most. 4096 x 4096 x 2048 of bfloat16
+// has too few wide tiles for the CUs: 77 us with tall ones, 91 with middle ones. The wide one's registers hold
+// bfloat16's operands only.
 struct TileCost
 {
-    int side, step, per_cu;
+    int side_n, side_k, step, per_cu;
     double alone, shared;
 };
-constexpr TileCost TILE_COST[3][3] = {
-    {{256, 32, 1, 28.0, 28.0}, {128, 32, 2, 13.0, 8.5}, {64, 64, 4, 7.0, 4.6}},    // bfloat16
-    {{}, {128, 32, 2, 32.0, 15.0}, {64, 64, 3, 13.0, 7.6}},                        // float16
-    {{}, {128, 32, 1, 22.0, 22.0}, {64, 64, 2, 17.0, 11.0}},                       // float32
+constexpr TileCost TILE_COST[3][4] = {
+    {{256, 256, 32, 1, 30.0, 30.0}, {128, 256, 32, 1, 18.0, 18.0}, {128, 128, 32, 2, 13.0, 9.0}, {64, 64, 64, 4, 6.5, 5.2}},  // bfloat16
+    {{}, {128, 256, 32, 1, 30.0, 30.0}, {128, 128, 32, 2, 21.0, 16.5}, {64, 64, 64, 3, 12.0, 7.6}},                         // float16
+    {{}, {128, 256, 32, 1, 43.0, 43.0}, {128, 128, 32, 1, 27.0, 27.0}, {64, 64, 64, 2, 17.0, 9.5}},                         // float32
 };
 constexpr int NUM_CU = 256;
 // Bytes of slots written and read a ns, rows a split sums at least, and at most (a split counts its rows in 32 bits).
@@ -352,19 +357,19 @@ constexpr double SLOT_RATE = 3200.0;
 constexpr int64_t SPLIT_ROWS = 48, SPLIT_MOST = 1 << 30;
 
 // The tile and the number of splits of the least estimated time: rounds of workgroups over the CUs, and the
-// slots' way to memory and back. The estimate picks within 1% of the best of all on average over 34
+// slots' way to memory and back. The estimate picks within 2% of the best of all on average over 41
 // measured shapes; one rule of thumb (the largest tile, splits up to two workgroups a CU) was 35% off
 // (2048 x 2048 x 2048 bfloat16: 52 us against 27 with middle tiles unsplit; 16384 x 512 x 512: 40 against 27 with small ones).
 static WeightPlan weight_plan(int planes, int64_t rows, int out, int cols)
 {
     WeightPlan best{};
     double best_ns = 0.0;
-    for (int t = planes == 1 ? 0 : 1; t < 3; ++t)
+    for (int t = planes == 1 ? 0 : 1; t < 4; ++t)
     {
         const TileCost& c = TILE_COST[planes - 1][t];
         // Tiles wider than an axis leave the branch-free loop.
-        if (t < 2 && (out < c.side || cols < c.side)) continue;
-        const int tiles_n = (out + c.side - 1) / c.side, tiles_k = (cols + c.side - 1) / c.side;
+        if (t < 3 && (out < c.side_n || cols < c.side_k)) continue;
+        const int tiles_n = (out + c.side_n - 1) / c.side_n, tiles_k = (cols + c.side_k - 1) / c.side_k;
         const int64_t tiles = (int64_t)tiles_n * tiles_k;
         for (int64_t wanted = 1; wanted <= 1024; wanted = wanted < 4 ? wanted + 1 : wanted % 3 ? wanted / 2 * 3 : wanted / 3 * 4)
         {
@@ -408,7 +413,8 @@ static hipError_t weight_launch(const WeightPlan& p, const T* gy, int64_t gys, c
     if (out_rows < UNIT || cols < UNIT) return run(SmallTile(), std::true_type());
     if constexpr (planes_of<T>() == 1)
         if (p.tile == 0) return run(WideTile(), std::false_type());
-    return p.tile == 1 ? run(MiddleTile(), std::false_type()) : run(SmallTile(), std::false_type());
+    if (p.tile == 1) return run(TallTile(), std::false_type());
+    return p.tile == 2 ? run(MiddleTile(), std::false_type()) : run(SmallTile(), std::false_type());
 }
 
 template <typename T, typename OT>

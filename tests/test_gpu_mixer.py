@@ -338,6 +338,13 @@ def test_weight_gradient(dtype, rows, out, cols):
         near(got, want, (2 * np.sqrt(rows) + 16) * f32 * size, got.dtype, f"dtype {to}")
 
 
+# Outputs large enough for the wide and the tall tiles, unsplit and split, with edges inside a tile.
+@pytest.mark.parametrize("rows,out,cols", [(333, 4050, 4060), (290, 4060, 2030), (4100, 1020, 2040), (17, 2050, 4100)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_weight_gradient_of_large_outputs(dtype, rows, out, cols):
+    test_weight_gradient(dtype, rows, out, cols)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_weight_gradient_keeps_every_bit_of_its_operands(dtype):
     """One row: the products alone, each exact but for the last rounding."""

@@ -486,11 +486,24 @@ Tensor grad_weight8(const Tensor& grad_output, const Tensor& codes, const Tensor
     return weight_gradient(grad_output.detach(), p, out);
 }
 
-// The plain product in the operands' type, under autocast too: what the backward runs, which autocast does not reach.
+// A tensor as a matrix of its last dimension's rows (a copy where its strides allow no view).
+Tensor matrix_of(const Tensor& t) { return t.dim() == 2 ? t : t.reshape({leading(t), t.size(-1)}); }
+
+Tensor with_rows_of(const Tensor& product, const Tensor& t)
+{
+    if (t.dim() == 2) return product;
+    std::vector<int64_t> shape = t.sizes().vec();
+    shape.back() = product.size(1);
+    return at::_unsafe_view(product, shape);  // no view to autograd: the product is nobody else's
+}
+
+// The plain product in the operands' type, under autocast too: what the backward runs, which autocast does not reach. Always of
+// matrices: of more dimensions with strides that allow no view torch makes a batched product, with the weight's transpose for
+// every batch.
 Tensor plain_product(const Tensor& x, const Tensor& weight)
 {
     const c10::impl::ExcludeDispatchKeyGuard guard(c10::DispatchKey::AutocastCUDA);
-    return at::linear(x, weight);
+    return with_rows_of(at::linear(matrix_of(x), weight), x);
 }
 
 class Linear8Function : public torch::autograd::Function<Linear8Function>
@@ -515,7 +528,7 @@ public:
         const auto saved = ctx->get_saved_variables();
         const c10::DeviceGuard guard(gy.device());
         Tensor gx, gw;
-        if (ctx->needs_input_grad(0)) gx = at::matmul(gy, saved[0]);
+        if (ctx->needs_input_grad(0)) gx = with_rows_of(at::mm(matrix_of(gy), saved[0]), gy);
         if (ctx->needs_input_grad(1)) gw = weight_gradient(gy, Packed{saved[1], saved[2]}, (at::ScalarType)ctx->saved_data["type"].toInt());
         return {gx, gw, Tensor(), Tensor()};
     }

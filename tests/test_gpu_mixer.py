@@ -390,6 +390,25 @@ def test_weight_gradient_not_finite():
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+def test_linear8_of_strides_without_a_matrix_view(dtype):
+    """Exchanged leading dimensions, expanded gradients and a transposed weight: the products of the dense tensors, bit for bit."""
+    x, w = randn(1, 20, 6, 64, dtype=dtype).transpose(0, 1), randn(2, 64, 40, dtype=dtype, scale=0.1).t()
+    assert torch.equal(F.linear8(x, w), F.linear8(x.contiguous(), w))
+    gy = randn(3, 20, 6, 40, dtype=dtype).transpose(0, 1)
+    for g in (gy, gy[:, :1].expand(6, 20, 40)):
+        got, want = [], []
+        for a, b, out in ((x, g, got), (x.contiguous(), g.contiguous(), want)):
+            a, v = a.detach().requires_grad_(), w.detach().requires_grad_()
+            y = F.linear8(a, v)
+            y += 1  # the output is no view
+            out += [y, *torch.autograd.grad(y, [a, v], b), *torch.autograd.grad(F.linear8(a, w), a, b)]
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+    near(F.linear8(x, w), np64(x) @ np64(w).T, 64 * f32 * (np.abs(np64(x)) @ np.abs(np64(w)).T), dtype)
+    assert F.linear8(x[0, 0], w).shape == (40,) and F.linear8(x[:0], w).shape == (0, 20, 40) and F.linear8(x[..., :0], w[:, :0]).shape == (6, 20, 40)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_linear8(dtype):
     x, w = randn(1, 3, 20, 96, dtype=dtype).requires_grad_(), randn(2, 50, 96, dtype=dtype, scale=0.1).requires_grad_()
     gy = randn(3, 3, 20, 50, dtype=dtype)

@@ -13,7 +13,8 @@ class Packed8(NamedTuple):
     """A tensor in 8-bit blocks of 32 values along its last dimension.
 
     codes : float8_e4m3fn, of the tensor's shape.
-    scales : float8_e8m0fnu, [..., ceil(last / 32)], a power of two for each block.
+    scales : float8_e8m0fnu, [..., ceil(last / 32)], a power of two for each block, 2^-117 to 2^119 (blocks made elsewhere are read
+        by the same rule from 2^-117 on; below it small codes are not exact, and the format's NaN scale is not one of them).
 
     A value is code * scale, within 1/16 of the original's magnitude or 2^-17 of its block's largest,
     whichever is more. It is exact in bfloat16 and float32. NaN and infinities become NaN.

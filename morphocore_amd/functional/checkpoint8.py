@@ -38,20 +38,27 @@ def unpack8(packed: Packed8, dtype: torch.dtype = torch.float32) -> torch.Tensor
 
 
 class _Checkpoint8(torch.autograd.Function):
+    # Returns the module's output, and x where the module wrote to an x that needs a gradient.
     @staticmethod
     def forward(ctx, module, state, x, *params):
+        packed = pack8(x)  # before the module, which may write to x
+        version = None if x.is_inference() else x._version
         with torch.no_grad():
             out = module(x)
         if not isinstance(out, torch.Tensor):
             raise TypeError(f"checkpoint8 takes a module that returns one tensor, not {type(out).__name__}")
         ctx.module, ctx.state, ctx.dtype = module, state, x.dtype
         ctx.autocast = dict(enabled=torch.is_autocast_enabled("cuda"), dtype=torch.get_autocast_dtype("cuda"))
-        ctx.save_for_backward(*pack8(x), *params)
-        return out
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(*packed, *params)
+        if not ctx.needs_input_grad[2] or version is None or x._version == version:
+            return out
+        ctx.mark_dirty(x)
+        return x if out is x else (out, x)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx, grad):
+    def backward(ctx, grad, grad_x=None):
         codes, scales, *params = ctx.saved_tensors
         x = unpack8(Packed8(codes, scales), ctx.dtype).requires_grad_(ctx.needs_input_grad[2])
         device = x.device
@@ -61,11 +68,13 @@ class _Checkpoint8(torch.autograd.Function):
             if ctx.state is not None:
                 torch.set_rng_state(ctx.state[0])
                 torch.cuda.set_rng_state(ctx.state[1], device)
-            out = ctx.module(x)
-        if not out.requires_grad:  # the output depends on none of them
+            given = torch.ops.aten._unsafe_view(x, x.shape)  # neither a leaf nor a view to autograd: the module may write to it
+            out = ctx.module(given)
+        results = [(t, g) for t, g in ((out, grad), (given, grad_x)) if g is not None and t.requires_grad]
+        if not results:  # they depend on none of the inputs
             return (None,) * len(ctx.needs_input_grad)
         wanted = [t for t, need in zip([x, *params], ctx.needs_input_grad[2:]) if need]
-        grads = iter(torch.autograd.grad(out, wanted, grad, allow_unused=True))
+        grads = iter(torch.autograd.grad([t for t, _ in results], wanted, [g for _, g in results], allow_unused=True))
         return None, None, *(next(grads) if need else None for need in ctx.needs_input_grad[2:])
 
 
@@ -75,7 +84,9 @@ def checkpoint8(module: torch.nn.Module, x: torch.Tensor) -> torch.Tensor:
 
     The output is the module's own. The gradients are those of the module at the kept values (see
     :class:`Packed8` for how far these are from ``x``). Modules that draw random numbers (dropout, weight noise) draw the same ones again.
-    A module with state that its forward changes (running statistics) changes it twice.
+    A module with state that its forward changes (running statistics) changes it twice. A module may write to its
+    input in place (torch refuses that for a view that needs a gradient: clone it first); an ``x`` that needs no
+    gradient then has the module's values, but no gradient of its parameters through them.
 
     module : a module of one tensor to one tensor; its parameters' gradients flow as without the checkpoint.
     x : float32, float16 or bfloat16 on a HIP device (any shape the module takes; blocks run along the last dimension).
@@ -85,4 +96,5 @@ def checkpoint8(module: torch.nn.Module, x: torch.Tensor) -> torch.Tensor:
         return module(x)
     # A module in training may draw; its draws are repeated from the generators' states.
     state = (torch.get_rng_state(), torch.cuda.get_rng_state(x.device)) if module.training and x.is_cuda else None
-    return _Checkpoint8.apply(module, state, x, *params)
+    out = _Checkpoint8.apply(module, state, x, *params)
+    return out if isinstance(out, torch.Tensor) else out[0]

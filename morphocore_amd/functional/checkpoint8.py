@@ -61,13 +61,13 @@ class _Checkpoint8(torch.autograd.Function):
     def backward(ctx, grad, grad_x=None):
         codes, scales, *params = ctx.saved_tensors
         x = unpack8(Packed8(codes, scales), ctx.dtype).requires_grad_(ctx.needs_input_grad[2])
-        device = x.device
-        devices = [] if ctx.state is None else [device]
+        devices = [x.device] if ctx.state is not None and x.is_cuda else []
         with torch.random.fork_rng(devices, enabled=ctx.state is not None, device_type="cuda"), torch.enable_grad(), \
                 torch.autocast("cuda", **ctx.autocast):
             if ctx.state is not None:
                 torch.set_rng_state(ctx.state[0])
-                torch.cuda.set_rng_state(ctx.state[1], device)
+                for device, state in zip(devices, ctx.state[1:]):
+                    torch.cuda.set_rng_state(state, device)
             given = torch.ops.aten._unsafe_view(x, x.shape)  # neither a leaf nor a view to autograd: the module may write to it
             out = ctx.module(given)
         results = [(t, g) for t, g in ((out, grad), (given, grad_x)) if g is not None and t.requires_grad]
@@ -78,23 +78,30 @@ class _Checkpoint8(torch.autograd.Function):
         return None, None, *(next(grads) if need else None for need in ctx.needs_input_grad[2:])
 
 
-def checkpoint8(module: torch.nn.Module, x: torch.Tensor) -> torch.Tensor:
+def checkpoint8(module: torch.nn.Module, x: torch.Tensor, preserve_rng: bool = True) -> torch.Tensor:
     """``module(x)``, keeping only ``x``, in 8 bits, for the backward, which runs the module again on the
     values kept and takes the gradients there.
 
     The output is the module's own. The gradients are those of the module at the kept values (see
-    :class:`Packed8` for how far these are from ``x``). Modules that draw random numbers (dropout, weight noise) draw the same ones again.
+    :class:`Packed8` for how far these are from ``x``). Modules that draw random numbers (dropout, weight noise) draw the
+    same ones again, in training or not, from torch's default generators of the CPU and of x's device.
     A module with state that its forward changes (running statistics) changes it twice. A module may write to its
     input in place (torch refuses that for a view that needs a gradient: clone it first); an ``x`` that needs no
     gradient then has the module's values, but no gradient of its parameters through them.
 
     module : a module of one tensor to one tensor; its parameters' gradients flow as without the checkpoint.
     x : float32, float16 or bfloat16 on a HIP device (any shape the module takes; blocks run along the last dimension).
+    preserve_rng : False for a module that draws nothing saves the generators' states. They cannot be read while a
+        graph is captured, so a captured step has to pass False.
     """
     params = [p for p in module.parameters() if p.requires_grad]
     if not torch.is_grad_enabled() or not (x.requires_grad or params):
         return module(x)
-    # A module in training may draw; its draws are repeated from the generators' states.
-    state = (torch.get_rng_state(), torch.cuda.get_rng_state(x.device)) if module.training and x.is_cuda else None
+    state = None
+    if preserve_rng:
+        if x.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("checkpoint8: the generators' states cannot be read while a graph is captured; pass preserve_rng=False "
+                               "for a module that draws no random numbers")
+        state = (torch.get_rng_state(), *([torch.cuda.get_rng_state(x.device)] if x.is_cuda else []))
     out = _Checkpoint8.apply(module, state, x, *params)
     return out if isinstance(out, torch.Tensor) else out[0]

@@ -1,0 +1,80 @@
+"""The channel-mixing operators on the GPU where their results are easily lost: checkpoints of modules that
+draw numbers, captured steps."""
+import pytest
+import torch
+
+import morphocore_amd.functional as F
+import morphocore_amd.nn as nn
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+
+
+def randn(seed, *shape, dtype=torch.float32, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=g) * scale).to(dtype).to(DEV)
+
+
+class Noise(torch.nn.Module):
+    """Draws whatever its training flag."""
+
+    def forward(self, x):
+        return x * torch.rand_like(x)
+
+
+def test_checkpoint_draws_the_forwards_numbers():
+    """A container in evaluation with a part in training, and a module that draws in evaluation too."""
+    torch.manual_seed(0)
+    mixed = torch.nn.Sequential(torch.nn.Linear(64, 48), torch.nn.Dropout(0.5)).to(DEV).eval()
+    mixed[1].train()
+    noise = torch.nn.Sequential(torch.nn.Linear(64, 48), Noise()).to(DEV).eval()
+    x, gy = F.unpack8(F.pack8(randn(1, 9, 64))), randn(2, 9, 48)  # values that a checkpoint holds exactly
+    for net in (mixed, noise):
+        results = []
+        for call in (net, lambda t: F.checkpoint8(net, t)):
+            torch.manual_seed(7)
+            a = x.clone().requires_grad_()
+            out = call(a)
+            results.append([out, *torch.autograd.grad(out, [a, *net.parameters()], gy), torch.rand(3, device=DEV)])
+        for plain, kept in zip(*results):
+            assert torch.equal(plain, kept)
+
+
+def test_captured_step_of_a_checkpoint():
+    """Forward and backward of checkpointed morphological layers and a channel mixer in one graph, whose every replay gives the eager
+    step's results; with the generators' states to keep, the capture is refused."""
+    torch.manual_seed(0)
+    net = nn.Checkpoint8(torch.nn.Sequential(nn.Opening(8, 8, 3), nn.Closing(8, 8, 3)), preserve_rng=False).to(DEV)
+    mixer = nn.ChannelMixer(8, 16, channels_first=True).to(DEV)
+    with torch.no_grad():
+        for p in net.parameters():
+            p.add_(0.1 * torch.randn_like(p))
+    params = [*net.parameters(), *mixer.parameters()]
+    x, go = randn(1, 2, 8, 20, 33).requires_grad_(), randn(2, 2, 8, 20, 33)
+
+    def step():
+        out, h = mixer(net(x), x)
+        return [out, h, *torch.autograd.grad([out, h], [x, *params], [go, go])]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for i in range(4):
+        with torch.no_grad():
+            x.copy_(randn(10 + i, 2, 8, 20, 33))
+        graph.replay()
+        torch.cuda.synchronize()
+        for k, (a, b) in enumerate(zip(got, step())):
+            assert torch.equal(a, b) or (a - b).norm() <= 1e-5 * b.norm(), f"replay {i}, result {k}"
+    net.preserve_rng = True
+    with pytest.raises(RuntimeError, match="preserve_rng=False"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            net(x)

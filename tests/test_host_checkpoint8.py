@@ -79,3 +79,53 @@ def test_leaf_that_needs_a_gradient_is_not_written_to():
     for call in (lambda m: m(x), lambda m: checkpoint8(m, x)):
         with pytest.raises(RuntimeError, match="leaf Variable that requires grad"):
             call(nn.Sequential(nn.LeakyReLU(0.1, inplace=True), nn.Linear(6, 3)))
+
+
+class Noise(nn.Module):
+    """Draws whatever its training flag."""
+
+    def forward(self, x):
+        return x * torch.rand(x.shape) + x * torch.rand(x.shape).sqrt()
+
+
+def part_in_training(module):
+    """A container in evaluation whose dropout is in training."""
+    module.eval()
+    module[1].train()
+    return module
+
+
+DRAWING = [lambda: nn.Sequential(nn.Linear(6, 6), nn.Dropout(0.5)), lambda: nn.Sequential(nn.Linear(6, 6), nn.Dropout(0.5)).eval(),
+           lambda: part_in_training(nn.Sequential(nn.Linear(6, 6), nn.Dropout(0.5))), lambda: nn.Sequential(nn.Linear(6, 6), Noise()),
+           lambda: nn.Sequential(nn.Linear(6, 6), Noise()).eval(), lambda: nn.Sequential(nn.Dropout(0.5, inplace=True), nn.Linear(6, 3))]
+
+
+@pytest.mark.parametrize("make", DRAWING)
+def test_rerun_draws_the_forwards_numbers(make):
+    torch.manual_seed(0)
+    module = make()
+    both(module, inner_with_gradient)
+    both(module, leaf_without_gradient)
+    # The caller's generator goes on as if the module had run once.
+    x = torch.randn(4, 6)
+    torch.manual_seed(7)
+    module(x.clone())
+    want = torch.rand(3)
+    torch.manual_seed(7)
+    out = checkpoint8(module, x.clone())
+    torch.autograd.grad(out.sum(), module.parameters())
+    assert torch.equal(torch.rand(3), want)
+
+
+def test_states_that_are_not_kept():
+    """preserve_rng=False: the rerun draws on from the generator as it is."""
+    module, x = nn.Sequential(nn.Linear(6, 6), nn.Dropout(0.5)), torch.randn(40, 6)
+    torch.manual_seed(7)
+    out = checkpoint8(module, x, preserve_rng=False)
+    got = torch.autograd.grad(out.sum(), module[0].bias)[0]
+    torch.manual_seed(7)
+    module(x)
+    want = torch.autograd.grad(module(x).sum(), module[0].bias)[0]
+    assert torch.equal(got, want)
+    from morphocore_amd.nn import Checkpoint8
+    assert Checkpoint8(module).preserve_rng and not Checkpoint8(module, preserve_rng=False).preserve_rng

@@ -43,12 +43,14 @@ class _Checkpoint8(torch.autograd.Function):
     def forward(ctx, module, state, x, *params):
         packed = pack8(x)  # before the module, which may write to x
         version = None if x.is_inference() else x._version
-        with torch.no_grad():
+        # Both runs go past autocast's cache of cast weights: it would keep this one's, which carry no gradient, for
+        # the rerun and for whoever uses the weights next in the same region.
+        ctx.autocast = dict(enabled=torch.is_autocast_enabled("cuda"), dtype=torch.get_autocast_dtype("cuda"), cache_enabled=False)
+        with torch.no_grad(), torch.autocast("cuda", **ctx.autocast):
             out = module(x)
         if not isinstance(out, torch.Tensor):
             raise TypeError(f"checkpoint8 takes a module that returns one tensor, not {type(out).__name__}")
         ctx.module, ctx.state, ctx.dtype = module, state, x.dtype
-        ctx.autocast = dict(enabled=torch.is_autocast_enabled("cuda"), dtype=torch.get_autocast_dtype("cuda"))
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(*packed, *params)
         if not ctx.needs_input_grad[2] or version is None or x._version == version:

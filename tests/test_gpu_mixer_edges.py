@@ -78,3 +78,27 @@ def test_captured_step_of_a_checkpoint():
     with pytest.raises(RuntimeError, match="preserve_rng=False"):
         with torch.cuda.graph(torch.cuda.CUDAGraph()):
             net(x)
+
+
+def test_checkpoint_leaves_no_cast_weights_behind():
+    """Under autocast: the gradients of a backward inside the region, and those of a weight that the same region uses again without the
+    checkpoint."""
+    torch.manual_seed(0)
+    net = torch.nn.Sequential(torch.nn.Linear(96, 96), torch.nn.Tanh()).to(DEV)
+    x, gy = F.unpack8(F.pack8(randn(1, 8, 96))), randn(2, 8, 96, dtype=torch.bfloat16)
+
+    def step(call, inside):
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            out = call(x) + net(x)
+            if inside:
+                return [out, *torch.autograd.grad(out, net.parameters(), gy)]
+        return [out, *torch.autograd.grad(out, net.parameters(), gy)]
+
+    want = step(net, False)
+    for inside in (False, True):
+        for a, b in zip(step(lambda t: F.checkpoint8(net, t), inside), want):
+            assert (a - b).norm() <= 2.0**-7 * b.norm()  # the two uses' bfloat16 gradients are added in another order
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        alone = torch.autograd.grad(F.checkpoint8(net, x), net.parameters(), gy)
+        plain = torch.autograd.grad(net(x), net.parameters(), gy)
+    assert all(torch.equal(a, b) for a, b in zip(alone, plain))

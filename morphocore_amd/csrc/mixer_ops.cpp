@@ -497,13 +497,19 @@ Tensor with_rows_of(const Tensor& product, const Tensor& t)
     return at::_unsafe_view(product, shape);  // no view to autograd: the product is nobody else's
 }
 
-// The plain product in the operands' type, under autocast too: what the backward runs, which autocast does not reach. Always of
-// matrices: of more dimensions with strides that allow no view torch makes a batched product, with the weight's transpose for
-// every batch.
+// The plain products in the operands' type, under autocast too (a backward called inside its region runs under it as well).
+// Always of matrices: of more dimensions with strides that allow no view torch makes a batched product, with the weight's
+// transpose for every batch.
 Tensor plain_product(const Tensor& x, const Tensor& weight)
 {
     const c10::impl::ExcludeDispatchKeyGuard guard(c10::DispatchKey::AutocastCUDA);
     return with_rows_of(at::linear(matrix_of(x), weight), x);
+}
+
+Tensor plain_product_grad(const Tensor& grad, const Tensor& weight)
+{
+    const c10::impl::ExcludeDispatchKeyGuard guard(c10::DispatchKey::AutocastCUDA);
+    return with_rows_of(at::mm(matrix_of(grad), weight), grad);
 }
 
 class Linear8Function : public torch::autograd::Function<Linear8Function>
@@ -528,7 +534,7 @@ public:
         const auto saved = ctx->get_saved_variables();
         const c10::DeviceGuard guard(gy.device());
         Tensor gx, gw;
-        if (ctx->needs_input_grad(0)) gx = with_rows_of(at::mm(matrix_of(gy), saved[0]), gy);
+        if (ctx->needs_input_grad(0)) gx = plain_product_grad(gy, saved[0]);
         if (ctx->needs_input_grad(1)) gw = weight_gradient(gy, Packed{saved[1], saved[2]}, (at::ScalarType)ctx->saved_data["type"].toInt());
         return {gx, gw, Tensor(), Tensor()};
     }

@@ -102,3 +102,18 @@ def test_checkpoint_leaves_no_cast_weights_behind():
         alone = torch.autograd.grad(F.checkpoint8(net, x), net.parameters(), gy)
         plain = torch.autograd.grad(net(x), net.parameters(), gy)
     assert all(torch.equal(a, b) for a, b in zip(alone, plain))
+
+
+def test_gradients_inside_an_autocast_region():
+    """linear8 and ChannelMixer keep their operands' type in a backward that runs inside the region: bit for bit the gradients outside."""
+    torch.manual_seed(0)
+    x, w, gy = randn(1, 8, 96).requires_grad_(), randn(2, 40, 96).requires_grad_(), randn(3, 8, 40)
+    mixer, go = nn.ChannelMixer(96, 64).to(DEV), randn(4, 8, 96)
+
+    def step():
+        out, h = mixer(x)
+        return [*torch.autograd.grad(F.linear8(x, w), [x, w], gy), *torch.autograd.grad([out, h], [x, *mixer.parameters()], [go, go])]
+
+    want = step()
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        assert all(torch.equal(a, b) for a, b in zip(step(), want))

@@ -148,9 +148,9 @@ int mca_gated_silu_backward(int dtype, const void* grad_y, int64_t grad_y_stride
     if ((rc = check_types(dtype, dtype)) || (rc = check_rows(rows, cols)) || (rc = check_stride({grad_y_stride, gate_stride, up_stride})))
         return rc;
     if (grad_stride < cols) return mca::api_fail("grad_stride must be at least cols");
-    if ((gate == nullptr) != (up == nullptr)) return mca::api_fail("gate and up go together");
     if (rows * cols > 0)
     {
+        if ((gate == nullptr) != (up == nullptr)) return mca::api_fail("gate and up go together");
         if (!grad_y || !grad_gate || !grad_up) return mca::api_fail("grad_y, grad_gate and grad_up must not be null");
         if (!gate && (!gate_codes || !gate_scales || !up_codes || !up_scales)) return mca::api_fail("gate and up, or their packed form, must be given");
     }

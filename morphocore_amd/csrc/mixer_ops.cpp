@@ -322,7 +322,8 @@ Gated gated_rows(const Tensor& gate, const Tensor& up)
     {
         g.cols = g.gate.cols / 2;
         g.shape.back() = g.cols;
-        g.up = (const char*)g.gate.data() + g.cols * gate.element_size();
+        const void* first = g.gate.data();  // null of an empty tensor
+        g.up = first ? (const char*)first + g.cols * gate.element_size() : nullptr;
         g.up_stride = g.gate.stride;
     }
     return g;
@@ -402,7 +403,8 @@ public:
         const int64_t cols = shape.back();
         if (joint) shape.back() *= 2;
         Tensor gg = torch::empty(shape, gy.options()), gu = joint ? Tensor() : torch::empty(shape, gy.options());
-        void* gu_data = joint ? (void*)((char*)gg.data_ptr() + cols * gy.element_size()) : gu.data_ptr();
+        char* first = (char*)gg.data_ptr();  // null of an empty tensor
+        void* gu_data = !joint ? gu.data_ptr() : first ? (void*)(first + cols * gy.element_size()) : nullptr;
         Gated in{};
         Kept kept = kept_of(g.rows, cols);
         if (eight)

@@ -117,3 +117,26 @@ def test_gradients_inside_an_autocast_region():
     want = step()
     with torch.autocast("cuda", dtype=torch.bfloat16):
         assert all(torch.equal(a, b) for a, b in zip(step(), want))
+
+
+@pytest.mark.parametrize("rows,cols", [((0,), 8), ((2, 0), 5), ((3,), 0), ((0,), 0), ((), 0)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_empty_steps(dtype, rows, cols):
+    """Forward and backward of every operator without rows or without columns."""
+    def empty(n):
+        return torch.zeros(*rows, n, dtype=dtype, device=DEV, requires_grad=True)
+
+    joint, gate, up, w = empty(2 * cols), empty(cols), empty(cols), torch.ones(cols, dtype=dtype, device=DEV, requires_grad=True)
+    for y, leaves in ((F.gated_silu(joint), [joint]), (F.gated_silu(gate, up), [gate, up]), (F.gated_silu8(joint).y, [joint]),
+                      (F.gated_silu8(gate, up).y, [gate, up]), (F.rms_norm(gate, w), [gate, w]), (F.rms_norm(gate, w, up)[0], [gate, w, up]),
+                      (F.rms_norm(gate, w, up)[1], [gate, w, up])):
+        assert y.shape == gate.shape
+        for g, t in zip(torch.autograd.grad(y, leaves, torch.ones_like(y)), leaves):
+            assert g.shape == t.shape and not g.any()
+    weight = torch.ones(6, cols, dtype=dtype, device=DEV, requires_grad=True)
+    for packed in (None, F.pack8(gate)):
+        y = F.linear8(gate, weight, packed)
+        assert y.shape == (*rows, 6) and not y.any()
+        gx, gw = torch.autograd.grad(y, [gate, weight], torch.ones_like(y))
+        assert gx.shape == gate.shape and gw.shape == weight.shape and not gw.any()
+    assert F.checkpoint8(torch.nn.Identity(), gate).shape == gate.shape

@@ -9,6 +9,7 @@
 #include <torch/all.h>
 #include <torch/library.h>
 
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
@@ -60,6 +61,14 @@ void check_type(const Tensor& x, const Tensor& t)
 void check_first_order(const char* name)
 {
     TORCH_CHECK(!torch::GradMode::is_enabled(), name, ": the backward cannot record a graph of its own (create_graph=True)");
+}
+
+// Forward-mode derivatives, which the operators do not carry on, are refused, not lost.
+void check_no_tangent(const char* name, std::initializer_list<Tensor> tensors)
+{
+    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+    for (const Tensor& t : tensors)
+        TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), name, ": forward-mode derivatives are not supported");
 }
 
 // A tensor as rows of its last dimension.
@@ -248,6 +257,7 @@ bool records(std::initializer_list<Tensor> tensors)
 void check_norm(const char* name, const Tensor& x, const Tensor& weight, const Tensor& residual, double eps)
 {
     check_rank(name, x);
+    check_no_tangent(name, {x, weight, residual});
     TORCH_CHECK(weight.dim() == 1 && weight.size(0) == x.size(-1), name, ": weight must be [", x.size(-1), "], got ", weight.sizes());
     TORCH_CHECK(eps >= 0.0, name, ": eps must be non negative");
     check_device(name, x, {weight});
@@ -421,6 +431,7 @@ public:
 void check_gated(const char* name, const Tensor& gate, const Tensor& up)
 {
     check_rank(name, gate);
+    check_no_tangent(name, {gate, up});
     check_device(name, gate, {});
     type_code(name, gate);
     if (!up.defined())

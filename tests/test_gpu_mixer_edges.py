@@ -140,3 +140,19 @@ def test_empty_steps(dtype, rows, cols):
         gx, gw = torch.autograd.grad(y, [gate, weight], torch.ones_like(y))
         assert gx.shape == gate.shape and gw.shape == weight.shape and not gw.any()
     assert F.checkpoint8(torch.nn.Identity(), gate).shape == gate.shape
+
+
+def test_forward_mode_derivatives():
+    """Refused by the operators that do not carry them on, right through linear8's plain product."""
+    import torch.autograd.forward_ad as forward
+
+    x, t, w = randn(1, 5, 64), randn(2, 5, 64), randn(3, 40, 64)
+    with forward.dual_level():
+        dual = forward.make_dual(x, t)
+        for call in (lambda: F.rms_norm(dual, w[0]), lambda: F.rms_norm8(x, w[0], dual), lambda: F.gated_silu(x, dual), lambda: F.gated_silu8(dual)):
+            with pytest.raises(RuntimeError, match="forward-mode derivatives are not supported"):
+                call()
+        assert torch.equal(forward.unpack_dual(F.linear8(dual, w)).tangent, F.linear8(t, w))
+        for call in (lambda: F.linear8(dual, w.requires_grad_()), lambda: F.checkpoint8(torch.nn.Linear(64, 3).to(DEV), dual)):
+            with pytest.raises(RuntimeError, match="jvp|forward AD"):
+                call()

@@ -83,6 +83,19 @@ __global__ __launch_bounds__(BLOCK) void unpack8_kernel(const uint8_t* __restric
     }
 }
 
+template <typename T>
+__global__ __launch_bounds__(BLOCK) void copy_rows_kernel(const T* __restrict__ x, int64_t xs, T* __restrict__ out, int64_t rows, int cols,
+                                                          int lanes, int magic)
+{
+    MCA_ROW_LOOP(unit, row)
+    {
+        const int c = unit * UNIT, valid = cols - c;
+        float v[UNIT] = {};
+        if (x) load_unit(x + row * xs + c, c, valid, v);
+        store_unit(out + row * cols + c, valid, v);
+    }
+}
+
 // The library's exponential for float32; the hardware's, whose error grows with the argument to a few
 // float32 units in the last place, where the result is rounded to 16 bits.
 template <typename T>
@@ -173,6 +186,15 @@ hipError_t unpack8(const uint8_t* codes, const uint8_t* scales, T* out, int64_t 
 }
 
 template <typename T>
+hipError_t copy_rows(const T* x, int64_t x_stride, T* out, int64_t rows, int cols, hipStream_t stream)
+{
+    if (rows <= 0 || cols <= 0) return hipSuccess;
+    const RowGrid g = row_grid(rows, cols);
+    copy_rows_kernel<T><<<g.grid, BLOCK, 0, stream>>>(x, x_stride, out, rows, cols, g.lanes, g.magic);
+    return hipGetLastError();
+}
+
+template <typename T>
 hipError_t gated_silu_forward(const T* gate, int64_t g_stride, const T* up, int64_t u_stride, T* y, PackedOut gate8, PackedOut up8,
                               PackedOut y8, int64_t rows, int cols, hipStream_t stream)
 {
@@ -203,6 +225,7 @@ hipError_t gated_silu_backward(const T* grad_y, int64_t gy_stride, const T* gate
 #define MCA_GATED(T)                                                                                                                    \
     template hipError_t pack8<T>(const T*, int64_t, uint8_t*, uint8_t*, int64_t, int, hipStream_t);                                     \
     template hipError_t unpack8<T>(const uint8_t*, const uint8_t*, T*, int64_t, int, hipStream_t);                                      \
+    template hipError_t copy_rows<T>(const T*, int64_t, T*, int64_t, int, hipStream_t);                                                 \
     template hipError_t gated_silu_forward<T>(const T*, int64_t, const T*, int64_t, T*, PackedOut, PackedOut, PackedOut, int64_t, int,  \
                                               hipStream_t);                                                                             \
     template hipError_t gated_silu_backward<T>(const T*, int64_t, const T*, int64_t, const T*, int64_t, PackedOut, PackedOut, T*, T*,   \

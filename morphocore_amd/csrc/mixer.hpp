@@ -16,6 +16,10 @@ hipError_t pack8(const T* x, int64_t x_stride, uint8_t* codes, uint8_t* scales, 
 template <typename T>
 hipError_t unpack8(const uint8_t* codes, const uint8_t* scales, T* out, int64_t rows, int cols, hipStream_t stream);
 
+// out = x's rows, or zeros where x is null.
+template <typename T>
+hipError_t copy_rows(const T* x, int64_t x_stride, T* out, int64_t rows, int cols, hipStream_t stream);
+
 // h = x (+ residual), y = h * rstd * w; residual, y, h, codes with scales, and rstd may be null.
 template <typename T, typename WT>
 hipError_t rms_norm_forward(const T* x, int64_t x_stride, const T* residual, int64_t r_stride, const WT* w, float eps, T* y, T* h,

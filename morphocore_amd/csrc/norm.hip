@@ -252,7 +252,7 @@ __global__ __launch_bounds__(norm_threads<G>()) void rms_norm_bwd_kernel(const T
     {
         RawUnit<T> rh[V], ry[V], rg[V];
         load_row<T, G, V>(h + row * hs, cols, rh);
-        if (gy) load_row<T, G, V>(gy + row * gys, cols, ry);
+        load_row<T, G, V>(gy + row * gys, cols, ry);
         if (gh && gx) load_row<T, G, V>(gh + row * ghs, cols, rg);
         const float q = rstd[row];
         float n[V][UNIT], a[V][UNIT];
@@ -262,7 +262,7 @@ __global__ __launch_bounds__(norm_threads<G>()) void rms_norm_bwd_kernel(const T
 #pragma unroll
             for (int j = 0; j < UNIT; ++j)
             {
-                const float g = gy ? ry[k][j] : 0.0f;
+                const float g = ry[k][j];
                 n[k][j] = rh[k][j] * q;
                 gw[k][j] += g * n[k][j];
                 a[k][j] = g * wv[k][j];
@@ -343,20 +343,19 @@ __global__ __launch_bounds__(1024) void rms_norm_bwd_wide_kernel(const T* __rest
             }
         };
         float s = 0.0f;
-        if (gy)
-            for (int unit = threadIdx.x; unit < units; unit += G)
-            {
-                float n[UNIT], a[UNIT];
-                load(unit, n, a);
+        for (int unit = threadIdx.x; unit < units; unit += G)
+        {
+            float n[UNIT], a[UNIT];
+            load(unit, n, a);
 #pragma unroll
-                for (int j = 0; j < UNIT; ++j) s += a[j] * n[j];
-            }
+            for (int j = 0; j < UNIT; ++j) s += a[j] * n[j];
+        }
         const float m = row_sum<G>(s, part, turn) * (1.0f / (float)cols);
         for (int unit = threadIdx.x; unit < units; unit += G)
         {
             const int c = unit * UNIT;
-            float n[UNIT] = {}, a[UNIT] = {};
-            if (gy) load(unit, n, a);
+            float n[UNIT], a[UNIT];
+            load(unit, n, a);
 #pragma unroll
             for (int j = 0; j < UNIT; ++j) a[j] = q * (a[j] - n[j] * m);
             if (gh)
@@ -489,13 +488,13 @@ hipError_t rms_norm_backward(const T* grad_y, int64_t gy_stride, const T* grad_h
             const hipError_t err = sum_slots_async<WT>(nullptr, 0, cols, grad_w, stream);
             if (err != hipSuccess) return err;
         }
-        if (rows <= 0 || !grad_x) return hipSuccess;
-        grad_w = nullptr;
+        // grad_h alone, whatever h and the weight hold: their products with a zero are NaN where they are not finite.
+        return grad_x ? copy_rows<T>(grad_h, gh_stride, grad_x, rows, cols, stream) : hipSuccess;
     }
     if (!grad_x && !grad_w) return hipSuccess;
     const int units = units_of(cols), slots = norm_slots(rows, cols);
     float* part = grad_w ? (float*)workspace : nullptr;
-    const bool streaming = streams((double)rows * cols * sizeof(T) * (1.0 + !!grad_y + !!grad_h + !!grad_x));
+    const bool streaming = streams((double)rows * cols * sizeof(T) * (2.0 + !!grad_h + !!grad_x));
     hipError_t err;
     if (units > NORM_MAX_UNITS)
     {

@@ -156,3 +156,31 @@ def test_forward_mode_derivatives():
         for call in (lambda: F.linear8(dual, w.requires_grad_()), lambda: F.checkpoint8(torch.nn.Linear(64, 3).to(DEV), dual)):
             with pytest.raises(RuntimeError, match="jvp|forward AD"):
                 call()
+
+
+@pytest.mark.parametrize("cols", [1, 31, 64, 500, 4096, 33000])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_norm_whose_output_has_no_gradient(dtype, cols):
+    """Only h is used: the gradient is h's own, bit for bit, whatever h and the weight hold, and the weight's is zero."""
+    x, r, w = randn(1, 6, cols, dtype=dtype), randn(2, 6, cols, dtype=dtype), randn(3, cols, dtype=dtype)
+    x[1, 0], x[2, cols // 2], r[3, cols - 1], w[cols // 2] = float("inf"), float("nan"), -float("inf"), float("inf")
+    for t in (x, r, w):
+        t.requires_grad_()
+    gh = randn(4, 6, 2 * cols, dtype=dtype)[:, cols:]
+    for f in (lambda: F.rms_norm(x, w, r)[1], lambda: F.rms_norm8(x, w, r).h):
+        gx, gr, gw = torch.autograd.grad(f(), [x, r, w], gh)
+        assert torch.equal(gx, gh) and torch.equal(gr, gh) and torch.equal(gw, torch.zeros_like(w))
+
+
+def test_abi_norm_backward_without_gradients():
+    """grad_y and grad_h both null: zeros."""
+    from morphocore_amd import _native
+
+    h, w, rstd = randn(1, 5, 77), randn(2, 77), torch.full((5,), float("nan"), device=DEV)
+    gx, gw = torch.full((5, 77), 7.0, device=DEV), torch.full((77,), 7.0, device=DEV)
+    lib = _native.lib()
+    need = lib.mca_rms_norm_backward_workspace_size(5, 77)
+    ws = torch.empty(need, dtype=torch.uint8, device=DEV)
+    rc = lib.mca_rms_norm_backward(0, 0, None, 0, None, 0, h.data_ptr(), 77, w.data_ptr(), rstd.data_ptr(), gx.data_ptr(), gw.data_ptr(), 5, 77,
+                                   ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0 and not gx.any() and not gw.any()

@@ -107,11 +107,13 @@ __device__ __forceinline__ TwoTerms rstd_of(float sum, double inv, float eps)
 }
 
 // v q w with one rounding at the end: the products' errors go along. Two roundings would move a value across a
-// rounding boundary of 16 or 8 bits several times as often.
+// rounding boundary of 16 or 8 bits several times as often. Where the errors make a NaN (0 or an infinity of the other sign
+// times an infinite weight) they are left out; the products alone make one only where v q w is one.
 __device__ __forceinline__ float scaled(float v, TwoTerms q, float w)
 {
     const float n = v * q.hi;
-    return fmaf(n, w, fmaf(v, q.lo, fmaf(v, q.hi, -n)) * w);
+    const float y = fmaf(n, w, fmaf(v, q.lo, fmaf(v, q.hi, -n)) * w);
+    return y == y ? y : n * w;
 }
 
 // A lane's values of a row as stored.

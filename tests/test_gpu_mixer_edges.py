@@ -184,3 +184,21 @@ def test_abi_norm_backward_without_gradients():
     rc = lib.mca_rms_norm_backward(0, 0, None, 0, None, 0, h.data_ptr(), 77, w.data_ptr(), rstd.data_ptr(), gx.data_ptr(), gw.data_ptr(), 5, 77,
                                    ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream)
     assert rc == 0 and not gx.any() and not gw.any()
+
+
+@pytest.mark.parametrize("cols", [3, 64, 500, 4096, 33000])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_norm_of_weights_and_rows_that_are_not_finite(dtype, cols):
+    """y is h * rstd * weight, infinite where the weight is and NaN only where that is NaN: an infinite weight on a zero, a NaN weight,
+    a row with an infinity (rstd 0) or a NaN."""
+    x, w = randn(1, 7, cols, dtype=dtype), randn(2, cols, dtype=torch.float32)
+    w[0], w[cols // 2], w[cols - 1] = float("inf"), -float("inf"), float("nan")
+    x[1, 0], x[2, 1], x[3, 1], x[4] = 0, float("inf"), float("nan"), 0
+    for wt in (w, w.to(dtype)):
+        v = x.double()
+        want = v / torch.sqrt(v.square().mean(-1, keepdim=True) + 1e-6) * wt.double()
+        for y in (F.rms_norm(x, wt), F.rms_norm8(x, wt).y, F.rms_norm(x, wt, torch.zeros_like(x))[0]):
+            same = torch.isnan(want) == torch.isnan(y)
+            assert same.all() and torch.equal(torch.isinf(want), torch.isinf(y))
+            infinite = torch.isinf(want)
+            assert torch.equal(y[infinite].double(), want[infinite])

@@ -1,5 +1,7 @@
-"""The channel-mixing operators on the GPU where their results are easily lost: checkpoints of modules that
-draw numbers, captured steps."""
+"""The channel-mixing operators on the GPU where their results are easily lost: checkpoints of modules that draw
+numbers, write to their input or run under autocast, captured steps, empty tensors, missing gradients, values that
+are not finite, the norm's gradients against the sum that its forward took, its widest rows."""
+import numpy as np
 import pytest
 import torch
 
@@ -202,3 +204,68 @@ def test_norm_of_weights_and_rows_that_are_not_finite(dtype, cols):
             assert same.all() and torch.equal(torch.isinf(want), torch.isinf(y))
             infinite = torch.isinf(want)
             assert torch.equal(y[infinite].double(), want[infinite])
+
+
+def test_checkpoint_of_a_module_that_writes_to_its_input():
+    torch.manual_seed(0)
+    net = torch.nn.Sequential(torch.nn.LeakyReLU(0.1, inplace=True), torch.nn.Linear(64, 48)).to(DEV)
+    x, gy = F.unpack8(F.pack8(randn(1, 9, 64))), randn(2, 9, 48)  # values that a checkpoint holds exactly
+    results = []
+    for call in (net, lambda t: F.checkpoint8(net, t)):
+        a = x.clone().requires_grad_()
+        b = a * 1.0
+        out = call(b)
+        got = [b, out, *torch.autograd.grad([out, b], [a, *net.parameters()], [gy, x])]
+        out = call(x.clone())
+        results.append([*got, *torch.autograd.grad(out, net.parameters(), gy)])
+    for plain, kept in zip(*results):
+        assert torch.equal(plain, kept)
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 40), (2000, 777), (50, 4096), (7, 33000)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_norm_gradients_against_the_unrounded_sum(dtype, rows, cols):
+    """The backward reads h as stored: its gradients are those of the sum x + residual that the forward normalised but for h's
+    rounding, at most u of each h.
+
+    Elementwise, with u the unit roundoff: u of the sum of the terms' magnitudes in the weight's gradient and twice u of n's share
+    in the input's, besides the bounds of the gradients at the stored h (64 units of 2^-24 of the terms, sums over rows
+    2 sqrt(rows) + 16, the output's u). Over all of the weight's gradient, two independent roundings of at most u / sqrt(3)
+    by norm each (h's and the output's): sqrt(2 / 3) u.
+    """
+    u, f = {torch.float16: 2.0**-11, torch.bfloat16: 2.0**-8}[dtype], 2.0**-24
+    x, r, w = randn(1, rows, cols, dtype=dtype).requires_grad_(), randn(2, rows, cols, dtype=dtype), (1 + 0.2 * randn(3, cols)).to(dtype).requires_grad_()
+    gy = randn(4, rows, cols, dtype=dtype, scale=0.1)
+    y, h = F.rms_norm(x, w, r, 1e-5)
+    gx, gw = torch.autograd.grad(y, [x, w], gy)
+    s, a = x.detach().double() + r.double(), gy.double() * w.detach().double()
+    rstd = 1 / torch.sqrt(s.square().mean(-1, keepdim=True) + 1e-5)
+    n = s * rstd
+    want = rstd * (a - n * (a * n).mean(-1, keepdim=True))
+    share = rstd * n.abs() * (a * n).abs().mean(-1, keepdim=True)
+    size = 64 * f * (rstd * a.abs() + share) + (2 * u + u * u) * share
+    assert ((gx.double() - want).abs() <= size + u * (want.abs() + size) + 2.0**-25).all()
+    terms = gy.double() * n
+    want, size = terms.sum(0), (u + (2 * np.sqrt(rows) + 16) * f) * terms.abs().sum(0)
+    assert ((gw.double() - want).abs() <= size + u * (want.abs() + size) + 2.0**-25).all()
+    if rows >= 50:
+        assert (gw.double() - want).norm() <= np.sqrt(2 / 3) * u * want.norm()
+
+
+@pytest.mark.parametrize("cols", [16384, 16385, 32801, 100003, 500009])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_norm_of_the_widest_rows(dtype, cols):
+    """A lane's sum has 8 ceil(units / 1024) terms, which grows with the width: the sum of squares is off by that many units
+    of 2^-24 and 10 of the tree, half of which the root leaves; 8 more for the root, the division and the products. float16's
+    subnormal results add half their spacing."""
+    f, u = 2.0**-24, {torch.float32: 2.0**-24, torch.float16: 2.0**-11, torch.bfloat16: 2.0**-8}[dtype]
+    half_spacing = 2.0**-25 if dtype == torch.float16 else 0.0
+    x, r, w = randn(1, 3, cols, dtype=dtype), randn(2, 3, cols, dtype=dtype), (1 + 0.2 * randn(3, cols)).to(dtype)
+    s = x.double() + r.double()
+    want = s / torch.sqrt(s.square().mean(-1, keepdim=True) + 1e-6) * w.double()
+    terms = 8 * -(-(-(-cols // 8)) // 1024)
+    y, h = F.rms_norm(x, w, r)
+    # The float32 sum x + residual rounds once more.
+    far = (y.double() - want).abs() - (((terms + 10) / 2 + 8) * f + u) * want.abs() - f * (x.double().abs() + r.double().abs())
+    assert (far[want.abs() >= 2.0**-14] <= 0).all() and (far <= half_spacing).all()
+    assert torch.equal(h, (x.float() + r.float()).to(dtype))

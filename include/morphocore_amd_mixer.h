@@ -41,7 +41,8 @@ int mca_rms_norm_forward(int dtype, int weight_dtype, const void* x, int64_t x_s
                          int64_t cols, void* stream);
 
 /* grad_x (also the residual's gradient) and grad_weight from grad_y, grad_h (the gradient of h as an output),
- * h and rstd. grad_y, grad_h, grad_x and grad_weight may be NULL. */
+ * h and rstd. grad_y, grad_h, grad_x and grad_weight may be NULL; without grad_y, grad_x is grad_h (or zeros) whatever h
+ * holds, and grad_weight zeros. */
 size_t mca_rms_norm_backward_workspace_size(int64_t rows, int64_t cols);
 int mca_rms_norm_backward(int dtype, int weight_dtype, const void* grad_y, int64_t grad_y_stride, const void* grad_h, int64_t grad_h_stride,
                           const void* h, int64_t h_stride, const void* weight, const float* rstd, void* grad_x, void* grad_weight,

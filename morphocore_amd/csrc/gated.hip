@@ -97,7 +97,10 @@ __global__ __launch_bounds__(BLOCK) void copy_rows_kernel(const T* __restrict__ 
 }
 
 // The library's exponential for float32; the hardware's, whose error grows with the argument to a few
-// float32 units in the last place, where the result is rounded to 16 bits.
+// float32 units in the last place, where the result is rounded to 16 bits (y of 8192 x 8192 bfloat16 is as far from
+// float64 with either, 0.00165; with the library's, gated_silu8 of it takes 119 us for 110, of 1999 x 2731 float16 14.4
+// for 13.1). g * sigmoid rounds once more in float32 than g / (1 + e) would (y 4.9e-8 from float64 for 4.6e-8), whose
+// division takes gated_silu8 of 8192 x 8192 float32 from 176 to 186 us.
 template <typename T>
 __device__ __forceinline__ float sigmoid_of(float g)
 {

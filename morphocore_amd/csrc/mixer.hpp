@@ -52,7 +52,7 @@ template <typename T, typename OT>
 hipError_t grad_weight8(const T* grad_y, int64_t gy_stride, const uint8_t* codes, const uint8_t* scales, OT* grad_weight, int64_t rows,
                         int out, int cols, void* workspace, hipStream_t stream);
 
-// out[j] = the sum of part[s * n + j] over the slots s, in slot order (in float64), rounded once.
+// out[j] = the sum of part[s * n + j] over the slots s, in a fixed order (in float64), rounded once.
 template <typename OT>
 hipError_t sum_slots_async(const float* part, int nslots, int64_t n, OT* out, hipStream_t stream);
 

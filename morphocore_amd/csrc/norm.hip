@@ -8,12 +8,14 @@
 // an image's channels, so that a wave carries several rows; a workgroup for wide ones), so that a lane holds
 // one unit where that is possible: registers are what limits the waves, and waves are what keeps loads in
 // flight (loading a row ahead instead was slower). Copies of this size run at 5.2 TB/s read and written.
-// Measured, bfloat16 with a residual and the 8-bit form: 8192 x 4096 forward 56 us (5.4 TB/s), backward with
-// grad_w 54 us (5.0); float32 without, 524288 x 64: 46 us (5.8) and 82 us (4.9). One row of 4096: 3.7 us.
+// Measured in training steps, bfloat16 with a residual and the 8-bit form: 8192 x 4096 forward 55 us (5.5 TB/s; 46
+// alone, launched back to back), backward 56 us (4.8) and 7 for grad_w's slots (50 alone, with them); float32 without,
+// 524288 x 64: 54 us (5.0) and 66 us (6.1, part of it from the cache) and 6. One row of 4096: 3.3 us.
 //
 // The forward normalises the float32 sum x + residual, not its rounded h (one rounding fewer), and rounds y
 // once. The backward reads h as stored: x and the residual again would be a quarter more to read and a tensor
-// more to keep, for a 16-bit grad_w that is 0.0017 from the exact one, its own rounding, instead of 0.0024.
+// more to keep, for a bfloat16 grad_w that is 0.0017 from the exact one, its own rounding, instead of 0.0025 (float16
+// 0.00021 instead of 0.00031). grad_x, where h's rounding enters through n's share alone, is as near as with the exact h.
 #include "block8.hpp"
 #include "launch.hpp"
 #include "mixer.hpp"
@@ -436,8 +438,9 @@ hipError_t rms_norm_forward(const T* x, int64_t x_stride, const T* residual, int
 {
     if (rows <= 0 || cols <= 0) return hipSuccess;
     const int units = units_of(cols);
-    // (A norm alone in float32, two stores a lane, is up to 8 us slower of 42 at 524288 x 64; its training step, whose
-    // backward then finds x in the cache, takes 123 us for 137.)
+    // (Of a float32 unit's two stores each is half a line, which past the caches costs a norm without residual, launched
+    // alone, up to 6 us: 8192 x 4096 50 us for 43; 524288 x 64 47 for 49. Its training step, whose backward then finds x in the
+    // cache, takes 123 us for 137, which is why float32 is not excepted here as it is where nothing is read again, in unpack8.)
     const bool streaming = streams((double)rows * cols * (sizeof(T) * (1.0 + !!residual + !!y + !!h) + !!codes));
     if (units > NORM_MAX_UNITS)
     {
@@ -455,9 +458,12 @@ hipError_t rms_norm_forward(const T* x, int64_t x_stride, const T* residual, int
 
 // Slots of grad_w's partial sums, one a workgroup of the backward: about as many threads as the 256 CUs hold at once by
 // their registers. Fewer leave loads unissued, more leave a last round half empty and make more slots to
-// add (8192 x 4096 bfloat16, 256 lanes of 2 units: 58 us with 1024 workgroups, 70 with 512; 2048 x 8192, 256 lanes of
-// 4: 48 with 1024, 39 with 512; both with the slots' sum). A workgroup takes two rows at least where that leaves two
-// workgroups for every CU.
+// add. bfloat16 with grad_h and with the slots' sum, by the number of workgroups:
+//   8192 x 4096 (512 lanes of 1 unit): 62 us with 256, 50 with 512, 54 with 1024;
+//   2048 x 8192 (1024 of 1): 39 us with 128, 33 with 256, 39 with 512;  16384 x 2048 (256 of 1): 59 with 512, 51 with 1024, 55 with 1536;
+//   65536 x 512 (64 of 1): 57 us with 512, 48 with 1024, 47 with 1536, 56 with 2048;
+//   4096 x 11000 (512 of 3): 162 us with 128, 97 with 256, 111 with 512;  2048 x 16384 (1024 of 2): 61 with 128, 53 with 256, 69 with 512.
+// A workgroup takes two rows at least where that leaves two workgroups for every CU.
 static int norm_slots(int64_t rows, int cols)
 {
     const int units = units_of(cols);

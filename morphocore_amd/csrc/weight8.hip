@@ -15,12 +15,13 @@
 // the way into LDS, once for the workgroup.
 //
 // Rows are split over workgroups where the output has too few tiles for the 256 CUs; each split writes its
-// float32 sums to a slot, and the slots are added in order (no atomics: the same result every time).
+// float32 sums to a slot, and the slots are added in a fixed order (no atomics: the same result every time).
 //
-// Measured: 8192 x 4096 x 4096 (rows, out, columns) bfloat16 234 us, 1172 TFLOP/s, where the library's bfloat16
-// product of 8192^3, the fastest measured, runs at 1202 and its product of these operands unpacked takes 287 us;
-// float16 452 us (1216 TFLOP/s of bfloat16 products), float32 667 us (1237). 524288 x 64 x 64 float32 36 us
-// (4.5 TB/s), bound by HBM. Tiles in between are bound by latency: 5003 x 1111 x 777 float16 36 us.
+// Measured: 8192 x 4096 x 4096 (rows, out, columns) bfloat16 248 us among other work, 1109 TFLOP/s (234 to 244 launched back to
+// back), where the library's bfloat16 product of 8192^3, the fastest measured, runs at 1202 and its product of these operands
+// unpacked takes 287 us; back to back float16 452 to 463 us (1187 to 1216 TFLOP/s of bfloat16 products), float32 667 to 681 us
+// (1211 to 1237). 524288 x 64 x 64 float32 36 us (4.5 TB/s), bound by HBM, and 6 for the slots. Tiles in between are bound by
+// latency: 5003 x 1111 x 777 float16 32 us and 6.
 #include "block8.hpp"
 #include "launch.hpp"
 #include "mixer.hpp"
@@ -360,6 +361,9 @@ constexpr int64_t SPLIT_ROWS = 48, SPLIT_MOST = 1 << 30;
 // slots' way to memory and back. The estimate picks within 2% of the best of all on average over 41
 // measured shapes; one rule of thumb (the largest tile, splits up to two workgroups a CU) was 35% off
 // (2048 x 2048 x 2048 bfloat16: 52 us against 27 with middle tiles unsplit; 16384 x 512 x 512: 40 against 27 with small ones).
+// The slots have one rate here, though their sum's loads come in whole rounds of its threads (17 slots cost what 128 do), so
+// between 17 and 128 splits it can pick a slower plan: 20000 x 128 x 1000 float32 39 us with the middle tile's 32 splits, 36
+// with the small one's 16.
 static WeightPlan weight_plan(int planes, int64_t rows, int out, int cols)
 {
     WeightPlan best{};

@@ -12,8 +12,11 @@
 // alone, launched back to back), backward 56 us (4.8) and 7 for grad_w's slots (50 alone, with them); float32 without,
 // 524288 x 64: 54 us (5.0) and 66 us (6.1, part of it from the cache) and 6. One row of 4096: 3.3 us.
 //
-// The forward normalises the float32 sum x + residual, not its rounded h (one rounding fewer), and rounds y
-// once. The backward reads h as stored: x and the residual again would be a quarter more to read and a tensor
+// The forward normalises the float32 sum x + residual, not its rounded h (one rounding fewer), sums the squares in
+// float64 and rounds y once: of float32 it is the correctly rounded value but for 2^-42, and of 16 bits hardly ever another
+// one's neighbour, whose 8-bit code may be another too. (Float32 sums moved one y in 100000 across a rounding boundary of 16 bits. The
+// wider ones cost nothing up to 4096 columns, 1 us of 28 at 2048 x 8192 bfloat16 and 2 of 52 at 2048 x 16384.)
+// The backward reads h as stored: x and the residual again would be a quarter more to read and a tensor
 // more to keep, for a bfloat16 grad_w that is 0.0017 from the exact one, its own rounding, instead of 0.0025 (float16
 // 0.00021 instead of 0.00031). grad_x, where h's rounding enters through n's share alone, is as near as with the exact h.
 #include "block8.hpp"
@@ -46,46 +49,62 @@ __device__ __forceinline__ int row_of_lane()
     return threadIdx.x / G;
 }
 
-template <int CTRL>
-__device__ __forceinline__ float dpp_add(float s)
+// A sum (float or double) as the 32-bit registers that lane exchanges move.
+template <typename S>
+struct Words
 {
-    return s + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(s), CTRL, 0xf, 0xf, true));
+    static constexpr int N = sizeof(S) / 4;
+    uint32_t w[N];
+};
+
+template <int CTRL, typename S>
+__device__ __forceinline__ S dpp_add(S s)
+{
+    Words<S> a = __builtin_bit_cast(Words<S>, s);
+#pragma unroll
+    for (int i = 0; i < a.N; ++i) a.w[i] = (uint32_t)__builtin_amdgcn_mov_dpp((int)a.w[i], CTRL, 0xf, 0xf, true);
+    return s + __builtin_bit_cast(S, a);
+}
+
+template <bool HALVES, typename S>
+__device__ __forceinline__ S swap_add(S s)
+{
+    Words<S> a = __builtin_bit_cast(Words<S>, s), b = a;
+#pragma unroll
+    for (int i = 0; i < a.N; ++i)
+    {
+        const auto t = HALVES ? __builtin_amdgcn_permlane32_swap(a.w[i], a.w[i], false, false) : __builtin_amdgcn_permlane16_swap(a.w[i], a.w[i], false, false);
+        a.w[i] = t[0], b.w[i] = t[1];
+    }
+    return __builtin_bit_cast(S, a) + __builtin_bit_cast(S, b);
 }
 
 // The sum over G consecutive lanes (a power of two up to the wave), in every one of them, on the vector unit.
-template <int G>
-__device__ __forceinline__ float lane_sum(float s)
+template <int G, typename S>
+__device__ __forceinline__ S lane_sum(S s)
 {
     if constexpr (G > 1) s = dpp_add<0xb1>(s);   // lane ^ 1
     if constexpr (G > 2) s = dpp_add<0x4e>(s);   // lane ^ 2
     if constexpr (G > 4) s = dpp_add<0x141>(s);  // the other 4 of 8 (mirrored)
     if constexpr (G > 8) s = dpp_add<0x140>(s);  // the other 8 of 16 (mirrored)
-    if constexpr (G > 16)
-    {
-        const auto t = __builtin_amdgcn_permlane16_swap(__float_as_uint(s), __float_as_uint(s), false, false);
-        s = __uint_as_float(t[0]) + __uint_as_float(t[1]);
-    }
-    if constexpr (G > 32)
-    {
-        const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(s), __float_as_uint(s), false, false);
-        s = __uint_as_float(t[0]) + __uint_as_float(t[1]);
-    }
+    if constexpr (G > 16) s = swap_add<false>(s);
+    if constexpr (G > 32) s = swap_add<true>(s);
     return s;
 }
 
 // The sum over the G lanes of a row, in every one of them. `part` holds one value per wave, for two rows in
 // turn (`turn`), so that one barrier a row suffices.
-template <int G>
-__device__ __forceinline__ float row_sum(float s, float* part, int turn)
+template <int G, typename S>
+__device__ __forceinline__ S row_sum(S s, S* part, int turn)
 {
     s = lane_sum<(G < WAVE ? G : WAVE)>(s);
     if constexpr (G > WAVE)
     {
         constexpr int N = G / WAVE;
-        float* p = part + turn * N;
+        S* p = part + turn * N;
         if (threadIdx.x % WAVE == 0) p[threadIdx.x / WAVE] = s;
         __syncthreads();
-        s = 0.0f;
+        s = S(0);
 #pragma unroll
         for (int i = 0; i < N; ++i) s += p[i];
     }
@@ -99,9 +118,9 @@ struct TwoTerms
     float hi, lo;
 };
 
-__device__ __forceinline__ TwoTerms rstd_of(float sum, double inv, float eps)
+__device__ __forceinline__ TwoTerms rstd_of(double sum, double inv, float eps)
 {
-    const double mean = (double)sum * inv + (double)eps;
+    const double mean = sum * inv + (double)eps;
     const float a = (float)mean, al = (float)(mean - (double)a), q = 1.0f / sqrtf(a);
     const float t = q * a, tl = fmaf(q, al, fmaf(q, a, -t));
     const float miss = fmaf(-q, tl, fmaf(-q, t, 1.0f));  // 1 - q^2 mean
@@ -138,7 +157,7 @@ __global__ __launch_bounds__(norm_threads<G>()) void rms_norm_fwd_kernel(const T
                                                                          int cols, bool streaming)
 {
     constexpr int ROWS = norm_threads<G>() / G;
-    __shared__ float part[2 * (G > WAVE ? G / WAVE : 1)];
+    __shared__ double part[2 * (G > WAVE ? G / WAVE : 1)];
     const int lane = threadIdx.x % G, nb = blocks_of(cols);
     const double inv = 1.0 / (double)cols;
     RawUnit<WT> wv[V];
@@ -150,7 +169,7 @@ __global__ __launch_bounds__(norm_threads<G>()) void rms_norm_fwd_kernel(const T
         load_row<T, G, V>(x + row * xs, cols, rx);
         if (r) load_row<T, G, V>(r + row * rs, cols, rr);
         float v[V][UNIT];
-        float s = 0.0f;
+        double s = 0.0;
 #pragma unroll
         for (int k = 0; k < V; ++k)
 #pragma unroll
@@ -158,7 +177,7 @@ __global__ __launch_bounds__(norm_threads<G>()) void rms_norm_fwd_kernel(const T
             {
                 v[k][j] = rx[k][j];
                 if (r) v[k][j] += rr[k][j];
-                s += v[k][j] * v[k][j];
+                s = fma((double)v[k][j], (double)v[k][j], s);
             }
         const TwoTerms q = rstd_of(row_sum<G>(s, part, turn), inv, eps);
         if (rstd && lane == 0) rstd[row] = q.hi;
@@ -187,7 +206,7 @@ __global__ __launch_bounds__(1024) void rms_norm_fwd_wide_kernel(const T* __rest
                                                                  float* __restrict__ rstd, int64_t rows, int cols, bool streaming)
 {
     constexpr int G = 1024;
-    __shared__ float part[2 * G / WAVE];
+    __shared__ double part[2 * G / WAVE];
     const int nb = blocks_of(cols), padded = nb * MX_LANES;
     int turn = 0;
     for (int64_t row = blockIdx.x; row < rows; row += gridDim.x, turn ^= 1)
@@ -205,13 +224,13 @@ __global__ __launch_bounds__(1024) void rms_norm_fwd_wide_kernel(const T* __rest
                 for (int j = 0; j < UNIT; ++j) v[j] += u[j];
             }
         };
-        float s = 0.0f;
+        double s = 0.0;
         for (int unit = threadIdx.x; unit < padded; unit += G)
         {
             float v[UNIT];
             load(unit, v);
 #pragma unroll
-            for (int j = 0; j < UNIT; ++j) s += v[j] * v[j];
+            for (int j = 0; j < UNIT; ++j) s = fma((double)v[j], (double)v[j], s);
         }
         const TwoTerms q = rstd_of(row_sum<G>(s, part, turn), 1.0 / (double)cols, eps);
         if (rstd && threadIdx.x == 0) rstd[row] = q.hi;

@@ -18,7 +18,8 @@ class Normed8(NamedTuple):
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None,
              eps: float = 1e-6) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
     """``y = h / sqrt(mean(h^2) + eps) * weight`` over the last dimension, h = x + residual; returns y, or
-    (y, h) with a residual. One pass over the data forward and one backward, sums in float32.
+    (y, h) with a residual. One pass over the data forward and one backward, sums in float64 forward (y is rounded
+    once) and in float32 backward.
 
     x : [..., C] float32, float16 or bfloat16 on a HIP device.
     weight : [C], of x's type or float32.

@@ -269,3 +269,30 @@ def test_norm_of_the_widest_rows(dtype, cols):
     far = (y.double() - want).abs() - (((terms + 10) / 2 + 8) * f + u) * want.abs() - f * (x.double().abs() + r.double().abs())
     assert (far[want.abs() >= 2.0**-14] <= 0).all() and (far <= half_spacing).all()
     assert torch.equal(h, (x.float() + r.float()).to(dtype))
+
+
+@pytest.mark.parametrize("rows,cols", [(300, 64), (200, 500), (50, 4096), (20, 16384), (9, 33000)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_norm_rounds_its_output_once(dtype, rows, cols):
+    """y is (x + residual, in float32) * rstd * weight rounded to float32 and then to its type.
+
+    What comes before the first rounding: the sum of squares in float64; rstd in two float32 terms, a Newton step from one within 2^-22
+    (its square, 2^-44); their products with v and the weight with the errors carried along, which round once more at 2^-24
+    of 2^-22 each: below 2^-42 in all. float16's subnormal results add half their spacing.
+    """
+    f, first = 2.0**-24, 2.0**-24 + 2.0**-42
+    u = {torch.float32: 0.0, torch.float16: 2.0**-11, torch.bfloat16: 2.0**-8}[dtype]
+    x, r = randn(1, rows, cols, dtype=dtype) * torch.exp(randn(2, rows, 1)).to(dtype), randn(3, rows, cols, dtype=dtype)
+    w = (1 + 0.2 * randn(4, cols)).to(dtype)
+    eps = float(np.float32(1e-6))
+    for residual in (None, r):
+        v = (x.float() if residual is None else x.float() + r.float()).double()
+        want = v / torch.sqrt(v.square().mean(-1, keepdim=True) + eps) * w.double()
+        y = F.rms_norm(x, w, residual, eps)
+        y = (y if residual is None else y[0]).double()
+        spacing = torch.where(want.abs() < 2.0**-14, 2.0**-25, 0.0) if dtype == torch.float16 else 0.0
+        assert ((y - want).abs() <= (first + u * (1 + first)) * want.abs() + spacing).all()
+        # Another value than the rounded float64 one only where the first rounding ends at a midpoint of the type's values: one in 2^13
+        # of float16 and 2^16 of bfloat16 at most, by half a step of float32 each way; four times that many are allowed.
+        if dtype != torch.float32:
+            assert (y != want.to(dtype).double()).double().mean() <= 4 * f / u

@@ -14,7 +14,7 @@
 //
 // The forward normalises the float32 sum x + residual, not its rounded h (one rounding fewer), sums the squares in
 // float64 and rounds y once: of float32 it is the correctly rounded value but for 2^-42, and of 16 bits hardly ever another
-// one's neighbour, whose 8-bit code may be another too. (Float32 sums moved one y in 100000 across a rounding boundary of 16 bits. The
+// one's neighbour, whose 8-bit code may be another too. (Float32 sums moved a few y in 100000 across a rounding boundary of 16 bits. The
 // wider ones cost nothing up to 4096 columns, 1 us of 28 at 2048 x 8192 bfloat16 and 2 of 52 at 2048 x 16384.)
 // The backward reads h as stored: x and the residual again would be a quarter more to read and a tensor
 // more to keep, for a bfloat16 grad_w that is 0.0017 from the exact one, its own rounding, instead of 0.0025 (float16

@@ -1,4 +1,4 @@
-"""ctypes binding of the C ABI in ``include/morphocore_amd.h`` and ``include/morphocore_amd_mixer.h``
+"""ctypes binding of the C ABI in ``include/morphocore_amd.h``, ``include/morphocore_amd_mixer.h`` and ``include/morphocore_amd_tokens.h``
 (``libmorphocore_amd.so``).
 
 The library holds the gfx950 kernels; nothing here computes. Every call enqueues work on the
@@ -91,6 +91,19 @@ MIXER_EXPORTS = (
     "mca_grad_weight8",
 )
 
+# Every symbol include/morphocore_amd_tokens.h declares.
+TOKENS_EXPORTS = (
+    "mca_axial_rotary",
+    "mca_rms_norm_rotary_forward",
+    "mca_rms_norm_rotary_backward_workspace_size",
+    "mca_rms_norm_rotary_backward",
+    "mca_linear_attention_forward_workspace_size",
+    "mca_linear_attention_forward",
+    "mca_linear_attention_backward_workspace_size",
+    "mca_linear_attention_backward",
+    "mca_linear_attention_step",
+)
+
 _lib = None
 
 
@@ -100,6 +113,24 @@ class StackLayer(ctypes.Structure):
                 ("fill", ctypes.c_double), ("out_channels", ctypes.c_int64), ("weight_channels", ctypes.c_int64),
                 ("kh", ctypes.c_int64), ("kw", ctypes.c_int64), ("weight", ctypes.c_void_p), ("alpha", ctypes.c_void_p),
                 ("grad_weight", ctypes.c_void_p), ("grad_alpha", ctypes.c_void_p)]
+
+
+class Heads(ctypes.Structure):
+    """mca_heads: tokens x heads x dim values."""
+    _fields_ = [("data", ctypes.c_void_p), ("batch_stride", ctypes.c_int64), ("token_stride", ctypes.c_int64),
+                ("head_stride", ctypes.c_int64), ("heads", ctypes.c_int64)]
+
+
+class Rotation(ctypes.Structure):
+    """mca_rotation: the tokens' positions and the pairs' frequencies."""
+    _fields_ = [("positions", ctypes.c_void_p), ("position_type", ctypes.c_int), ("rows", ctypes.c_int64), ("axes", ctypes.c_int64),
+                ("pairs", ctypes.c_int64), ("frequencies", ctypes.c_void_p), ("interleaved", ctypes.c_int)]
+
+
+class Sequences(ctypes.Structure):
+    """mca_sequences: a batch of sequences of one length, or packed ones."""
+    _fields_ = [("offsets", ctypes.c_void_p), ("wide", ctypes.c_int), ("count", ctypes.c_int64), ("tokens", ctypes.c_int64)]
+
 
 _I, _I64, _P, _SZ = ctypes.c_int, ctypes.c_int64, ctypes.c_void_p, ctypes.c_size_t
 _GEOM = [_I64] * 8
@@ -129,6 +160,20 @@ def lib() -> ctypes.CDLL:
                        ("mca_grad_weight8", [_I, _I, _P, _I64, _P, _P, _P, _I64, _I64, _I64, _P, _SZ, _P])):
         getattr(so, name).argtypes = args
         getattr(so, name).restype = _I
+    _H, _F = ctypes.POINTER(Heads), ctypes.c_float
+    _R, _S = ctypes.POINTER(Rotation), ctypes.POINTER(Sequences)
+    for name, args, result in (
+            ("mca_axial_rotary", [_I, _H, _P, _I64, _I64, _R, _I, _P], _I),
+            ("mca_rms_norm_rotary_forward", [_I, _I, _H, _H, _P, _P, _F, _P, _P, _I64, _I64, _R, _P], _I),
+            ("mca_rms_norm_rotary_backward_workspace_size", [_I64] * 4, _SZ),
+            ("mca_rms_norm_rotary_backward", [_I, _I, _H, _H, _H, _H, _P, _P, _F, _P, _P, _P, _I64, _I64, _R, _P, _SZ, _P], _I),
+            ("mca_linear_attention_forward_workspace_size", [_I, _S, _I64, _I64, _I64], _SZ),
+            ("mca_linear_attention_forward", [_I, _S, _H, _H, _H, _P, _P, _P, _P, _I64, _I64, _F, _P, _SZ, _P], _I),
+            ("mca_linear_attention_backward_workspace_size", [_I, _S, _I64, _I64, _I64, _I64], _SZ),
+            ("mca_linear_attention_backward", [_I, _S, _H, _P, _H, _H, _H, _P, _P, _P, _P, _P, _P, _I64, _I64, _F, _P, _SZ, _P], _I),
+            ("mca_linear_attention_step", [_I, _H, _H, _H, _P, _P, _I64, _I64, _P, _I, _I64, _P, _I64, _I64, _I64, _F, _P], _I)):
+        getattr(so, name).argtypes = args
+        getattr(so, name).restype = result
     so.mca_rms_norm_backward_workspace_size.argtypes = [_I64, _I64]
     so.mca_rms_norm_backward_workspace_size.restype = _SZ
     so.mca_grad_weight8_workspace_size.argtypes = [_I, _I64, _I64, _I64]

@@ -1,0 +1,374 @@
+// Rotary positions with several axes, alone or with the root-mean-square norm of each head's row before them:
+//   n = x / sqrt(mean(x^2) + eps) * w;  angle_j = sum over the axes of position * frequency_j;
+//   pair j of a row, (a, b) -> (a cos - b sin, b cos + a sin); values behind the last pair stay.
+// Gradients: the rotation by the negative angles gives g, then the norm's, with r = 1 / sqrt(..), m = x r, t = g w:
+//   grad_x = r (t - m mean(t m)),  grad_w = sum over tokens and heads of g m.
+//
+// Bound by HBM: every row is read once and written once. A lane holds 8 pairs (their two halves apart, or side by
+// side) or 16 values behind the last pair, so the lanes of a row exchange only the norm's sums. The lanes of a row take
+// heads of one token in turn and form its 8 angles each once, without a table in memory; queries and keys share
+// them in one launch. Few tokens are spread over more groups of lanes, each with fewer heads.
+//
+// Angles are float64 up to a fraction of a turn: in float32 a position of 100000 would be off by 0.004 radians. What is
+// left of a turn goes through float32 sine and cosine, the rounding of a result.
+#include "block8.hpp"
+#include "lanes.hpp"
+#include "launch.hpp"
+#include "mixer.hpp"
+#include "tokens.hpp"
+
+#include "../../include/morphocore_amd_tokens.h"
+
+namespace mca
+{
+
+// The lanes of a row: of pairs, 8 a lane, then of the values behind them, 16 a lane.
+inline int rotary_lanes(int dim, int pairs) { return (pairs + UNIT - 1) / UNIT + (dim - 2 * pairs + 2 * UNIT - 1) / (2 * UNIT); }
+
+// The two units of a lane.
+struct RowPart
+{
+    int c[2], valid[2], pair, pairs;  // first pair, and how many
+};
+
+__device__ __forceinline__ RowPart row_part(int lane, int dim, const Rotation& r)
+{
+    RowPart p;
+    p.pair = lane * UNIT;
+    p.pairs = min(max(r.pairs - p.pair, 0), UNIT);
+    if (p.pairs > 0)
+    {
+        p.c[0] = r.interleaved ? 2 * p.pair : p.pair;
+        p.c[1] = r.interleaved ? 2 * p.pair + UNIT : r.pairs + p.pair;
+        p.valid[0] = r.interleaved ? min(2 * p.pairs, UNIT) : p.pairs;
+        p.valid[1] = r.interleaved ? max(2 * p.pairs - UNIT, 0) : p.pairs;
+    }
+    else
+    {
+        const int behind = lane - (r.pairs + UNIT - 1) / UNIT;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+        {
+            p.c[i] = 2 * r.pairs + (2 * behind + i) * UNIT;
+            p.valid[i] = min(max(dim - p.c[i], 0), UNIT);
+        }
+    }
+    return p;
+}
+
+// Units as they are stored. A partial one is read as the 8 values that end with it where the row has as many before.
+template <typename T>
+__device__ __forceinline__ void load_part(const T* __restrict__ row, const RowPart& p, RawUnit<T> (&u)[2])
+{
+#pragma unroll
+    for (int i = 0; i < 2; ++i) load_raw(row + p.c[i], p.c[i] + p.valid[i] >= UNIT, p.valid[i], u[i]);
+}
+
+template <typename T>
+__device__ __forceinline__ void store_part(T* __restrict__ row, const RowPart& p, const float (&v)[2][UNIT], bool streaming)
+{
+#pragma unroll
+    for (int i = 0; i < 2; ++i) store_unit(row + p.c[i], p.valid[i], v[i], streaming);
+}
+
+struct Turn
+{
+    float cos[UNIT], sin[UNIT];
+};
+
+__device__ __forceinline__ Turn turn_of(const Rotation& r, int64_t token, const RowPart& p, bool inverse)
+{
+    const int64_t row = token < r.rows ? token : token % r.rows;
+    double angle[UNIT] = {};
+    for (int a = 0; a < r.axes; ++a)
+    {
+        const int64_t at = row * r.axes + a;
+        const double position = r.position_type == MCA_POSITION_INT32   ? (double)((const int32_t*)r.positions)[at]
+                                : r.position_type == MCA_POSITION_INT64 ? (double)((const int64_t*)r.positions)[at]
+                                                                        : (double)((const float*)r.positions)[at];
+#pragma unroll
+        for (int e = 0; e < UNIT; ++e)
+            if (e < p.pairs) angle[e] = fma(position, r.frequencies[(int64_t)a * r.pairs + p.pair + e], angle[e]);
+    }
+    Turn t;
+#pragma unroll
+    for (int e = 0; e < UNIT; ++e)
+    {
+        const double turns = angle[e] * 0.15915494309189535;  // 1 / (2 pi)
+        sincospif((float)(2.0 * (turns - rint(turns))), &t.sin[e], &t.cos[e]);
+        if (inverse) t.sin[e] = -t.sin[e];
+    }
+    return t;
+}
+
+// Of a lane behind the pairs the angles are 0, which leaves its values as they are (but for a NaN beside an infinity).
+__device__ __forceinline__ void rotate(float (&v)[2][UNIT], const Turn& t, bool interleaved, bool turned)
+{
+    if (!turned) return;
+    if (interleaved)
+    {
+#pragma unroll
+        for (int e = 0; e < UNIT; ++e)
+        {
+            float &a = v[e / 4][2 * e % UNIT], &b = v[e / 4][2 * e % UNIT + 1];
+            const float x = a * t.cos[e] - b * t.sin[e];
+            b = b * t.cos[e] + a * t.sin[e];
+            a = x;
+        }
+    }
+    else
+    {
+#pragma unroll
+        for (int e = 0; e < UNIT; ++e)
+        {
+            float &a = v[0][e], &b = v[1][e];
+            const float x = a * t.cos[e] - b * t.sin[e];
+            b = b * t.cos[e] + a * t.sin[e];
+            a = x;
+        }
+    }
+}
+
+enum RotaryMode
+{
+    ROTATE,
+    NORM_FORWARD,
+    NORM_BACKWARD
+};
+
+// One tensor of the call: x (or the gradient of the result, with the norm's input in `h`), its scale and its result.
+template <typename T, typename WT>
+struct RotaryTensor
+{
+    HeadRows<T> x, h;
+    const WT* w;
+    T* out;
+};
+
+template <typename T, typename WT, int G, int MODE>
+__global__ __launch_bounds__(BLOCK) void rotary_kernel(RotaryTensor<T, WT> q, RotaryTensor<T, WT> k, int64_t tokens, int splits, int dim,
+                                                       Rotation r, bool inverse, float eps, float* __restrict__ gw_part, bool streaming)
+{
+    constexpr int GROUPS = BLOCK / G;
+    const int lane = threadIdx.x % G;
+    const RowPart part = row_part(lane, dim, r);
+    const float inv = 1.0f / (float)dim;
+    const int64_t groups = tokens * splits;
+    float gw[2][2][UNIT] = {};
+    for (int64_t group = (int64_t)blockIdx.x * GROUPS + threadIdx.x / G; group < groups; group += (int64_t)gridDim.x * GROUPS)
+    {
+        const int64_t token = group / splits;
+        const int split = (int)(group - token * splits);
+        const Turn turn = turn_of(r, token, part, inverse);
+#pragma unroll
+        for (int which = 0; which < 2; ++which)
+        {
+            const RotaryTensor<T, WT>& t = which ? k : q;
+            RawUnit<WT> w[2];
+            if (MODE != ROTATE && t.x.heads > 0) load_part(t.w, part, w);
+            // The second tensor's heads go on where the first one's end, so that the groups have equal shares.
+            const int first = which ? (splits - q.x.heads % splits + split) % splits : split;
+            for (int head = first; head < t.x.heads; head += splits)
+            {
+                RawUnit<T> raw[2], rawh[2];
+                load_part(t.x.x + token * t.x.token_stride + head * t.x.head_stride, part, raw);
+                if (MODE == NORM_BACKWARD) load_part(t.h.x + token * t.h.token_stride + head * t.h.head_stride, part, rawh);
+                float v[2][UNIT];
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < UNIT; ++j) v[i][j] = raw[i][j];
+                if constexpr (MODE == NORM_FORWARD)
+                {
+                    float s = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int j = 0; j < UNIT; ++j) s = fmaf(v[i][j], v[i][j], s);
+                    const float rstd = 1.0f / sqrtf(fmaf(lane_sum<G>(s), inv, eps));
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int j = 0; j < UNIT; ++j) v[i][j] = v[i][j] * rstd * w[i][j];
+                }
+                rotate(v, turn, r.interleaved, part.pairs > 0);
+                if constexpr (MODE == NORM_BACKWARD)
+                {
+                    float s = 0.0f, d = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int j = 0; j < UNIT; ++j)
+                        {
+                            s = fmaf(rawh[i][j], rawh[i][j], s);
+                            d = fmaf(v[i][j] * w[i][j], rawh[i][j], d);
+                        }
+                    const float rstd = 1.0f / sqrtf(fmaf(lane_sum<G>(s), inv, eps));
+                    const float mean = lane_sum<G>(d) * rstd * inv;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int j = 0; j < UNIT; ++j)
+                        {
+                            const float m = rawh[i][j] * rstd;
+                            gw[which][i][j] = fmaf(v[i][j], m, gw[which][i][j]);
+                            v[i][j] = rstd * (v[i][j] * w[i][j] - m * mean);
+                        }
+                }
+                if (t.out) store_part(t.out + (token * t.x.heads + head) * dim, part, v, streaming);
+            }
+        }
+    }
+    if constexpr (MODE == NORM_BACKWARD)
+    {
+        if (!gw_part) return;
+        // Over the groups of a wave, then over the waves, in a fixed order, into the workgroup's slot.
+        __shared__ float sums[NWAVES][2][G][2 * UNIT];
+#pragma unroll
+        for (int which = 0; which < 2; ++which)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < UNIT; ++j)
+                {
+                    float s = gw[which][i][j];
+#pragma unroll
+                    for (int d = G; d < WAVE; d *= 2) s += __shfl_xor(s, d);
+                    if (threadIdx.x % WAVE < G) sums[threadIdx.x / WAVE][which][lane][i * UNIT + j] = s;
+                }
+        __syncthreads();
+        float* __restrict__ out = gw_part + (int64_t)blockIdx.x * 2 * dim;
+        for (int which = threadIdx.x / WAVE; which < 2; which += NWAVES)
+            for (int l = threadIdx.x % WAVE; l < G; l += WAVE)
+            {
+                const RowPart p = row_part(l, dim, r);
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < UNIT; ++j)
+                        if (j < p.valid[i])
+                        {
+                            const int at = i * UNIT + j;
+                            out[which * dim + p.c[i] + j] = ((sums[0][which][l][at] + sums[1][which][l][at]) + sums[2][which][l][at]) + sums[3][which][l][at];
+                        }
+            }
+    }
+}
+
+// Groups of lanes that a launch aims at: 4 waves for each of the 1024 SIMDs.
+static int rotary_splits(int64_t tokens, int heads, int lanes)
+{
+    const int64_t want = 4096 * (int64_t)(WAVE / lanes), s = (want + tokens - 1) / tokens;
+    return (int)(s < 1 ? 1 : s > heads ? heads : s);
+}
+
+template <typename F>
+static hipError_t by_lanes(int lanes, F&& f)
+{
+    using std::integral_constant;
+    if (lanes <= 1) return f(integral_constant<int, 1>());
+    if (lanes <= 2) return f(integral_constant<int, 2>());
+    if (lanes <= 4) return f(integral_constant<int, 4>());
+    if (lanes <= 8) return f(integral_constant<int, 8>());
+    if (lanes <= 16) return f(integral_constant<int, 16>());
+    if (lanes <= 32) return f(integral_constant<int, 32>());
+    return f(integral_constant<int, 64>());
+}
+
+struct RotaryPlan
+{
+    int splits, blocks;
+};
+
+// Slots of grad_w's partial sums: one a workgroup.
+template <int G>
+static RotaryPlan rotary_plan(int64_t tokens, int heads, int64_t most)
+{
+    RotaryPlan p;
+    p.splits = rotary_splits(tokens, heads, G);
+    const int64_t groups = tokens * p.splits, blocks = (groups + BLOCK / G - 1) / (BLOCK / G);
+    p.blocks = (int)(blocks < most ? blocks : most);
+    return p;
+}
+
+constexpr int64_t ROTARY_BLOCKS = 1 << 20, ROTARY_SLOTS = 1024;
+
+template <int MODE, typename T, typename WT>
+static hipError_t rotary_launch(const RotaryTensor<T, WT>& q, const RotaryTensor<T, WT>& k, int64_t tokens, int dim, const Rotation& r, bool inverse,
+                                float eps, float* gw_part, hipStream_t stream)
+{
+    const int heads = q.x.heads + k.x.heads;
+    const double values = (double)tokens * heads * dim;
+    const bool streaming = streams(values * sizeof(T) * (MODE == NORM_BACKWARD ? 3.0 : 2.0));
+    return by_lanes(rotary_lanes(dim, r.pairs), [&](auto g) {
+        constexpr int G = decltype(g)::value;
+        const RotaryPlan p = rotary_plan<G>(tokens, heads, MODE == NORM_BACKWARD ? ROTARY_SLOTS : ROTARY_BLOCKS);
+        rotary_kernel<T, WT, G, MODE><<<p.blocks, BLOCK, 0, stream>>>(q, k, tokens, p.splits, dim, r, inverse, eps, gw_part, streaming);
+        return hipGetLastError();
+    });
+}
+
+template <typename T>
+hipError_t axial_rotary(HeadRows<T> x, T* out, int64_t tokens, int dim, const Rotation& r, bool inverse, hipStream_t stream)
+{
+    if (tokens <= 0 || x.heads <= 0) return hipSuccess;
+    const RotaryTensor<T, T> q = {x, {}, nullptr, out}, none = {};
+    return rotary_launch<ROTATE>(q, none, tokens, dim, r, inverse, 0.0f, nullptr, stream);
+}
+
+template <typename T, typename WT>
+hipError_t rms_norm_rotary_forward(HeadRows<T> q, HeadRows<T> k, const WT* q_weight, const WT* k_weight, float eps, T* out_q, T* out_k,
+                                   int64_t tokens, int dim, const Rotation& r, hipStream_t stream)
+{
+    if (tokens <= 0 || q.heads + k.heads <= 0) return hipSuccess;
+    const RotaryTensor<T, WT> tq = {q, {}, q_weight, out_q}, tk = {k, {}, k_weight, out_k};
+    return rotary_launch<NORM_FORWARD>(tq, tk, tokens, dim, r, false, eps, nullptr, stream);
+}
+
+static int rotary_slots(int64_t tokens, int heads, int dim, int pairs)
+{
+    int slots = 0;
+    (void)by_lanes(rotary_lanes(dim, pairs), [&](auto g) {
+        slots = rotary_plan<decltype(g)::value>(tokens, heads, ROTARY_SLOTS).blocks;
+        return hipSuccess;
+    });
+    return slots;
+}
+
+size_t rms_norm_rotary_backward_workspace(int64_t tokens, int heads, int dim, int pairs)
+{
+    return tokens > 0 && heads > 0 ? align_up((size_t)rotary_slots(tokens, heads, dim, pairs) * 2 * (size_t)dim * sizeof(float)) : 0;
+}
+
+template <typename T, typename WT>
+hipError_t rms_norm_rotary_backward(HeadRows<T> gy_q, HeadRows<T> gy_k, HeadRows<T> q, HeadRows<T> k, const WT* q_weight, const WT* k_weight,
+                                    float eps, T* grad_q, T* grad_k, WT* grad_weights, int64_t tokens, int dim, const Rotation& r,
+                                    void* workspace, hipStream_t stream)
+{
+    const bool none = tokens <= 0 || q.heads + k.heads <= 0;
+    float* part = grad_weights && !none ? (float*)workspace : nullptr;
+    if (!none)
+    {
+        const RotaryTensor<T, WT> tq = {gy_q, q, q_weight, grad_q}, tk = {gy_k, k, k_weight, grad_k};
+        const hipError_t err = rotary_launch<NORM_BACKWARD>(tq, tk, tokens, dim, r, true, eps, part, stream);
+        if (err != hipSuccess) return err;
+    }
+    if (!grad_weights) return hipSuccess;
+    return sum_slots_async<WT>(part, none ? 0 : rotary_slots(tokens, q.heads + k.heads, dim, r.pairs), 2 * (int64_t)dim, grad_weights, stream);
+}
+
+#define MCA_ROTARY(T, WT)                                                                                                                    \
+    template hipError_t rms_norm_rotary_forward<T, WT>(HeadRows<T>, HeadRows<T>, const WT*, const WT*, float, T*, T*, int64_t, int,          \
+                                                       const Rotation&, hipStream_t);                                                        \
+    template hipError_t rms_norm_rotary_backward<T, WT>(HeadRows<T>, HeadRows<T>, HeadRows<T>, HeadRows<T>, const WT*, const WT*, float, T*, \
+                                                        T*, WT*, int64_t, int, const Rotation&, void*, hipStream_t)
+template hipError_t axial_rotary<float>(HeadRows<float>, float*, int64_t, int, const Rotation&, bool, hipStream_t);
+template hipError_t axial_rotary<_Float16>(HeadRows<_Float16>, _Float16*, int64_t, int, const Rotation&, bool, hipStream_t);
+template hipError_t axial_rotary<__bf16>(HeadRows<__bf16>, __bf16*, int64_t, int, const Rotation&, bool, hipStream_t);
+MCA_ROTARY(float, float);
+MCA_ROTARY(_Float16, _Float16);
+MCA_ROTARY(_Float16, float);
+MCA_ROTARY(__bf16, __bf16);
+MCA_ROTARY(__bf16, float);
+
+}  // namespace mca

@@ -4,10 +4,10 @@
 
 Two shared libraries, both written for gfx950 only:
   * morphocore_amd/libmorphocore_amd.so — the hand-written HIP kernels and their C ABI
-    (include/morphocore_amd.h, include/morphocore_amd_mixer.h), compiled by hipcc with --offload-arch=gfx950; it depends only on the
+    (include/morphocore_amd.h, include/morphocore_amd_mixer.h, include/morphocore_amd_tokens.h), compiled by hipcc with --offload-arch=gfx950; it depends only on the
     HIP runtime;
   * morphocore_amd/_C*.so — the PyTorch-ROCm extension that registers torch.ops.morphocore.* and its
-    C++ autograd Functions (csrc/torch_ops.cpp, csrc/mixer_ops.cpp, host code compiled against torch's headers), linked
+    C++ autograd Functions (csrc/torch_ops.cpp, csrc/mixer_ops.cpp, csrc/tokens_ops.cpp, host code compiled against torch's headers), linked
     to the kernel library.
 The sources are HIP and C++ only: no CUDA sources, no hipify step, no Triton. Objects are rebuilt when
 a source or a shared header is newer than them (--force rebuilds everything); sources compile in
@@ -32,10 +32,11 @@ ROCM_INCLUDE = "/opt/rocm/include"
 
 # The longest compiles first.
 KERNEL_SOURCES = ["morpho_fwd_f32_dilation.hip", "morpho_fwd_f32_erosion.hip", "morpho_fwd_f16.hip", "morpho_fwd_bf16.hip", "smorph_static.hip",
-                  "morpho_fwd_f64.hip", "morpho_fused.hip", "morpho_bwd.hip", "smorph.hip", "smorph_element.hip", "smorph_rows.hip", "morpho_ident.hip", "morpho_scatter.hip", "morpho_fwd.hip", "norm.hip", "weight8.hip", "gated.hip", "util.hip",
-                  "capi.cpp", "stack.cpp", "mixer_api.cpp"]
-KERNEL_HEADERS = ["common.hpp", "launch.hpp", "morpho_fwd.hpp", "smorph_common.hpp", "smorph_element.hpp", "block8.hpp", "mixer.hpp",
-                  os.path.join("..", "..", "include", "morphocore_amd.h"), os.path.join("..", "..", "include", "morphocore_amd_mixer.h")]
+                  "morpho_fwd_f64.hip", "morpho_fused.hip", "morpho_bwd.hip", "smorph.hip", "smorph_element.hip", "smorph_rows.hip", "morpho_ident.hip", "morpho_scatter.hip", "morpho_fwd.hip", "norm.hip", "weight8.hip", "gated.hip", "linear_attention.hip", "rotary.hip", "util.hip",
+                  "capi.cpp", "stack.cpp", "mixer_api.cpp", "tokens_api.cpp"]
+KERNEL_HEADERS = ["common.hpp", "launch.hpp", "morpho_fwd.hpp", "smorph_common.hpp", "smorph_element.hpp", "block8.hpp", "lanes.hpp", "mixer.hpp", "tokens.hpp",
+                  os.path.join("..", "..", "include", "morphocore_amd.h"), os.path.join("..", "..", "include", "morphocore_amd_mixer.h"),
+                  os.path.join("..", "..", "include", "morphocore_amd_tokens.h")]
 # Packed FP32 instructions stay disabled: only scalar fp32 VALU forms are emitted.
 HIP_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-munsafe-fp-atomics", "-Wall", "-Wno-unused-function",
              "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
@@ -99,7 +100,8 @@ class HipBuildExt(build_ext):
         os.makedirs(os.path.dirname(target), exist_ok=True)
         torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
         deps = list(ext.sources) + [os.path.join(CSRC, "smorph_element.hpp"), os.path.join(ROOT, "include", "morphocore_amd.h"),
-                                     os.path.join(ROOT, "include", "morphocore_amd_mixer.h"), KERNEL_LIB]
+                                     os.path.join(ROOT, "include", "morphocore_amd_mixer.h"), os.path.join(ROOT, "include", "morphocore_amd_tokens.h"),
+                                     os.path.join(CSRC, "ops.hpp"), KERNEL_LIB]
         if not _stale(target, deps, self.force):
             return
         abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
@@ -125,7 +127,7 @@ setup(
     version="0.13.1",
     description="morphocore's dilation / erosion / smorph hot path as HIP kernels for AMD Instinct MI355X (gfx950)",
     packages=["morphocore_amd", "morphocore_amd.functional", "morphocore_amd.nn"],
-    ext_modules=[Extension("morphocore_amd._C", sources=[os.path.join("morphocore_amd", "csrc", src) for src in ("torch_ops.cpp", "mixer_ops.cpp")])],
+    ext_modules=[Extension("morphocore_amd._C", sources=[os.path.join("morphocore_amd", "csrc", src) for src in ("torch_ops.cpp", "mixer_ops.cpp", "tokens_ops.cpp")])],
     cmdclass={"build_ext": HipBuildExt},
     python_requires=">=3.9",
 )

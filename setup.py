@@ -32,9 +32,9 @@ ROCM_INCLUDE = "/opt/rocm/include"
 
 # The longest compiles first.
 KERNEL_SOURCES = ["morpho_fwd_f32_dilation.hip", "morpho_fwd_f32_erosion.hip", "morpho_fwd_f16.hip", "morpho_fwd_bf16.hip", "smorph_static.hip",
-                  "morpho_fwd_f64.hip", "morpho_fused.hip", "morpho_bwd.hip", "smorph.hip", "smorph_element.hip", "smorph_rows.hip", "morpho_ident.hip", "morpho_scatter.hip", "morpho_fwd.hip", "norm.hip", "weight8.hip", "gated.hip", "linear_attention.hip", "rotary.hip", "util.hip",
+                  "morpho_fwd_f64.hip", "morpho_fused.hip", "morpho_bwd.hip", "smorph.hip", "smorph_element.hip", "smorph_rows.hip", "morpho_ident.hip", "morpho_scatter.hip", "morpho_fwd.hip", "norm.hip", "weight8.hip", "gated.hip", "linear_attention_f32.hip", "linear_attention_f16.hip", "linear_attention_bf16.hip", "linear_attention.hip", "rotary.hip", "util.hip",
                   "capi.cpp", "stack.cpp", "mixer_api.cpp", "tokens_api.cpp"]
-KERNEL_HEADERS = ["common.hpp", "launch.hpp", "morpho_fwd.hpp", "smorph_common.hpp", "smorph_element.hpp", "block8.hpp", "lanes.hpp", "mixer.hpp", "tokens.hpp",
+KERNEL_HEADERS = ["common.hpp", "launch.hpp", "morpho_fwd.hpp", "smorph_common.hpp", "smorph_element.hpp", "block8.hpp", "lanes.hpp", "mixer.hpp", "tokens.hpp", "linear_attention.hpp",
                   os.path.join("..", "..", "include", "morphocore_amd.h"), os.path.join("..", "..", "include", "morphocore_amd_mixer.h"),
                   os.path.join("..", "..", "include", "morphocore_amd_tokens.h")]
 # Packed FP32 instructions stay disabled: only scalar fp32 VALU forms are emitted.

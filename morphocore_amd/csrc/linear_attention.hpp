@@ -8,7 +8,7 @@
 // No quotient of decays is formed, so nothing overflows however fast a head forgets.
 //
 // A workgroup walks over the chunks of a segment of one head of one sequence, for N of the state's columns: a wave holds all
-// rows of its 16 or 32 columns in the accumulators of the state's own product. Long sequences are split into segments
+// rows of its 16 columns in the accumulators of the state's own product. Long sequences are split into segments
 // where there are too few heads to fill the chip: one launch sums every segment's state by itself, a second joins them (both
 // read b and c only), then every segment starts from its state.
 //
@@ -19,8 +19,7 @@
 // Layouts. Of a 16 x 16 x 32 product lane l gives the first operand's row l % 16 and the second's column l % 16 with 8 values
 // of the summed axis from 8 (l / 16) on, and gets column l % 16, rows 4 (l / 16) to + 3. The transposing LDS read takes a row's 4-value
 // groups from wherever a lane points, so the state's 32 rows of two products are numbered such that a lane's two
-// results are 8 neighbouring rows: the first operand of a S, with no exchange between lanes. The same numbering of columns makes a
-// lane's results of two products 8 neighbouring values of out, stored at once. Rows of the staged tiles are units of 8 values whose order
+// results are 8 neighbouring rows: the first operand of a S, with no exchange between lanes. Rows of the staged tiles are units of 8 values whose order
 // changes from row to row, so that row and transposing reads both spread over the banks.
 #pragma once
 
@@ -41,6 +40,9 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 // Decays and sequences.
 // ------------------------------------------------------------------------------------------------
 
+// A value that every lane has, in a scalar register.
+__device__ __forceinline__ float uniform(float v) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v))); }
+
 // Decays below exp(-16384) are 0 anyway, and times 0 must stay 0.
 __device__ __forceinline__ float log_decay_of(const float* __restrict__ log_decay, int head)
 {
@@ -57,7 +59,7 @@ struct Decay
     __device__ __forceinline__ Decay(float log_decay, double n)
     {
         const double d = exp((double)log_decay * n);
-        hi = (float)d, lo = d < 1e30 ? (float)(d - (double)hi) : 0.0f;
+        hi = uniform((float)d), lo = uniform(d < 1e30 ? (float)(d - (double)hi) : 0.0f);
     }
     __device__ __forceinline__ float of(float s) const { return fmaf(s, hi, s * lo); }
 };
@@ -142,17 +144,17 @@ constexpr int terms_of()
     return std::is_same_v<T, float> ? 3 : std::is_same_v<T, _Float16> ? 2 : 1;
 }
 
-// DK: rows of the state (the values of a and b), W waves of NT * 16 columns each.
-template <typename T, int DK_, int W_, int NT_>
+// DK: rows of the state (the values of a and b), W waves of 16 columns each.
+template <typename T, int DK_, int W_>
 struct Walk
 {
-    static constexpr int DK = DK_, W = W_, NT = NT_, N = 16 * W * NT, THREADS = W * WAVE;
+    static constexpr int DK = DK_, W = W_, N = 16 * W, THREADS = W * WAVE;
     static constexpr int PL = terms_of<T>(), PS = PL == 3 ? 3 : 2;  // terms of the operands, and of scores and states
     // Rows of a chunk: what two workgroups' tiles leave room for in a CU's 160 KB, or one's.
     static constexpr int C = PL == 3 || (PL == 2 && DK == 256) ? 32 : 64;
     static constexpr int AB = C * DK * 2, V = C * N * 2, P = C * C * 2;  // bytes of a term's tile
     static constexpr int LDS = 2 * PL * AB + PL * V + PS * P;
-    static constexpr int BLOCKS = LDS <= 76 * 1024 && W == 4 ? 2 : 1;
+    static constexpr int BLOCKS = W < 4 ? 1 : W == 4 && LDS <= 76 * 1024 ? 2 : 1;
 };
 
 // Where unit x (8 values) of row r lies in a tile of U units a row: in 64 banks, 16 rows' units x and 4 rows' units x to x + 3 lie apart.
@@ -173,18 +175,17 @@ __device__ __forceinline__ int unit_byte(int r, int x)
 
 // A lane's 8 values of the summed axis, which lies along the rows: row `row` + lane % 16, values 32 k + 8 (lane / 16) on.
 template <int U>
-__device__ __forceinline__ bf16x8 row_fragment(const char* tile, int row, int k)
+__device__ __forceinline__ bf16x8 row_fragment(const char* tile, int l, int row, int k)
 {
-    const int l = threadIdx.x % WAVE;
     return *(const bf16x8*)(tile + unit_byte<U>(row + l % 16, 4 * k + l / 16));
 }
 
 // The same where it lies across the rows: rows `row` + 8 (lane / 16) on, of the column that lane % 16 stands for: value lane % 4 of
 // the 4 at unit(lane / 4 % 4), half(..). The lane points at the group (lane % 4) of row lane / 4 % 4.
 template <int U>
-__device__ __forceinline__ bf16x8 column_fragment(const char* tile, int row, int unit, int half)
+__device__ __forceinline__ bf16x8 column_fragment(const char* tile, int l, int row, int unit, int half)
 {
-    const int l = threadIdx.x % WAVE, r = row + 8 * (l / 16) + ((l >> 2) & 3);
+    const int r = row + 8 * (l / 16) + ((l >> 2) & 3);
     typedef __attribute__((address_space(3))) bf16x4* lds4;
     const bf16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(tile + unit_byte<U>(r, unit) + 8 * half));
     const bf16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(tile + unit_byte<U>(r + 4, unit) + 8 * half));
@@ -254,7 +255,7 @@ __device__ __forceinline__ bool not_finite(const RawUnit<T>& u)
 template <typename L>
 struct Spoiled
 {
-    int any;          // the last chunk's number that has some, plus 1
+    int any;          // the last chunk's number that has some
     int row;          // its first row with such a b
     int col[L::N];    // the first row with such a c, by column
     int dim[L::DK];   // whether b has one in this place
@@ -268,48 +269,111 @@ __device__ __forceinline__ void clear_spoiled(Spoiled<L>& s)
     if (threadIdx.x == 0) s.row = L::C, s.any = 0;
 }
 
-// A tile of C rows on its way from memory to LDS.
+// A staged tile's values that are not finite: zeros in their place, and f(row, column) for each. (The first term tells: it is cut.)
+template <typename L, int COLS, typename F>
+__device__ __forceinline__ void take_out_spoiled(char* tile, F&& f)
+{
+    constexpr int U = COLS / UNIT, BYTES = L::C * COLS * 2;
+#pragma unroll 1
+    for (int i = threadIdx.x; i < L::C * COLS; i += L::THREADS)
+    {
+        const int r = i / COLS, c = i % COLS, at = unit_byte<U>(r, c / UNIT) + c % UNIT * 2;
+        if ((*(const uint16_t*)(tile + at) & 0x7f80u) != 0x7f80u) continue;
+        for (int p = 0; p < L::PL; ++p) *(uint16_t*)(tile + p * BYTES + at) = 0;
+        f(r, c);
+    }
+}
+
+// A tile of C rows on its way from memory to LDS. The units of a thread lie in one column of the tile, STEP rows apart.
 template <typename T, typename L, int COLS>
 struct TileLoad
 {
-    static constexpr int U = COLS / UNIT, UNITS = L::C * U, COUNT = (UNITS + L::THREADS - 1) / L::THREADS;
-    static_assert(UNITS % L::THREADS == 0 || COUNT == 1);
+    static constexpr int U = COLS / UNIT, UNITS = L::C * U, COUNT = (UNITS + L::THREADS - 1) / L::THREADS, STEP = L::THREADS / U;
+    static_assert((UNITS % L::THREADS == 0 || COUNT == 1) && STEP * U == L::THREADS);
     RawUnit<T> raw[COUNT];
+    const T* at;  // the thread's first unit of the next chunk
 
-    // Rows [0, n) of `base` + row * stride (which may fall), values [c0, cols).
-    __device__ __forceinline__ void load(const T* __restrict__ base, int64_t stride, int n, int c0, int cols)
+    // A row's last, partial unit is read as the 8 values that end with it, and moved down by this much. `left`: the values of a row that are
+    // there from the tile's first, c0, on.
+    static __device__ __forceinline__ int down(int c0, int left)
     {
-#pragma unroll
-        for (int i = 0; i < COUNT; ++i)
-        {
-            const int u = threadIdx.x + i * L::THREADS, r = u / U, c = c0 + u % U * UNIT;
-            load_raw(base + r * stride + c, c, r < n ? cols - c : 0, raw[i]);  // r >= C of threads without a unit: n is at most C
-        }
+        const int c = (int)threadIdx.x % U * UNIT;
+        return left - c >= UNIT || left - c <= 0 || c0 + left < UNIT ? 0 : UNIT - (left - c);
     }
 
-    template <bool CHECK, typename F>
-    __device__ __forceinline__ void store(char* tile, F&& spoil)
+    // `base`: the first row's value c0.
+    __device__ __forceinline__ void begin(const T* base, int64_t stride, int c0, int left)
+    {
+        at = base + (int)threadIdx.x / U * stride + ((int)threadIdx.x % U * UNIT - down(c0, left));
+    }
+
+    // The next chunk, of n rows; whole: all of the tile is there.
+    __device__ __forceinline__ void load(int64_t stride, bool whole, int n, int c0, int left)
+    {
+        if (whole)
+        {
+#pragma unroll
+            for (int i = 0; i < COUNT; ++i, at += STEP * stride)
+                if (UNITS % L::THREADS == 0 || (int)threadIdx.x < UNITS) __builtin_memcpy(raw[i].d, at, sizeof(raw[i].d));
+        }
+        else
+        {
+            const int r = (int)threadIdx.x / U, c = (int)threadIdx.x % U * UNIT;
+            const bool few = c0 + left < UNIT;  // rows of fewer than 8 values
+            const T* const first = at;
+#pragma unroll
+            for (int i = 0; i < COUNT; ++i, at += STEP * stride)
+            {
+#pragma unroll
+                for (int k = 0; k < RawUnit<T>::DWORDS; ++k) raw[i].d[k] = 0;
+                if (!few && c < left && r + i * STEP < n) __builtin_memcpy(raw[i].d, at, sizeof(raw[i].d));
+            }
+            if (few && c == 0)
+            {
+#pragma unroll 1
+                for (int j = 0; j < left; ++j)
+#pragma unroll
+                    for (int i = 0; i < COUNT; ++i)
+                    {
+                        if (r + i * STEP >= n) continue;
+                        constexpr int PER = 4 / (int)sizeof(T);
+                        uint32_t v;
+                        if constexpr (PER == 1)
+                            v = __builtin_bit_cast(uint32_t, first[i * (STEP * stride) + j]);
+                        else
+                            v = (uint32_t)__builtin_bit_cast(uint16_t, first[i * (STEP * stride) + j]) << (16 * (j % 2));
+#pragma unroll
+                        for (int k = 0; k < RawUnit<T>::DWORDS; ++k) raw[i].d[k] |= j / PER == k ? v : 0;
+                    }
+            }
+        }
+        static_assert(COUNT * STEP == L::C || COUNT == 1);
+        if (COUNT * STEP != L::C) at += (L::C - COUNT * STEP) * stride;
+    }
+
+    // Whether a value is not finite.
+    __device__ __forceinline__ bool spoiled() const
+    {
+        bool any = false;
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) any |= not_finite<T>(raw[i]);
+        return any;
+    }
+
+    __device__ __forceinline__ void store(char* tile, bool whole, int c0, int left)
     {
         constexpr int BYTES = L::C * COLS * 2;
+        if (!whole)
+        {
+            const int n = down(c0, left);
+#pragma unroll
+            for (int i = 0; i < COUNT; ++i) raw[i].shift(n);
+        }
 #pragma unroll
         for (int i = 0; i < COUNT; ++i)
         {
             const int u = threadIdx.x + i * L::THREADS, r = u / U, x = u % U;
             if (UNITS % L::THREADS && u >= UNITS) break;
-            if (CHECK && not_finite<T>(raw[i]))
-            {
-#pragma unroll
-                for (int j = 0; j < UNIT; ++j)
-                {
-                    const float v = raw[i][j];
-                    if (fabsf(v) <= 3.4028235e38f) continue;
-                    spoil(r, x * UNIT + j);
-                    if constexpr (sizeof(T) == 4)
-                        raw[i].d[j] = 0;
-                    else
-                        raw[i].d[j / 2] &= j % 2 ? 0xffffu : 0xffff0000u;
-                }
-            }
             if constexpr (L::PL == 1)
             {
                 *(bf16x8*)(tile + unit_byte<U>(r, x)) = __builtin_bit_cast(bf16x8, raw[i]);
@@ -334,14 +398,6 @@ struct Passes
     float* states[3];  // of the segments
 };
 
-// A lane's place in the state: rows 32 u + 8 (lane / 16) + 4 h + r, and the column.
-template <typename L>
-__device__ __forceinline__ int state_column(int t)
-{
-    const int l = threadIdx.x % WAVE, w = threadIdx.x / WAVE, n = l % 16;
-    return L::NT == 2 ? 32 * w + 8 * (n >> 2) + 4 * t + (n & 3) : 16 * w + n;
-}
-
 // Values of a segment's state of one tile, in the order in which lanes hold them.
 template <typename L>
 constexpr int64_t state_values()
@@ -349,12 +405,30 @@ constexpr int64_t state_values()
     return (int64_t)L::DK * L::N;
 }
 
+// 32 rows of a tile's state from or to memory, neighbouring values by neighbouring threads.
+template <typename L>
+__device__ __forceinline__ void move_state(float* __restrict__ lds, const States& s, int64_t state0, int row, int rows, int col, int cols, bool in)
+{
+    const bool by_rows = s.row_stride == 1;
+#pragma unroll 1
+    for (int i = threadIdx.x; i < 32 * L::N; i += L::THREADS)
+    {
+        const int d = by_rows ? i % 32 : i / L::N, c = by_rows ? i / 32 : i % L::N;
+        const bool there = row + d < rows && col + c < cols;
+        float* __restrict__ p = s.p + state0 + (row + d) * s.row_stride + (col + c) * s.col_stride;
+        if (in)
+            lds[d * L::N + c] = there ? *p : 0.0f;
+        else if (there)
+            *p = lds[d * L::N + c];
+    }
+}
+
 // ONLY: the segments' own states (from 0) to the workspace, of all but the last of a sequence; no results.
 template <typename T, typename L, bool ONLY>
 __global__ __launch_bounds__(L::THREADS, L::BLOCKS) void attention_walk_kernel(Sequences seq, Segments segments, int heads,
                                                                                const float* __restrict__ log_decay, Passes passes, int tiles)
 {
-    constexpr int C = L::C, DK = L::DK, N = L::N, NT = L::NT, PL = L::PL, PS = L::PS, RT = C / 16, KS = C / 32, KD = DK / 32;
+    constexpr int C = L::C, DK = L::DK, N = L::N, PL = L::PL, PS = L::PS, RT = C / 16, KS = C / 32, KD = DK / 32;
     constexpr int UD = DK / UNIT, UN = N / UNIT, UC = C / UNIT;
     __shared__ __align__(16) char lds[ONLY ? PL * (L::AB + L::V) : L::LDS];
     __shared__ Spoiled<L> spoiled;
@@ -362,17 +436,22 @@ __global__ __launch_bounds__(L::THREADS, L::BLOCKS) void attention_walk_kernel(S
     char* const tc = tb + PL * L::AB;
     char* const ta = ONLY ? nullptr : tc + PL * L::V;
     char* const tp = ONLY ? nullptr : ta + PL * L::AB;
-    const int l = threadIdx.x % WAVE, wave = threadIdx.x / WAVE, g = l / 16;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
     const Pass& p = passes.p[blockIdx.y];
     const int s = p.backwards ? 1 : 0;
-    if constexpr (!ONLY)
+    auto clear_scores = [&] {
         for (int i = threadIdx.x; i < PS * L::P / 16; i += L::THREADS) ((uint4*)tp)[i] = make_uint4(0, 0, 0, 0);
+    };
+    if constexpr (!ONLY) clear_scores();
     clear_spoiled(spoiled);
     int chunk = 0;
 
     const int64_t work = segments.count * heads * tiles;
     for (int64_t item = blockIdx.x; item < work; item += gridDim.x)
     {
+        int l = threadIdx.x % WAVE;
+        asm volatile("" : "+v"(l));
+        const int g = l / 16;
         const int tile = (int)(item % tiles), head = (int)(item / tiles % heads);
         const int64_t at = item / tiles / heads;
         const Segment part = segment_at(seq, segments, at);
@@ -399,58 +478,44 @@ __global__ __launch_bounds__(L::THREADS, L::BLOCKS) void attention_walk_kernel(S
         // A sequence without rows has one segment (number 0), which hands its state on.
         if (ONLY ? last || n_all == 0 : n_all == 0 && part.number != 0) continue;
 
-        const float lg = log_decay_of(log_decay, head), lg2 = lg * 1.4426950408889634f;
+        const float lg = uniform(log_decay_of(log_decay, head)), lg2 = uniform(lg * 1.4426950408889634f);
         auto power = [&](int n) { return __builtin_amdgcn_exp2f(lg2 * (float)n); };
-        const Decay chunk_decay(lg, C);
         const float update = p.update, read = p.read;
-        // e^(i - j) of two tiles of rows `d` apart, in a lane's place; e^(i + 1 - s); e^(7 - v) of a lane's 8 rows of c.
-        float near[RT][4], far[RT], tail[UNIT];
-        if constexpr (!ONLY)
-        {
+        const Decay chunk_decay(lg, C), end_decay(lg, (double)(n_all % C));
+        const float e16 = uniform(power(16));
+        float tail[UNIT];  // e^(7 - v) of 8 rows of c
 #pragma unroll
-            for (int d = 0; d < RT; ++d)
-            {
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                {
-                    const int gap = 16 * d + l % 16 - 4 * g - r;
-                    near[d][r] = gap < 0 ? 0.0f : power(gap) * (update * read);
-                }
-                far[d] = power(16 * d + l % 16 + 1 - s) * read;
-            }
-        }
-#pragma unroll
-        for (int v = 0; v < UNIT; ++v) tail[v] = power(UNIT - 1 - v) * update;
+        for (int v = 0; v < UNIT; ++v) tail[v] = uniform(power(UNIT - 1 - v) * update);
 
-        // The state: from the workspace, as lanes hold it, or the pass's first.
-        f32x4 S[KD][2][NT];
+        // The state: from the workspace, as lanes hold it, or the pass's first, 32 rows at a time through LDS.
+        f32x4 S[KD][2] = {};
         const int64_t state0 = (part.q.batch * heads + head) * p.dim * cols;
-        const bool joined = !ONLY && part.number > 0;
-        const float* __restrict__ begin = joined ? passes.states[blockIdx.y] + (((at - 1) * heads + head) * tiles + tile) * state_values<L>() : nullptr;
+        if (!ONLY && part.number > 0)
+        {
+            const float* __restrict__ begin = passes.states[blockIdx.y] + (((at - 1) * heads + head) * tiles + tile) * state_values<L>();
 #pragma unroll
-        for (int u = 0; u < KD; ++u)
+            for (int u = 0; u < KD; ++u)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+                for (int h = 0; h < 2; ++h)
+                    S[u][h] = *(const f32x4*)(begin + (((int64_t)wave * KD + u) * 2 + h) * WAVE * 4 + l * 4);
+        }
+        else if (!ONLY && p.first.p)
+        {
+            __syncthreads();
 #pragma unroll
-                for (int t = 0; t < NT; ++t)
-                {
-                    f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-                    if (joined)
-                    {
-                        x = *(const f32x4*)(begin + ((((int64_t)wave * KD + u) * 2 + h) * NT + t) * WAVE * 4 + l * 4);
-                    }
-                    else if (!ONLY && p.first.p)
-                    {
-                        const int c = col0 + state_column<L>(t);
+            for (int u = 0; u < KD; ++u)
+            {
+                move_state<L>((float*)lds, p.first, state0, 32 * u, p.dim, col0, cols, true);
+                __syncthreads();
 #pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                        {
-                            const int d = 32 * u + 8 * g + 4 * h + r;
-                            if (d < p.dim && c < cols) x[r] = p.first.p[state0 + d * p.first.row_stride + c * p.first.col_stride];
-                        }
-                    }
-                    S[u][h][t] = x;
-                }
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) S[u][h][r] = ((const float*)lds)[(8 * g + 4 * h + r) * N + (16 * wave + l % 16)];
+                __syncthreads();
+            }
+            // The scores above the diagonal are where some of it was.
+            if constexpr (!ONLY) clear_scores();
+        }
 
         // Position 0's rows; the rows of later positions follow, or come before it where time runs backwards.
         const int64_t dir = s ? -1 : 1, t0 = part.q.start + (s ? part.q.length - 1 - part.first : part.first);
@@ -463,149 +528,163 @@ __global__ __launch_bounds__(L::THREADS, L::BLOCKS) void attention_walk_kernel(S
         const int64_t sa = dir * p.a.token_stride, sb = dir * p.b.token_stride, sc = dir * p.c.token_stride;
         TileLoad<T, L, DK> la, lb;
         TileLoad<T, L, N> lc;
+        if constexpr (!ONLY) la.begin(pa, sa, 0, p.dim);
+        lb.begin(pb, sb, 0, p.dim);
+        lc.begin(pc + col0, sc, col0, cols - col0);
+        const bool wide = p.dim == DK && col0 + N <= cols;
         auto load = [&](int64_t first) {
             const int n = (int)(n_all - first < C ? n_all - first : C);
-            if constexpr (!ONLY) la.load(pa + first * sa, sa, n, 0, p.dim);
-            lb.load(pb + first * sb, sb, n, 0, p.dim);
-            lc.load(pc + first * sc, sc, n, col0, cols);
+            const bool whole = wide && n == C;
+            if constexpr (!ONLY) la.load(sa, whole, n, 0, p.dim);
+            lb.load(sb, whole, n, 0, p.dim);
+            lc.load(sc, whole, n, col0, cols - col0);
         };
         if (n_all > 0) load(0);
         for (int64_t first = 0; first < n_all; first += C)
         {
             const int n = (int)(n_all - first < C ? n_all - first : C);
             ++chunk;
+            // The lane's places in LDS follow from this copy anew in every chunk: kept from chunk to chunk they would fill the registers.
+            int l = threadIdx.x % WAVE;
+            asm volatile("" : "+v"(l));
+            const int g = l / 16;
             __syncthreads();
-            if constexpr (!ONLY) la.template store<false>(ta, [](int, int) {});
-            lb.template store<true>(tb, [&](int r, int c) {
-                spoiled.any = chunk;
-                spoiled.dim[c] = 1;
-                atomicMin(&spoiled.row, r);
-            });
-            lc.template store<true>(tc, [&](int r, int c) {
-                spoiled.any = chunk;
-                atomicMin(&spoiled.col[c], r);
-            });
+            if constexpr (!ONLY) la.store(ta, wide, 0, p.dim);
+            lb.store(tb, wide, 0, p.dim);
+            lc.store(tc, wide, col0, cols - col0);
+            if ((int)lb.spoiled() | (int)lc.spoiled()) spoiled.any = chunk;
             if (first + C < n_all) load(first + C);
             __syncthreads();
+            const bool spoils = spoiled.any == chunk;
+            if (spoils)
+            {
+                take_out_spoiled<L, DK>(tb, [&](int r, int c) {
+                    spoiled.dim[c] = 1;
+                    atomicMin(&spoiled.row, r);
+                });
+                take_out_spoiled<L, N>(tc, [&](int r, int c) { atomicMin(&spoiled.col[c], r); });
+                __syncthreads();
+            }
 
-            f32x4 o[RT][NT] = {};
+            f32x4 o[RT] = {};
             if constexpr (!ONLY)
             {
-                // Scores of the wave's rows, decayed, in terms to LDS.
+                // Scores, decayed, in terms to LDS: tiles of 16 x 16 on and below the diagonal, by the waves in turn.
 #pragma unroll
-                for (int rt0 = 0; rt0 < RT; rt0 += L::W)
+                for (int i0 = 0; i0 < RT * (RT + 1) / 2; i0 += L::W)
                 {
-                    const int rt = rt0 + wave;
-                    if (rt >= RT) continue;
-                    bf16x8 fa[KD][PL];
+                    const int index = i0 + wave;
+                    if (index >= RT * (RT + 1) / 2) break;
+                    const int rt = index < 1 ? 0 : index < 3 ? 1 : index < 6 ? 2 : 3, ct = index - rt * (rt + 1) / 2;
+                    f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                     for (int k = 0; k < KD; ++k)
-#pragma unroll
-                        for (int i = 0; i < PL; ++i) fa[k][i] = row_fragment<UD>(ta + i * L::AB, 16 * rt, k);
-#pragma unroll
-                    for (int ct = 0; ct < RT; ++ct)
                     {
-                        if (ct > rt) continue;
-                        f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                        for (int k = 0; k < KD; ++k)
-#pragma unroll
-                            for (int j = 0; j < PL; ++j)
-                            {
-                                const bf16x8 fb = row_fragment<UD>(tb + j * L::AB, 16 * ct, k);
-#pragma unroll
-                                for (int i = 0; i < PL; ++i)
-                                    if (i + j <= 2) x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb, fa[k][i], x, 0, 0, 0);
-                            }
-                        float v[4];
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                        {
-                            float w = 0.0f;
-#pragma unroll
-                            for (int d = 0; d < RT; ++d) w = rt - ct == d ? near[d][r] : w;
-                            // What lies above the diagonal is no product with 0: a query's infinity stays in its row.
-                            v[r] = rt == ct && l % 16 - 4 * g - r < 0 ? 0.0f : x[r] * w;
-                        }
-                        __bf16 term[PS][4];
-                        split<PS, false>(v, term);
-#pragma unroll
-                        for (int i = 0; i < PS; ++i)
-                            *(bf16x4*)(tp + i * L::P + unit_byte<UC>(16 * rt + l % 16, 2 * ct + (g >> 1)) + 8 * (g & 1)) = term_vector<bf16x4>(term, i);
-                    }
-                }
-                // a S, with the state's terms as they lie in the lanes.
-#pragma unroll
-                for (int u = 0; u < KD; ++u)
-                {
-                    bf16x8 fs[NT][PS];
-#pragma unroll
-                    for (int t = 0; t < NT; ++t)
-                    {
-                        float v[UNIT];
-#pragma unroll
-                        for (int j = 0; j < UNIT; ++j) v[j] = S[u][j / 4][t][j % 4];
-                        __bf16 term[PS][UNIT];
-                        split<PS, false>(v, term);
-#pragma unroll
-                        for (int i = 0; i < PS; ++i) fs[t][i] = term_vector<bf16x8>(term, i);
-                    }
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt)
+                        bf16x8 fa[PL], fb[PL];
 #pragma unroll
                         for (int i = 0; i < PL; ++i)
                         {
-                            const bf16x8 fa = row_fragment<UD>(ta + i * L::AB, 16 * rt, u);
-#pragma unroll
-                            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                                for (int j = 0; j < PS; ++j)
-                                    if (i + j < PS) o[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fs[t][j], fa, o[rt][t], 0, 0, 0);
+                            fa[i] = row_fragment<UD>(ta + i * L::AB, l, 16 * rt, k);
+                            fb[i] = row_fragment<UD>(tb + i * L::AB, l, 16 * ct, k);
                         }
+#pragma unroll
+                        for (int i = 0; i < PL; ++i)
+#pragma unroll
+                            for (int j = 0; j < PL; ++j)
+                                if (i + j <= 2) x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[j], fa[i], x, 0, 0, 0);
+                    }
+                    // e^(i - j), of the tile on the diagonal value by value (nothing above it: no product with 0, so that a query's infinity
+                    // stays in its row), of others from the lane's last row on.
+                    float v[4];
+                    const int gap = 16 * (rt - ct) + l % 16 - 4 * g;
+                    if (rt == ct)
+                    {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) v[r] = gap - r < 0 ? 0.0f : x[r] * (power(gap - r) * (update * read));
+                    }
+                    else
+                    {
+                        const float near = power(gap - 3) * read;
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) v[r] = x[r] * (near * tail[4 + r]);
+                    }
+                    __bf16 term[PS][4];
+                    split<PS, false>(v, term);
+#pragma unroll
+                    for (int i = 0; i < PS; ++i)
+                        *(bf16x4*)(tp + i * L::P + unit_byte<UC>(16 * rt + l % 16, 2 * ct + (g >> 1)) + 8 * (g & 1)) = term_vector<bf16x4>(term, i);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
+                // a S, with the state's terms as they lie in the lanes; the next 32 rows' fragments of a are read while these are multiplied.
+                bf16x8 fa[2][RT][PL];
+                auto read_a = [&](int u) {
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt)
+                    for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-                    for (int t = 0; t < NT; ++t) o[rt][t] *= far[rt];
+                        for (int i = 0; i < PL; ++i) fa[u % 2][rt][i] = row_fragment<UD>(ta + i * L::AB, l, 16 * rt, u);
+                };
+                read_a(0);
+#pragma unroll
+                for (int u = 0; u < KD; ++u)
+                {
+                    if (u + 1 < KD) read_a(u + 1);
+                    {
+                        float v[UNIT];
+#pragma unroll
+                        for (int j = 0; j < UNIT; ++j) v[j] = S[u][j / 4][j % 4];
+                        __bf16 term[PS][UNIT];
+                        split<PS, false>(v, term);
+#pragma unroll
+                        for (int j = 0; j < PS; ++j)
+                        {
+                            const bf16x8 fs = term_vector<bf16x8>(term, j);
+#pragma unroll
+                            for (int i = 0; i < PL; ++i)
+                                if (i + j < PS)
+#pragma unroll
+                                    for (int rt = 0; rt < RT; ++rt) o[rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fs, fa[u % 2][rt][i], o[rt], 0, 0, 0);
+                        }
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                float reach = power(l % 16 + 1 - s) * read;
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt, reach *= e16)
+                    o[rt] *= reach;
                 __syncthreads();
             }
 
             // Scores times c, and the state after the chunk.
             const bool whole = n == C;
-            const Decay decay = whole ? chunk_decay : Decay(lg, n);
+            const Decay decay = whole ? chunk_decay : end_decay;
 #pragma unroll
             for (int u = 0; u < KD; ++u)
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int t = 0; t < NT; ++t)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) S[u][h][t][r] = decay.of(S[u][h][t][r]);
+                        for (int r = 0; r < 4; ++r) S[u][h][r] = decay.of(S[u][h][r]);
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
             {
-                bf16x8 fc[NT][PL], fd[NT][3];
+                bf16x8 fc[PL], fd[3];
                 // e^(n - 1 + s - j) of the lane's last row j = 32 ks + 8 g + 7 (rows behind the chunk's end are 0).
                 const int past = n - 1 + s - (32 * ks + 8 * g + 7);
                 const float base = power(past);
-#pragma unroll
-                for (int t = 0; t < NT; ++t)
                 {
                     float v[UNIT] = {};
 #pragma unroll
                     for (int i = 0; i < PL; ++i)
                     {
-                        fc[t][i] = NT == 2 ? column_fragment<UN>(tc + i * L::V, 32 * ks, 4 * wave + (l & 3), t)
-                                           : column_fragment<UN>(tc + i * L::V, 32 * ks, 2 * wave + ((l & 3) >> 1), l & 1);
+                        fc[i] = column_fragment<UN>(tc + i * L::V, l, 32 * ks, 2 * wave + ((l & 3) >> 1), l & 1);
 #pragma unroll
-                        for (int j = 0; j < UNIT; ++j) v[j] += (float)fc[t][i][j];
+                        for (int j = 0; j < UNIT; ++j) v[j] += (float)fc[i][j];
                     }
 #pragma unroll
-                    for (int j = 0; j < UNIT; ++j) v[j] = past >= 0 ? v[j] * (tail[j] * base) : past + 7 - j >= 0 ? v[j] * (power(past + 7 - j) * update) : 0.0f;
+                    for (int j = 0; j < UNIT; ++j) v[j] *= whole ? tail[j] * base : past + 7 - j >= 0 ? power(past + 7 - j) * update : 0.0f;
                     __bf16 term[3][UNIT];
                     split<3, false>(v, term);
 #pragma unroll
-                    for (int i = 0; i < 3; ++i) fd[t][i] = term_vector<bf16x8>(term, i);
+                    for (int i = 0; i < 3; ++i) fd[i] = term_vector<bf16x8>(term, i);
                 }
                 if constexpr (!ONLY)
                 {
@@ -614,52 +693,54 @@ __global__ __launch_bounds__(L::THREADS, L::BLOCKS) void attention_walk_kernel(S
 #pragma unroll
                         for (int j = 0; j < PS; ++j)
                         {
-                            const bf16x8 fp = row_fragment<UC>(tp + j * L::P, 16 * rt, ks);
-#pragma unroll
-                            for (int t = 0; t < NT; ++t)
+                            const bf16x8 fp = row_fragment<UC>(tp + j * L::P, l, 16 * rt, ks);
 #pragma unroll
                                 for (int i = 0; i < PL; ++i)
-                                    if (i + j < PS) o[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fc[t][i], fp, o[rt][t], 0, 0, 0);
+                                    if (i + j < PS) o[rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fc[i], fp, o[rt], 0, 0, 0);
                         }
                 }
+                __builtin_amdgcn_sched_barrier(0);
+                // b's columns for 16 rows of the state at a time, the next ones read while these are multiplied.
+                bf16x8 fb[2][PL];
+                auto read_b = [&](int uh) {
 #pragma unroll
-                for (int u = 0; u < KD; ++u)
+                    for (int i = 0; i < PL; ++i) fb[uh % 2][i] = column_fragment<UD>(tb + i * L::AB, l, 32 * ks, 4 * (uh / 2) + (l & 3), uh % 2);
+                };
+                read_b(0);
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
+                for (int uh = 0; uh < 2 * KD; ++uh)
+                {
+                    if (uh + 1 < 2 * KD) read_b(uh + 1);
+#pragma unroll
+                    for (int j = 0; j < 3; ++j)
 #pragma unroll
                         for (int i = 0; i < PL; ++i)
-                        {
-                            const bf16x8 fb = column_fragment<UD>(tb + i * L::AB, 32 * ks, 4 * u + (l & 3), h);
-#pragma unroll
-                            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                                for (int j = 0; j < 3; ++j)
-                                    if (i + j <= 2) S[u][h][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb, fd[t][j], S[u][h][t], 0, 0, 0);
-                        }
+                            if (i + j <= 2)
+                                    S[uh / 2][uh % 2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[uh % 2][i], fd[j], S[uh / 2][uh % 2], 0, 0, 0);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
-            if (spoiled.any == chunk)
+            if (spoils)
             {
                 const float nan = __builtin_nanf("");
-#pragma unroll
-                for (int t = 0; t < NT; ++t)
                 {
-                    const int by = spoiled.col[state_column<L>(t)];
+                    const int by = spoiled.col[(16 * wave + l % 16)];
 #pragma unroll
                     for (int u = 0; u < KD; ++u)
 #pragma unroll
                         for (int h = 0; h < 2; ++h)
 #pragma unroll
                             for (int r = 0; r < 4; ++r)
-                                if (by < C || spoiled.dim[32 * u + 8 * g + 4 * h + r]) S[u][h][t][r] = nan;
+                                if (by < C || spoiled.dim[32 * u + 8 * g + 4 * h + r]) S[u][h][r] = nan;
                     if constexpr (!ONLY)
                     {
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
                         {
-                            const int from = min(spoiled.row, spoiled.col[NT == 2 ? 32 * wave + 8 * g + 4 * t + r : 16 * wave + 4 * g + r]);
+                            const int from = min(spoiled.row, spoiled.col[16 * wave + 4 * g + r]);
 #pragma unroll
                             for (int rt = 0; rt < RT; ++rt)
-                                if (16 * rt + l % 16 >= from) o[rt][t][r] = nan;
+                                if (16 * rt + l % 16 >= from) o[rt][r] = nan;
                         }
                     }
                 }
@@ -676,16 +757,33 @@ __global__ __launch_bounds__(L::THREADS, L::BLOCKS) void attention_walk_kernel(S
                         const int i = 16 * rt + l % 16;
                         if (i >= n) continue;
                         const int64_t pos = part.first + first + i, row = row0 + (s ? part.q.length - 1 - pos : pos);
-                        const int c = col0 + (NT == 2 ? 32 * wave + 8 * g : 16 * wave + 4 * g);
+                        const int c = col0 + 16 * wave + 4 * g;
                         const int64_t to = (row * heads + head) * cols + c;
-                        float v[UNIT] = {};
-#pragma unroll
-                        for (int j = 0; j < 4 * NT; ++j) v[j] = o[rt][j / 4][j % 4];
-                        const int valid = min(cols - c, 4 * NT);
-                        if (p.out32)
-                            store_unit(p.out32 + to, valid, v);
+                        if (c + 4 <= cols)
+                        {
+                            if (p.out32)
+                            {
+                                __builtin_memcpy(p.out32 + to, &o[rt], 16);
+                            }
+                            else
+                            {
+                                typedef T Tx4 __attribute__((ext_vector_type(4)));
+                                const Tx4 v = __builtin_convertvector(o[rt], Tx4);
+                                __builtin_memcpy((T*)p.out + to, &v, sizeof(v));
+                            }
+                        }
                         else
-                            store_unit((T*)p.out + to, valid, v);
+                        {
+#pragma unroll
+                            for (int j = 0; j < 3; ++j)
+                            {
+                                if (c + j >= cols) break;
+                                if (p.out32)
+                                    p.out32[to + j] = o[rt][j];
+                                else
+                                    ((T*)p.out)[to + j] = (T)o[rt][j];
+                            }
+                        }
                     }
                 }
             }
@@ -698,23 +796,23 @@ __global__ __launch_bounds__(L::THREADS, L::BLOCKS) void attention_walk_kernel(S
             for (int u = 0; u < KD; ++u)
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) *(f32x4*)(end + ((((int64_t)wave * KD + u) * 2 + h) * NT + t) * WAVE * 4 + l * 4) = S[u][h][t];
+                    *(f32x4*)(end + (((int64_t)wave * KD + u) * 2 + h) * WAVE * 4 + l * 4) = S[u][h];
         }
         else if (last && p.last.p)
         {
+            __syncthreads();
 #pragma unroll
             for (int u = 0; u < KD; ++u)
+            {
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int t = 0; t < NT; ++t)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                        {
-                            const int d = 32 * u + 8 * g + 4 * h + r, c = col0 + state_column<L>(t);
-                            if (d < p.dim && c < cols) p.last.p[state0 + d * p.last.row_stride + c * p.last.col_stride] = S[u][h][t][r];
-                        }
+                        for (int r = 0; r < 4; ++r) ((float*)lds)[(8 * g + 4 * h + r) * N + (16 * wave + l % 16)] = S[u][h][r];
+                __syncthreads();
+                move_state<L>((float*)lds, p.last, state0, 32 * u, p.dim, col0, cols, false);
+                __syncthreads();
+            }
+            if constexpr (!ONLY) clear_scores();
         }
     }
 }
@@ -742,9 +840,8 @@ __global__ __launch_bounds__(BLOCK) void attention_join_kernel(Sequences seq, Se
         const int e = block * BLOCK + threadIdx.x;
         if (count <= 0 || e >= VALUES) continue;
         // The value's place: see attention_walk_kernel's workspace.
-        const int r = e % 4, l = e / 4 % WAVE, t = e / 4 / WAVE % L::NT, h = e / 4 / WAVE / L::NT % 2, u = e / 4 / WAVE / L::NT / 2 % (L::DK / 32);
-        const int w = e / 4 / WAVE / L::NT / 2 / (L::DK / 32), n = l % 16, d = 32 * u + 8 * (l / 16) + 4 * h + r;
-        const int c = tile * L::N + (L::NT == 2 ? 32 * w + 8 * (n >> 2) + 4 * t + (n & 3) : 16 * w + n);
+        const int r = e % 4, l = e / 4 % WAVE, h = e / 4 / WAVE % 2, u = e / 4 / WAVE / 2 % (L::DK / 32), w = e / 4 / WAVE / 2 / (L::DK / 32);
+        const int d = 32 * u + 8 * (l / 16) + 4 * h + r, c = tile * L::N + 16 * w + l % 16;
         const Decay decay(log_decay_of(log_decay, head), (double)segments.rows);
         float x = 0.0f;
         if (p.first.p && d < p.dim && c < p.cols)
@@ -776,22 +873,22 @@ __global__ __launch_bounds__(BLOCK) void attention_join_kernel(Sequences seq, Se
 template <typename T, typename F>
 hipError_t by_walk(const Pass& p, F&& f)
 {
-#define MCA_WALK(DK, W, NT) return f(Walk<T, DK, W, NT>())
-#define MCA_WALKS(DK)                        \
-    do                                       \
-    {                                        \
-        if (p.cols <= 64) MCA_WALK(DK, 4, 1); \
-        MCA_WALK(DK, 4, 2);                  \
+#define MCA_WALK(DK, W) return f(Walk<T, DK, W>())
+#define MCA_WALKS(DK)                    \
+    do                                   \
+    {                                    \
+        if (p.cols <= 64) MCA_WALK(DK, 4); \
+        MCA_WALK(DK, 8);                 \
     } while (0)
     if (p.dim <= 64 && p.cols <= 32)
     {
         if (p.dim <= 32)
         {
-            if (p.cols <= 16) MCA_WALK(32, 1, 1);
-            MCA_WALK(32, 2, 1);
+            if (p.cols <= 16) MCA_WALK(32, 1);
+            MCA_WALK(32, 2);
         }
-        if (p.cols <= 16) MCA_WALK(64, 1, 1);
-        MCA_WALK(64, 2, 1);
+        if (p.cols <= 16) MCA_WALK(64, 1);
+        MCA_WALK(64, 2);
     }
     if (p.dim <= 32) MCA_WALKS(32);
     if (p.dim <= 64) MCA_WALKS(64);

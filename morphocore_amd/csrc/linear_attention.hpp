@@ -56,6 +56,7 @@ struct Decay
 {
     float hi, lo;
 
+    Decay() = default;
     __device__ __forceinline__ Decay(float log_decay, double n)
     {
         const double d = exp((double)log_decay * n);
@@ -153,18 +154,23 @@ struct Walk
     // Rows of a chunk: what two workgroups' tiles leave room for in a CU's 160 KB, or one's.
     static constexpr int C = PL == 3 || (PL == 2 && DK == 256) ? 32 : 64;
     static constexpr int AB = C * DK * 2, V = C * N * 2, P = C * C * 2;  // bytes of a term's tile
-    static constexpr int LDS = 2 * PL * AB + PL * V + PS * P;
-    static constexpr int BLOCKS = W < 4 ? 1 : W == 4 && LDS <= 76 * 1024 ? 2 : 1;
+    static constexpr int OUT = C * N * (PL == 3 ? 4 : 2), A = PL * AB > OUT ? PL * AB : OUT;  // a's tile is out's too
+    static constexpr int LDS = A + PL * AB + PL * V + PS * P;
+    // Where two workgroups' tiles fit, registers are kept to what lets two run: the next chunk is loaded late.
+    static constexpr bool LATE = W == 8 && LDS <= 76 * 1024;
+    static constexpr int WAVES = LATE ? 4 : W >= 4 ? 2 : 1;  // a SIMD, at least
 };
 
-// Where unit x (8 values) of row r lies in a tile of U units a row: in 64 banks, 16 rows' units x and 4 rows' units x to x + 3 lie apart.
+// Where unit x (8 values) of row r lies in a tile of U units a row. The 16 lanes that read 16 bytes each at once have rows 0 to 3 and 12 to 15 of unit
+// x and rows 4 to 11 of unit x ^ 1, or the other way round: in 64 banks they lie apart, as do 4 rows' units x to x + 3.
 template <int U>
 __device__ __forceinline__ int unit_place(int r, int x)
 {
-    if constexpr (U >= 16) return x ^ (4 * (r & 3) + ((r >> 2) & 3));
-    if constexpr (U == 8) return x ^ (4 * ((r >> 1) & 1) + ((r >> 2) & 3));
-    if constexpr (U == 4) return x ^ ((r >> 2) & 3);
-    return x ^ ((r >> 3) & 1);
+    const int a = (r >> 2) & 1, b = (r >> 3) & 1, turn = 2 * (a ^ b) + b;
+    if constexpr (U >= 16) return x ^ (4 * (r & 3) + turn);
+    if constexpr (U == 8) return x ^ (4 * ((r >> 1) & 1) + turn);
+    if constexpr (U == 4) return x ^ turn;
+    return x ^ b;
 }
 
 template <int U>
@@ -173,22 +179,30 @@ __device__ __forceinline__ int unit_byte(int r, int x)
     return (r * U + unit_place<U>(r, x)) * 16;
 }
 
-// A lane's 8 values of the summed axis, which lies along the rows: row `row` + lane % 16, values 32 k + 8 (lane / 16) on.
+// A lane's byte in row l % 16 of a tile for 8 values of the summed axis, which lies along the rows: its part of the unit is lane / 16. Of row
+// + 16 n the byte is 256 U n further, of unit + 4 k it is xor 64 k (unit_place's xor commutes).
 template <int U>
-__device__ __forceinline__ bf16x8 row_fragment(const char* tile, int l, int row, int k)
+__device__ __forceinline__ int row_place(int l)
 {
-    return *(const bf16x8*)(tile + unit_byte<U>(row + l % 16, 4 * k + l / 16));
+    return unit_byte<U>(l % 16, l / 16);
 }
 
-// The same where it lies across the rows: rows `row` + 8 (lane / 16) on, of the column that lane % 16 stands for: value lane % 4 of
-// the 4 at unit(lane / 4 % 4), half(..). The lane points at the group (lane % 4) of row lane / 4 % 4.
+__device__ __forceinline__ bf16x8 row_fragment(const char* tile, int place, int k) { return *(const bf16x8*)(tile + (place ^ (64 * k))); }
+
+// The same where it lies across the rows, in one of the column's 4 values that lane % 16 / 4 stands for: the lane points at 4 values of row
+// 8 (lane / 16) + lane / 4 % 4, and of the one 4 rows below, which is xor 32 by the units' order.
 template <int U>
-__device__ __forceinline__ bf16x8 column_fragment(const char* tile, int l, int row, int unit, int half)
+__device__ __forceinline__ int column_place(int l, int unit)
 {
-    const int r = row + 8 * (l / 16) + ((l >> 2) & 3);
+    return unit_byte<U>(8 * (l / 16) + ((l >> 2) & 3), unit);
+}
+
+template <int U>
+__device__ __forceinline__ bf16x8 column_fragment(const char* tile, int place, int k)
+{
     typedef __attribute__((address_space(3))) bf16x4* lds4;
-    const bf16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(tile + unit_byte<U>(r, unit) + 8 * half));
-    const bf16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(tile + unit_byte<U>(r + 4, unit) + 8 * half));
+    const bf16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(tile + (place ^ (64 * k))));
+    const bf16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(tile + (place ^ (64 * k) ^ (U > 2 ? 32 : 0)) + 64 * U));
     return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
@@ -291,7 +305,6 @@ struct TileLoad
     static constexpr int U = COLS / UNIT, UNITS = L::C * U, COUNT = (UNITS + L::THREADS - 1) / L::THREADS, STEP = L::THREADS / U;
     static_assert((UNITS % L::THREADS == 0 || COUNT == 1) && STEP * U == L::THREADS);
     RawUnit<T> raw[COUNT];
-    const T* at;  // the thread's first unit of the next chunk
 
     // A row's last, partial unit is read as the 8 values that end with it, and moved down by this much. `left`: the values of a row that are
     // there from the tile's first, c0, on.
@@ -301,14 +314,14 @@ struct TileLoad
         return left - c >= UNIT || left - c <= 0 || c0 + left < UNIT ? 0 : UNIT - (left - c);
     }
 
-    // `base`: the first row's value c0.
-    __device__ __forceinline__ void begin(const T* base, int64_t stride, int c0, int left)
+    // The thread's first unit of a tile whose first row begins at `base`, with value c0.
+    static __device__ __forceinline__ const T* begin(const T* base, int64_t stride, int c0, int left)
     {
-        at = base + (int)threadIdx.x / U * stride + ((int)threadIdx.x % U * UNIT - down(c0, left));
+        return base + (int)threadIdx.x / U * stride + ((int)threadIdx.x % U * UNIT - down(c0, left));
     }
 
-    // The next chunk, of n rows; whole: all of the tile is there.
-    __device__ __forceinline__ void load(int64_t stride, bool whole, int n, int c0, int left)
+    // The chunk at `at`, which goes on to the next one: n rows; whole: all of the tile is there.
+    __device__ __forceinline__ void load(const T*& at, int64_t stride, bool whole, int n, int c0, int left)
     {
         if (whole)
         {
@@ -425,24 +438,24 @@ __device__ __forceinline__ void move_state(float* __restrict__ lds, const States
 
 // ONLY: the segments' own states (from 0) to the workspace, of all but the last of a sequence; no results.
 template <typename T, typename L, bool ONLY>
-__global__ __launch_bounds__(L::THREADS, L::BLOCKS) void attention_walk_kernel(Sequences seq, Segments segments, int heads,
+__global__ __launch_bounds__(L::THREADS, L::WAVES) void attention_walk_kernel(Sequences seq, Segments segments, int heads,
                                                                                const float* __restrict__ log_decay, Passes passes, int tiles)
 {
     constexpr int C = L::C, DK = L::DK, N = L::N, PL = L::PL, PS = L::PS, RT = C / 16, KS = C / 32, KD = DK / 32;
     constexpr int UD = DK / UNIT, UN = N / UNIT, UC = C / UNIT;
     __shared__ __align__(16) char lds[ONLY ? PL * (L::AB + L::V) : L::LDS];
     __shared__ Spoiled<L> spoiled;
+    __shared__ Decay kept[2][L::W];  // the decays of a chunk, and of the segment's last one: each wave's own, to spare registers
     char* const tb = lds;
     char* const tc = tb + PL * L::AB;
     char* const ta = ONLY ? nullptr : tc + PL * L::V;
-    char* const tp = ONLY ? nullptr : ta + PL * L::AB;
+    char* const tp = ONLY ? nullptr : ta + L::A;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
     const Pass& p = passes.p[blockIdx.y];
     const int s = p.backwards ? 1 : 0;
-    auto clear_scores = [&] {
-        for (int i = threadIdx.x; i < PS * L::P / 16; i += L::THREADS) ((uint4*)tp)[i] = make_uint4(0, 0, 0, 0);
-    };
-    if constexpr (!ONLY) clear_scores();
+    static_assert(32 * N * 4 <= PL * (L::AB + L::V));  // 32 rows of the state on their way, which the scores outlive
+    if constexpr (!ONLY)
+        for (int i = threadIdx.x; i < PS * L::P / 16; i += L::THREADS) ((uint4*)tp)[i] = make_uint4(0, 0, 0, 0);  // above the diagonal they stay so
     clear_spoiled(spoiled);
     int chunk = 0;
 
@@ -481,11 +494,8 @@ __global__ __launch_bounds__(L::THREADS, L::BLOCKS) void attention_walk_kernel(S
         const float lg = uniform(log_decay_of(log_decay, head)), lg2 = uniform(lg * 1.4426950408889634f);
         auto power = [&](int n) { return __builtin_amdgcn_exp2f(lg2 * (float)n); };
         const float update = p.update, read = p.read;
-        const Decay chunk_decay(lg, C), end_decay(lg, (double)(n_all % C));
-        const float e16 = uniform(power(16));
-        float tail[UNIT];  // e^(7 - v) of 8 rows of c
-#pragma unroll
-        for (int v = 0; v < UNIT; ++v) tail[v] = uniform(power(UNIT - 1 - v) * update);
+        const float e1 = uniform(power(1)), e16 = uniform(power(16));
+        kept[0][wave] = Decay(lg, C), kept[1][wave] = Decay(lg, (double)((n_all + C - 1) % C + 1));
 
         // The state: from the workspace, as lanes hold it, or the pass's first, 32 rows at a time through LDS.
         f32x4 S[KD][2] = {};
@@ -513,8 +523,6 @@ __global__ __launch_bounds__(L::THREADS, L::BLOCKS) void attention_walk_kernel(S
                         for (int r = 0; r < 4; ++r) S[u][h][r] = ((const float*)lds)[(8 * g + 4 * h + r) * N + (16 * wave + l % 16)];
                 __syncthreads();
             }
-            // The scores above the diagonal are where some of it was.
-            if constexpr (!ONLY) clear_scores();
         }
 
         // Position 0's rows; the rows of later positions follow, or come before it where time runs backwards.
@@ -522,38 +530,46 @@ __global__ __launch_bounds__(L::THREADS, L::BLOCKS) void attention_walk_kernel(S
         auto row_base = [&](const TokenRows& r) {
             return (const T*)r.p + (seq.offsets ? 0 : part.q.batch * r.batch_stride) + t0 * r.token_stride + head / r.share * r.head_stride;
         };
-        const T* __restrict__ pa = ONLY ? nullptr : row_base(p.a);
-        const T* __restrict__ pb = row_base(p.b);
-        const T* __restrict__ pc = row_base(p.c);
+        const T* pa = ONLY ? nullptr : row_base(p.a);
+        const T* pb = row_base(p.b);
+        const T* pc = row_base(p.c);
         const int64_t sa = dir * p.a.token_stride, sb = dir * p.b.token_stride, sc = dir * p.c.token_stride;
-        TileLoad<T, L, DK> la, lb;
-        TileLoad<T, L, N> lc;
-        if constexpr (!ONLY) la.begin(pa, sa, 0, p.dim);
-        lb.begin(pb, sb, 0, p.dim);
-        lc.begin(pc + col0, sc, col0, cols - col0);
+        pa = ONLY ? nullptr : TileLoad<T, L, DK>::begin(pa, sa, 0, p.dim);
+        pb = TileLoad<T, L, DK>::begin(pb, sb, 0, p.dim);
+        pc = TileLoad<T, L, N>::begin(pc + col0, sc, col0, cols - col0);
         const bool wide = p.dim == DK && col0 + N <= cols;
-        auto load = [&](int64_t first) {
-            const int n = (int)(n_all - first < C ? n_all - first : C);
-            const bool whole = wide && n == C;
-            if constexpr (!ONLY) la.load(sa, whole, n, 0, p.dim);
-            lb.load(sb, whole, n, 0, p.dim);
-            lc.load(sc, whole, n, col0, cols - col0);
-        };
-        if (n_all > 0) load(0);
-        for (int64_t first = 0; first < n_all; first += C)
+        struct Stage
         {
-            const int n = (int)(n_all - first < C ? n_all - first : C);
+            TileLoad<T, L, DK> a, b;
+            TileLoad<T, L, N> c;
+        } stage;
+        const int chunks = (int)((n_all + C - 1) / C), rest = (int)(n_all - (int64_t)(chunks - 1) * C);  // and the last one's rows
+        auto load = [&](Stage& st, int i) {
+            const int n = i + 1 < chunks ? C : rest;
+            const bool whole = wide && n == C;
+            if constexpr (!ONLY) st.a.load(pa, sa, whole, n, 0, p.dim);
+            st.b.load(pb, sb, whole, n, 0, p.dim);
+            st.c.load(pc, sc, whole, n, col0, cols - col0);
+        };
+        // Where the next chunk's result goes.
+        const int64_t out_step = dir * heads * cols;
+        int64_t out0 = ((row0 + t0 - part.q.start) * heads + head) * cols + col0;
+        if (chunks > 0) load(stage, 0);
+        for (int i0 = 0; i0 < chunks; ++i0)
+        {
+            const int n = i0 + 1 < chunks ? C : rest;
             ++chunk;
             // The lane's places in LDS follow from this copy anew in every chunk: kept from chunk to chunk they would fill the registers.
             int l = threadIdx.x % WAVE;
             asm volatile("" : "+v"(l));
-            const int g = l / 16;
+            const int g = l / 16, row_d = row_place<UD>(l), row_c = row_place<UC>(l), column_d = column_place<UD>(l, l & 3);
+            const int column_n = column_place<UN>(l, 2 * wave + ((l >> 1) & 1)) + 8 * (l & 1), score_c = unit_byte<UC>(l % 16, g >> 1) + 8 * (g & 1);
             __syncthreads();
-            if constexpr (!ONLY) la.store(ta, wide, 0, p.dim);
-            lb.store(tb, wide, 0, p.dim);
-            lc.store(tc, wide, col0, cols - col0);
-            if ((int)lb.spoiled() | (int)lc.spoiled()) spoiled.any = chunk;
-            if (first + C < n_all) load(first + C);
+            if constexpr (!ONLY) stage.a.store(ta, wide, 0, p.dim);
+            stage.b.store(tb, wide, 0, p.dim);
+            stage.c.store(tc, wide, col0, cols - col0);
+            if ((int)stage.b.spoiled() | (int)stage.c.spoiled()) spoiled.any = chunk;
+            if (!L::LATE && i0 + 1 < chunks) load(stage, i0 + 1);
             __syncthreads();
             const bool spoils = spoiled.any == chunk;
             if (spoils)
@@ -571,9 +587,9 @@ __global__ __launch_bounds__(L::THREADS, L::BLOCKS) void attention_walk_kernel(S
             {
                 // Scores, decayed, in terms to LDS: tiles of 16 x 16 on and below the diagonal, by the waves in turn.
 #pragma unroll
-                for (int i0 = 0; i0 < RT * (RT + 1) / 2; i0 += L::W)
+                for (int t0 = 0; t0 < RT * (RT + 1) / 2; t0 += L::W)
                 {
-                    const int index = i0 + wave;
+                    const int index = t0 + wave;
                     if (index >= RT * (RT + 1) / 2) break;
                     const int rt = index < 1 ? 0 : index < 3 ? 1 : index < 6 ? 2 : 3, ct = index - rt * (rt + 1) / 2;
                     f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -584,8 +600,8 @@ __global__ __launch_bounds__(L::THREADS, L::BLOCKS) void attention_walk_kernel(S
 #pragma unroll
                         for (int i = 0; i < PL; ++i)
                         {
-                            fa[i] = row_fragment<UD>(ta + i * L::AB, l, 16 * rt, k);
-                            fb[i] = row_fragment<UD>(tb + i * L::AB, l, 16 * ct, k);
+                            fa[i] = row_fragment(ta + i * L::AB + rt * (256 * UD), row_d, k);
+                            fb[i] = row_fragment(tb + i * L::AB + ct * (256 * UD), row_d, k);
                         }
 #pragma unroll
                         for (int i = 0; i < PL; ++i)
@@ -604,30 +620,26 @@ __global__ __launch_bounds__(L::THREADS, L::BLOCKS) void attention_walk_kernel(S
                     }
                     else
                     {
-                        const float near = power(gap - 3) * read;
+                        float near = power(gap - 3) * (update * read);
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) v[r] = x[r] * (near * tail[4 + r]);
+                        for (int r = 3; r >= 0; --r, near *= e1) v[r] = x[r] * near;
                     }
                     __bf16 term[PS][4];
                     split<PS, false>(v, term);
 #pragma unroll
                     for (int i = 0; i < PS; ++i)
-                        *(bf16x4*)(tp + i * L::P + unit_byte<UC>(16 * rt + l % 16, 2 * ct + (g >> 1)) + 8 * (g & 1)) = term_vector<bf16x4>(term, i);
+                        *(bf16x4*)(tp + i * L::P + rt * (256 * UC) + (score_c ^ (32 * ct))) = term_vector<bf16x4>(term, i);
                     __builtin_amdgcn_sched_barrier(0);
                 }
-                // a S, with the state's terms as they lie in the lanes; the next 32 rows' fragments of a are read while these are multiplied.
-                bf16x8 fa[2][RT][PL];
-                auto read_a = [&](int u) {
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                        for (int i = 0; i < PL; ++i) fa[u % 2][rt][i] = row_fragment<UD>(ta + i * L::AB, l, 16 * rt, u);
-                };
-                read_a(0);
+                // a S, with the state's terms as they lie in the lanes.
 #pragma unroll
                 for (int u = 0; u < KD; ++u)
                 {
-                    if (u + 1 < KD) read_a(u + 1);
+                    bf16x8 fa[RT][PL];
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                        for (int i = 0; i < PL; ++i) fa[rt][i] = row_fragment(ta + i * L::AB + rt * (256 * UD), row_d, u);
                     {
                         float v[UNIT];
 #pragma unroll
@@ -642,7 +654,7 @@ __global__ __launch_bounds__(L::THREADS, L::BLOCKS) void attention_walk_kernel(S
                             for (int i = 0; i < PL; ++i)
                                 if (i + j < PS)
 #pragma unroll
-                                    for (int rt = 0; rt < RT; ++rt) o[rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fs, fa[u % 2][rt][i], o[rt], 0, 0, 0);
+                                    for (int rt = 0; rt < RT; ++rt) o[rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fs, fa[rt][i], o[rt], 0, 0, 0);
                         }
                     }
                     __builtin_amdgcn_sched_barrier(0);
@@ -654,138 +666,171 @@ __global__ __launch_bounds__(L::THREADS, L::BLOCKS) void attention_walk_kernel(S
                 __syncthreads();
             }
 
-            // Scores times c, and the state after the chunk.
+            const float nan = __builtin_nanf("");
+            if constexpr (!ONLY)
+            {
+                // Scores times c, and out.
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks)
+                {
+                    bf16x8 fc[PL];
+#pragma unroll
+                    for (int i = 0; i < PL; ++i) fc[i] = column_fragment<UN>(tc + i * L::V + ks * (512 * UN), column_n, 0);
+#pragma unroll
+                    for (int j = 0; j < PS; ++j)
+#pragma unroll
+                        for (int rt = 2 * ks; rt < RT; ++rt)
+                        {
+                            const bf16x8 fp = row_fragment(tp + j * L::P + rt * (256 * UC), row_c, ks);
+#pragma unroll
+                            for (int i = 0; i < PL; ++i)
+                                if (i + j < PS) o[rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fc[i], fp, o[rt], 0, 0, 0);
+                        }
+                }
+                if (spoils)
+                {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                    {
+                        const int from = min(spoiled.row, spoiled.col[16 * wave + 4 * g + r]);
+#pragma unroll
+                        for (int rt = 0; rt < RT; ++rt)
+                            if (16 * rt + l % 16 >= from) o[rt][r] = nan;
+                    }
+                }
+                if (p.out32)
+                {
+                    const int c = col0 + 16 * wave + 4 * g;
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt)
+                    {
+                        if (16 * rt + l % 16 >= n) continue;
+                        float* __restrict__ to = p.out32 + out0 + (16 * rt + l % 16) * out_step + 16 * wave + 4 * g;
+                        if (c + 4 <= cols)
+                            __builtin_memcpy(to, &o[rt], 16);
+                        else
+#pragma unroll
+                            for (int j = 0; j < 3; ++j)
+                                if (c + j < cols) to[j] = o[rt][j];
+                    }
+                }
+                else if (p.out)
+                {
+                    // Through a's tile, which nobody reads any more, so that whole rows go to memory at once.
+                    typedef T Tx4 __attribute__((ext_vector_type(4)));
+                    constexpr int E = 16 / (int)sizeof(T), UO = N / E;
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt)
+                    {
+                        const Tx4 v = __builtin_convertvector(o[rt], Tx4);
+                        __builtin_memcpy(ta + rt * (256 * UO) + unit_byte<UO>(l % 16, (16 * wave + 4 * g) / E) + (4 * g) % E * (int)sizeof(T), &v, sizeof(v));
+                    }
+                    __syncthreads();
+                    T* __restrict__ out = (T*)p.out + out0;
+#pragma unroll
+                    for (int i = 0; i < C * UO / L::THREADS; ++i)
+                    {
+                        const int u = threadIdx.x + i * L::THREADS, r = u / UO, x = u % UO;
+                        if (r >= n) break;
+                        T* __restrict__ to = out + r * out_step + x * E;
+                        const uint4 v = *(const uint4*)(ta + unit_byte<UO>(r, x));
+                        if (col0 + (x + 1) * E <= cols)
+                        {
+                            __builtin_memcpy(to, &v, 16);
+                        }
+                        else
+                        {
+                            const uint32_t d[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                            for (int j = 0; j < E - 1; ++j)
+                                if (col0 + x * E + j < cols)
+                                {
+                                    if constexpr (sizeof(T) == 4)
+                                        to[j] = __builtin_bit_cast(T, d[j]);
+                                    else
+                                        to[j] = __builtin_bit_cast(T, (uint16_t)(d[j / 2] >> (16 * (j % 2))));
+                                }
+                        }
+                    }
+                }
+                out0 += C * out_step;
+                __builtin_amdgcn_sched_barrier(0);
+            }
+
+            if (L::LATE && i0 + 1 < chunks) load(stage, i0 + 1);
+            __builtin_amdgcn_sched_barrier(0);
+
+            // The state after the chunk.
             const bool whole = n == C;
-            const Decay decay = whole ? chunk_decay : end_decay;
+            const Decay decay = kept[i0 + 1 < chunks ? 0 : 1][wave];
 #pragma unroll
             for (int u = 0; u < KD; ++u)
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) S[u][h][r] = decay.of(S[u][h][r]);
+                    for (int r = 0; r < 4; ++r) S[u][h][r] = decay.of(S[u][h][r]);
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
             {
-                bf16x8 fc[PL], fd[3];
+                bf16x8 fd[3];
                 // e^(n - 1 + s - j) of the lane's last row j = 32 ks + 8 g + 7 (rows behind the chunk's end are 0).
                 const int past = n - 1 + s - (32 * ks + 8 * g + 7);
-                const float base = power(past);
                 {
                     float v[UNIT] = {};
 #pragma unroll
                     for (int i = 0; i < PL; ++i)
                     {
-                        fc[i] = column_fragment<UN>(tc + i * L::V, l, 32 * ks, 2 * wave + ((l & 3) >> 1), l & 1);
+                        const bf16x8 fc = column_fragment<UN>(tc + i * L::V + ks * (512 * UN), column_n, 0);
 #pragma unroll
-                        for (int j = 0; j < UNIT; ++j) v[j] += (float)fc[i][j];
+                        for (int j = 0; j < UNIT; ++j) v[j] += (float)fc[j];
                     }
+                    if (whole)
+                    {
+                        float w = power(past) * update;
 #pragma unroll
-                    for (int j = 0; j < UNIT; ++j) v[j] *= whole ? tail[j] * base : past + 7 - j >= 0 ? power(past + 7 - j) * update : 0.0f;
+                        for (int j = UNIT - 1; j >= 0; --j, w *= e1) v[j] *= w;
+                    }
+                    else
+                    {
+#pragma unroll
+                        for (int j = 0; j < UNIT; ++j) v[j] *= past + 7 - j >= 0 ? power(past + 7 - j) * update : 0.0f;
+                    }
                     __bf16 term[3][UNIT];
                     split<3, false>(v, term);
 #pragma unroll
                     for (int i = 0; i < 3; ++i) fd[i] = term_vector<bf16x8>(term, i);
                 }
-                if constexpr (!ONLY)
+                // b's columns for 32 rows of the state at a time.
+#pragma unroll
+                for (int u = 0; u < KD; ++u)
                 {
+                    bf16x8 fb[2][PL];
 #pragma unroll
-                    for (int rt = 2 * ks; rt < RT; ++rt)
+                    for (int h = 0; h < 2; ++h)
 #pragma unroll
-                        for (int j = 0; j < PS; ++j)
-                        {
-                            const bf16x8 fp = row_fragment<UC>(tp + j * L::P, l, 16 * rt, ks);
-#pragma unroll
-                                for (int i = 0; i < PL; ++i)
-                                    if (i + j < PS) o[rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fc[i], fp, o[rt], 0, 0, 0);
-                        }
-                }
-                __builtin_amdgcn_sched_barrier(0);
-                // b's columns for 16 rows of the state at a time, the next ones read while these are multiplied.
-                bf16x8 fb[2][PL];
-                auto read_b = [&](int uh) {
-#pragma unroll
-                    for (int i = 0; i < PL; ++i) fb[uh % 2][i] = column_fragment<UD>(tb + i * L::AB, l, 32 * ks, 4 * (uh / 2) + (l & 3), uh % 2);
-                };
-                read_b(0);
-#pragma unroll
-                for (int uh = 0; uh < 2 * KD; ++uh)
-                {
-                    if (uh + 1 < 2 * KD) read_b(uh + 1);
+                        for (int i = 0; i < PL; ++i) fb[h][i] = column_fragment<UD>(tb + i * L::AB + ks * (512 * UD) + 8 * h, column_d, u);
 #pragma unroll
                     for (int j = 0; j < 3; ++j)
 #pragma unroll
                         for (int i = 0; i < PL; ++i)
                             if (i + j <= 2)
-                                    S[uh / 2][uh % 2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[uh % 2][i], fd[j], S[uh / 2][uh % 2], 0, 0, 0);
-                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                                for (int h = 0; h < 2; ++h) S[u][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[h][i], fd[j], S[u][h], 0, 0, 0);
+                    if (L::LATE || u % 2) __builtin_amdgcn_sched_barrier(0);
                 }
             }
             if (spoils)
             {
-                const float nan = __builtin_nanf("");
-                {
-                    const int by = spoiled.col[(16 * wave + l % 16)];
+                const int by = spoiled.col[16 * wave + l % 16];
 #pragma unroll
-                    for (int u = 0; u < KD; ++u)
+                for (int u = 0; u < KD; ++u)
 #pragma unroll
-                        for (int h = 0; h < 2; ++h)
-#pragma unroll
-                            for (int r = 0; r < 4; ++r)
-                                if (by < C || spoiled.dim[32 * u + 8 * g + 4 * h + r]) S[u][h][r] = nan;
-                    if constexpr (!ONLY)
-                    {
+                    for (int h = 0; h < 2; ++h)
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
-                        {
-                            const int from = min(spoiled.row, spoiled.col[16 * wave + 4 * g + r]);
-#pragma unroll
-                            for (int rt = 0; rt < RT; ++rt)
-                                if (16 * rt + l % 16 >= from) o[rt][r] = nan;
-                        }
-                    }
-                }
+                            if (by < C || spoiled.dim[32 * u + 8 * g + 4 * h + r]) S[u][h][r] = nan;
                 __syncthreads();
                 clear_spoiled(spoiled);
-            }
-            if constexpr (!ONLY)
-            {
-                if (p.out)
-                {
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt)
-                    {
-                        const int i = 16 * rt + l % 16;
-                        if (i >= n) continue;
-                        const int64_t pos = part.first + first + i, row = row0 + (s ? part.q.length - 1 - pos : pos);
-                        const int c = col0 + 16 * wave + 4 * g;
-                        const int64_t to = (row * heads + head) * cols + c;
-                        if (c + 4 <= cols)
-                        {
-                            if (p.out32)
-                            {
-                                __builtin_memcpy(p.out32 + to, &o[rt], 16);
-                            }
-                            else
-                            {
-                                typedef T Tx4 __attribute__((ext_vector_type(4)));
-                                const Tx4 v = __builtin_convertvector(o[rt], Tx4);
-                                __builtin_memcpy((T*)p.out + to, &v, sizeof(v));
-                            }
-                        }
-                        else
-                        {
-#pragma unroll
-                            for (int j = 0; j < 3; ++j)
-                            {
-                                if (c + j >= cols) break;
-                                if (p.out32)
-                                    p.out32[to + j] = o[rt][j];
-                                else
-                                    ((T*)p.out)[to + j] = (T)o[rt][j];
-                            }
-                        }
-                    }
-                }
             }
         }
 
@@ -812,7 +857,6 @@ __global__ __launch_bounds__(L::THREADS, L::BLOCKS) void attention_walk_kernel(S
                 move_state<L>((float*)lds, p.last, state0, 32 * u, p.dim, col0, cols, false);
                 __syncthreads();
             }
-            if constexpr (!ONLY) clear_scores();
         }
     }
 }

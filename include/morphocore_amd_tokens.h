@@ -42,7 +42,7 @@ typedef struct
     int interleaved;
 } mca_rotation;
 
-/* out [tokens, x.heads, dim] = x rotated, or by the negative angles (the gradient). dim up to 512. */
+/* out [tokens, x.heads, dim] = x rotated, or by the negative angles (the gradient). dim up to 512, heads up to 65536. */
 int mca_axial_rotary(int dtype, const mca_heads* x, void* out, int64_t tokens, int64_t dim, const mca_rotation* rotation, int inverse,
                      void* stream);
 

@@ -28,79 +28,132 @@ hipError_t sum_shared_heads(const float* part, T* out, int64_t rows, int heads, 
     return hipGetLastError();
 }
 
-// One head of one sequence of the batch, `COLS` columns. Rows of the batch that name the same slot are taken by the first of them, in order.
-template <typename T>
+// Bound by HBM: the states are read once and written once, float32. A workgroup has 4 LC columns of one head's state in registers, 4
+// neighbouring values a thread in every RB-th row, all loads in flight at once; q S is summed over a thread's rows, the lanes and
+// the waves, in a fixed order. Rows of the batch that name the same slot are taken by the first of them, in order, the state staying
+// where it is.
+template <typename T, int LC, int R>
 __global__ __launch_bounds__(BLOCK) void attention_step_kernel(TokenRows q, TokenRows k, TokenRows v, const float* __restrict__ log_decay,
                                                                float* __restrict__ states, int64_t slot_stride, int64_t head_stride,
                                                                const void* __restrict__ slot_of, bool wide, int64_t slots, T* __restrict__ out,
-                                                               int64_t batch, int heads, int dim, int cols, float scale, int tiles)
+                                                               int64_t batch, int heads, int dim, int cols, float scale, int tiles, bool streaming)
 {
-    constexpr int ROWS = 64;
-    __shared__ float sq[256], sk[256], part[NWAVES][WAVE];
-    const int tile = blockIdx.x % tiles, head = blockIdx.x / tiles % heads;
-    const int64_t first = blockIdx.x / tiles / heads;
+    constexpr int RB = BLOCK / LC;
+    static_assert(LC <= WAVE);
+    __shared__ float sq[RB * R], sk[RB * R];
+    __shared__ f32x4 part[NWAVES][LC];
+    const int lane = threadIdx.x % LC, row0 = threadIdx.x / LC;
     auto slot_at = [&](int64_t b) -> int64_t {
         if (!slot_of) return b;
         return wide ? ((const int64_t*)slot_of)[b] : (int64_t)((const int32_t*)slot_of)[b];
     };
-    const int64_t slot = slot_at(first);
-    const int col = tile * WAVE + threadIdx.x % WAVE, wave = threadIdx.x / WAVE;
-    auto store = [&](int64_t b, float x) {
-        if (wave == 0 && col < cols) out[(b * heads + head) * cols + col] = (T)x;
-    };
-    if (slot < 0 || slot >= slots)
+    const int64_t work = batch * heads * tiles;
+    for (int64_t item = blockIdx.x; item < work; item += gridDim.x)
     {
-        store(first, 0.0f);
-        return;
-    }
-    if (slot_of)
-    {
-        bool before = false;
-        for (int64_t b = threadIdx.x; b < first; b += BLOCK) before |= slot_at(b) == slot;
-        if (__syncthreads_or(before)) return;
-    }
-    const Decay decay(log_decay_of(log_decay, head), 1);
-    float* __restrict__ state = states + slot * slot_stride + head * head_stride;
-    float s[ROWS];
-#pragma unroll
-    for (int i = 0; i < ROWS; ++i)
-    {
-        const int row = NWAVES * i + wave;
-        s[i] = row < dim && col < cols ? state[(int64_t)row * cols + col] : 0.0f;
-    }
-    for (int64_t b = first; b < batch; ++b)
-    {
-        if (b > first && (!slot_of || slot_at(b) != slot)) continue;
-        const T* rq = (const T*)q.p + b * q.token_stride + head / q.share * q.head_stride;
-        const T* rk = (const T*)k.p + b * k.token_stride + head / k.share * k.head_stride;
-        __syncthreads();
-        if ((int)threadIdx.x < dim)
+        const int tile = (int)(item % tiles), head = (int)(item / tiles % heads);
+        const int64_t first = item / tiles / heads, slot = slot_at(first);
+        const int col = (tile * LC + lane) * 4, valid = min(max(cols - col, 0), 4);
+        if (slot < 0 || slot >= slots)
         {
-            sq[threadIdx.x] = (float)rq[threadIdx.x];
-            sk[threadIdx.x] = (float)rk[threadIdx.x];
+            if (threadIdx.x < LC)
+                for (int j = 0; j < valid; ++j) out[(first * heads + head) * cols + col + j] = (T)0.0f;
+            continue;
         }
-        __syncthreads();
-        const float c = col < cols ? (float)((const T*)v.p + b * v.token_stride + head / v.share * v.head_stride)[col] : 0.0f;
-        float x = 0.0f;
+        float* __restrict__ state = states + slot * slot_stride + head * head_stride + col;
+        f32x4 s[R];
 #pragma unroll
-        for (int i = 0; i < ROWS; ++i)
+        for (int i = 0; i < R; ++i)
         {
-            const int r = NWAVES * i + wave;
-            if (r < dim)
+            const int row = RB * i + row0;
+            s[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            if (row >= dim) continue;
+            if (valid == 4)
+                __builtin_memcpy(&s[i], state + (int64_t)row * cols, 16);
+            else
+#pragma unroll
+                for (int j = 0; j < 3; ++j)
+                    if (j < valid) s[i][j] = state[(int64_t)row * cols + j];
+        }
+        bool again = false;
+        if (slot_of)
+        {
+            bool before = false, after = false;
+            for (int64_t b = threadIdx.x; b < batch; b += BLOCK)
             {
-                s[i] = fmaf(sk[r], c, decay.of(s[i]));
-                x = fmaf(sq[r], s[i], x);
+                const bool same = b != first && slot_at(b) == slot;
+                before |= same && b < first;
+                after |= same && b > first;
+            }
+            if (__syncthreads_or(before)) continue;
+            again = __syncthreads_or(after);
+        }
+        const Decay decay(log_decay_of(log_decay, head), 1);
+        for (int64_t b = first; b < batch; ++b)
+        {
+            if (b > first && (!again || slot_at(b) != slot))
+            {
+                if (!again) break;
+                continue;
+            }
+            __syncthreads();
+            for (int i = threadIdx.x; i < dim; i += BLOCK)
+            {
+                sq[i] = (float)((const T*)q.p + b * q.token_stride + head / q.share * q.head_stride)[i];
+                sk[i] = (float)((const T*)k.p + b * k.token_stride + head / k.share * k.head_stride)[i];
+            }
+            const T* __restrict__ pv = (const T*)v.p + b * v.token_stride + head / v.share * v.head_stride + col;
+            f32x4 c = {0.0f, 0.0f, 0.0f, 0.0f}, x = c;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (j < valid) c[j] = (float)pv[j];
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+            {
+                const int row = RB * i + row0;
+                if (row >= dim) continue;
+                const float a = sq[row], w = sk[row];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                {
+                    s[i][j] = fmaf(w, c[j], decay.of(s[i][j]));
+                    x[j] = fmaf(a, s[i][j], x[j]);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int d = LC; d < WAVE; d *= 2) x[j] += __shfl_xor(x[j], d);
+            if (threadIdx.x % WAVE < LC) part[threadIdx.x / WAVE][lane] = x;
+            __syncthreads();
+            if (threadIdx.x < LC)
+            {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (j < valid)
+                        out[(b * heads + head) * cols + col + j] =
+                            (T)(scale * ((part[0][lane][j] + part[1][lane][j]) + (part[2][lane][j] + part[3][lane][j])));
             }
         }
-        part[wave][threadIdx.x % WAVE] = x;
-        __syncthreads();
-        store(b, scale * ((part[0][threadIdx.x % WAVE] + part[1][threadIdx.x % WAVE]) + (part[2][threadIdx.x % WAVE] + part[3][threadIdx.x % WAVE])));
-    }
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i)
-    {
-        const int row = NWAVES * i + wave;
-        if (row < dim && col < cols) state[(int64_t)row * cols + col] = s[i];
+        for (int i = 0; i < R; ++i)
+        {
+            const int row = RB * i + row0;
+            if (row >= dim) continue;
+            float* __restrict__ to = state + (int64_t)row * cols;
+            if (valid == 4)
+            {
+                typedef f32x4 unaligned __attribute__((aligned(4)));
+                if (streaming)
+                    __builtin_nontemporal_store(s[i], (unaligned*)to);
+                else
+                    *(unaligned*)to = s[i];
+            }
+            else
+#pragma unroll
+                for (int j = 0; j < 3; ++j)
+                    if (j < valid) to[j] = s[i][j];
+        }
     }
 }
 
@@ -110,10 +163,31 @@ hipError_t linear_attention_step(TokenRows q, TokenRows k, TokenRows v, const fl
                                  int cols, float scale, hipStream_t stream)
 {
     if (batch <= 0 || heads <= 0) return hipSuccess;
-    const int tiles = (cols + WAVE - 1) / WAVE;
-    attention_step_kernel<T><<<(unsigned)(batch * heads * tiles), BLOCK, 0, stream>>>(q, k, v, log_decay, states, slot_stride, head_stride,
-                                                                                     slot_of, wide, slots, out, batch, heads, dim, cols, scale, tiles);
-    return hipGetLastError();
+    const bool streaming = streams(8.0 * (double)batch * heads * dim * cols);
+    auto run = [&](auto lc, auto r) {
+        constexpr int LC = decltype(lc)::value, R = decltype(r)::value;
+        const int tiles = (cols + 4 * LC - 1) / (4 * LC);
+        const int64_t work = batch * heads * tiles, most = 1 << 20;
+        attention_step_kernel<T, LC, R><<<(unsigned)(work < most ? work : most), BLOCK, 0, stream>>>(
+            q, k, v, log_decay, states, slot_stride, head_stride, slot_of, wide, slots, out, batch, heads, dim, cols, scale, tiles, streaming);
+        return hipGetLastError();
+    };
+    using std::integral_constant;
+    auto by_rows = [&](auto lc) {
+        constexpr int LC = decltype(lc)::value, RB = BLOCK / LC, MOST = 256 / RB;
+        if constexpr (MOST >= 8)
+        {
+            if (dim <= RB * (MOST / 8)) return run(lc, integral_constant<int, MOST / 8>());
+        }
+        if (dim <= RB * (MOST / 4)) return run(lc, integral_constant<int, MOST / 4>());
+        if (dim <= RB * (MOST / 2)) return run(lc, integral_constant<int, MOST / 2>());
+        return run(lc, integral_constant<int, MOST>());
+    };
+    // Whole rows of the state at once, up to 512 bytes, where there are workgroups enough; parts of 128 bytes otherwise.
+    if (cols > 64 && batch * heads >= 512) return by_rows(integral_constant<int, 32>());
+    if (cols > 32 && batch * heads >= 256) return by_rows(integral_constant<int, 16>());
+    if (cols > 16) return by_rows(integral_constant<int, 8>());
+    return by_rows(integral_constant<int, 4>());
 }
 
 #define MCA_ATTENTION(T)                                                                                                                       \

@@ -5,9 +5,9 @@
 //   grad_x = r (t - m mean(t m)),  grad_w = sum over tokens and heads of g m.
 //
 // Bound by HBM: every row is read once and written once. A lane holds 8 pairs (their two halves apart, or side by
-// side) or 16 values behind the last pair, so the lanes of a row exchange only the norm's sums. The lanes of a row take
-// heads of one token in turn and form its 8 angles each once, without a table in memory; queries and keys share
-// them in one launch. Few tokens are spread over more groups of lanes, each with fewer heads.
+// side) or 16 values behind the last pair, so the lanes of a row exchange only the norm's sums. A workgroup takes a few
+// tokens: it forms their sines and cosines once, in LDS, then all their heads, of queries and keys, in the order in which they lie in
+// memory. Few tokens' heads are spread over several workgroups.
 //
 // Angles are float64 up to a fraction of a turn: in float32 a position of 100000 would be off by 0.004 radians. What is
 // left of a turn goes through float32 sine and cosine, the rounding of a result.
@@ -76,56 +76,44 @@ struct Turn
     float cos[UNIT], sin[UNIT];
 };
 
-__device__ __forceinline__ Turn turn_of(const Rotation& r, int64_t token, const RowPart& p, bool inverse)
+// The sine and cosine of a token's pair.
+__device__ __forceinline__ void sine_cosine(const Rotation& r, int64_t token, int pair, bool inverse, float& sine, float& cosine)
 {
     const int64_t row = token < r.rows ? token : token % r.rows;
-    double angle[UNIT] = {};
+    double angle = 0.0;
     for (int a = 0; a < r.axes; ++a)
     {
         const int64_t at = row * r.axes + a;
         const double position = r.position_type == MCA_POSITION_INT32   ? (double)((const int32_t*)r.positions)[at]
                                 : r.position_type == MCA_POSITION_INT64 ? (double)((const int64_t*)r.positions)[at]
                                                                         : (double)((const float*)r.positions)[at];
-#pragma unroll
-        for (int e = 0; e < UNIT; ++e)
-            if (e < p.pairs) angle[e] = fma(position, r.frequencies[(int64_t)a * r.pairs + p.pair + e], angle[e]);
+        angle = fma(position, r.frequencies[(int64_t)a * r.pairs + pair], angle);
     }
-    Turn t;
-#pragma unroll
-    for (int e = 0; e < UNIT; ++e)
-    {
-        const double turns = angle[e] * 0.15915494309189535;  // 1 / (2 pi)
-        sincospif((float)(2.0 * (turns - rint(turns))), &t.sin[e], &t.cos[e]);
-        if (inverse) t.sin[e] = -t.sin[e];
-    }
-    return t;
+    const double turns = angle * 0.15915494309189535;  // 1 / (2 pi)
+    sincospif((float)(2.0 * (turns - rint(turns))), &sine, &cosine);
+    if (inverse) sine = -sine;
 }
 
-// Of a lane behind the pairs the angles are 0, which leaves its values as they are (but for a NaN beside an infinity).
-__device__ __forceinline__ void rotate(float (&v)[2][UNIT], const Turn& t, bool interleaved, bool turned)
+__device__ __forceinline__ void turn_pair(float& a, float& b, float c, float s)
 {
-    if (!turned) return;
-    if (interleaved)
+    const float x = a * c - b * s;
+    b = b * c + a * s;
+    a = x;
+}
+
+// Of a unit's pairs those that are there.
+template <bool INTERLEAVED>
+__device__ __forceinline__ void rotate(float (&v)[2][UNIT], const Turn& t, int pairs)
+{
+    if constexpr (INTERLEAVED)
     {
 #pragma unroll
-        for (int e = 0; e < UNIT; ++e)
-        {
-            float &a = v[e / 4][2 * e % UNIT], &b = v[e / 4][2 * e % UNIT + 1];
-            const float x = a * t.cos[e] - b * t.sin[e];
-            b = b * t.cos[e] + a * t.sin[e];
-            a = x;
-        }
+        for (int e = 0; e < UNIT; ++e) turn_pair(v[e / 4][2 * e % UNIT], v[e / 4][2 * e % UNIT + 1], e < pairs ? t.cos[e] : 1.0f, e < pairs ? t.sin[e] : 0.0f);
     }
     else
     {
 #pragma unroll
-        for (int e = 0; e < UNIT; ++e)
-        {
-            float &a = v[0][e], &b = v[1][e];
-            const float x = a * t.cos[e] - b * t.sin[e];
-            b = b * t.cos[e] + a * t.sin[e];
-            a = x;
-        }
+        for (int e = 0; e < UNIT; ++e) turn_pair(v[0][e], v[1][e], e < pairs ? t.cos[e] : 1.0f, e < pairs ? t.sin[e] : 0.0f);
     }
 }
 
@@ -145,34 +133,56 @@ struct RotaryTensor
     T* out;
 };
 
-template <typename T, typename WT, int G, int MODE>
-__global__ __launch_bounds__(BLOCK) void rotary_kernel(RotaryTensor<T, WT> q, RotaryTensor<T, WT> k, int64_t tokens, int splits, int dim,
+// Sines and cosines that a workgroup holds: of as many tokens as have them, 16 at most.
+constexpr int ROTARY_TABLE = 256, ROTARY_TOKENS = 16;
+
+inline int rotary_tokens(int pairs) { return pairs * ROTARY_TOKENS <= ROTARY_TABLE ? ROTARY_TOKENS : ROTARY_TABLE / pairs; }
+
+// Workgroup item b: tokens [b / splits * per, ..), every splits-th share of their rows.
+template <typename T, typename WT, int G, int MODE, bool INTERLEAVED>
+__global__ __launch_bounds__(BLOCK) void rotary_kernel(RotaryTensor<T, WT> q, RotaryTensor<T, WT> k, int64_t tokens, int per, int splits, int dim,
                                                        Rotation r, bool inverse, float eps, float* __restrict__ gw_part, bool streaming)
 {
     constexpr int GROUPS = BLOCK / G;
-    const int lane = threadIdx.x % G;
+    __shared__ __align__(16) float cosines[ROTARY_TABLE + UNIT], sines[ROTARY_TABLE + UNIT];
+    const int lane = threadIdx.x % G, group = threadIdx.x / G;
     const RowPart part = row_part(lane, dim, r);
     const float inv = 1.0f / (float)dim;
-    const int64_t groups = tokens * splits;
-    float gw[2][2][UNIT] = {};
-    for (int64_t group = (int64_t)blockIdx.x * GROUPS + threadIdx.x / G; group < groups; group += (int64_t)gridDim.x * GROUPS)
+    RawUnit<WT> w[2][2];
+    if constexpr (MODE != ROTATE)
     {
-        const int64_t token = group / splits;
-        const int split = (int)(group - token * splits);
-        const Turn turn = turn_of(r, token, part, inverse);
+        if (q.x.heads > 0) load_part(q.w, part, w[0]);
+        if (k.x.heads > 0) load_part(k.w, part, w[1]);
+    }
+    float gw[2][2][UNIT] = {};
+    const int64_t items = (tokens + per - 1) / per * splits;
+    for (int64_t item = blockIdx.x; item < items; item += gridDim.x)
+    {
+        const int64_t token0 = item / splits * per;
+        const int split = (int)(item % splits), n = (int)(tokens - token0 < per ? tokens - token0 : per);
+        __syncthreads();
+        for (int i = threadIdx.x; i < n * r.pairs; i += BLOCK) sine_cosine(r, token0 + i / r.pairs, i % r.pairs, inverse, sines[i], cosines[i]);
+        __syncthreads();
 #pragma unroll
         for (int which = 0; which < 2; ++which)
         {
             const RotaryTensor<T, WT>& t = which ? k : q;
-            RawUnit<WT> w[2];
-            if (MODE != ROTATE && t.x.heads > 0) load_part(t.w, part, w);
-            // The second tensor's heads go on where the first one's end, so that the groups have equal shares.
-            const int first = which ? (splits - q.x.heads % splits + split) % splits : split;
-            for (int head = first; head < t.x.heads; head += splits)
+            const float per_head = 1.0f / (float)t.x.heads;
+            for (int i = split * GROUPS + group; i < n * t.x.heads; i += splits * GROUPS)
             {
+                const int at = (int)(((float)i + 0.5f) * per_head), head = i - at * t.x.heads;  // exact below 2^20
+                const int64_t token = token0 + at;
                 RawUnit<T> raw[2], rawh[2];
                 load_part(t.x.x + token * t.x.token_stride + head * t.x.head_stride, part, raw);
                 if (MODE == NORM_BACKWARD) load_part(t.h.x + token * t.h.token_stride + head * t.h.head_stride, part, rawh);
+                Turn turn;
+#pragma unroll
+                for (int e = 0; e < UNIT; ++e)
+                {
+                    // (A partial unit's further ones are other pairs', or what lies behind the table, for values that are not there.)
+                    turn.cos[e] = cosines[min(at * r.pairs + part.pair, ROTARY_TABLE) + e];
+                    turn.sin[e] = sines[min(at * r.pairs + part.pair, ROTARY_TABLE) + e];
+                }
                 float v[2][UNIT];
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
@@ -189,9 +199,9 @@ __global__ __launch_bounds__(BLOCK) void rotary_kernel(RotaryTensor<T, WT> q, Ro
 #pragma unroll
                     for (int i = 0; i < 2; ++i)
 #pragma unroll
-                        for (int j = 0; j < UNIT; ++j) v[i][j] = v[i][j] * rstd * w[i][j];
+                        for (int j = 0; j < UNIT; ++j) v[i][j] = v[i][j] * rstd * w[which][i][j];
                 }
-                rotate(v, turn, r.interleaved, part.pairs > 0);
+                rotate<INTERLEAVED>(v, turn, part.pairs);
                 if constexpr (MODE == NORM_BACKWARD)
                 {
                     float s = 0.0f, d = 0.0f;
@@ -201,7 +211,7 @@ __global__ __launch_bounds__(BLOCK) void rotary_kernel(RotaryTensor<T, WT> q, Ro
                         for (int j = 0; j < UNIT; ++j)
                         {
                             s = fmaf(rawh[i][j], rawh[i][j], s);
-                            d = fmaf(v[i][j] * w[i][j], rawh[i][j], d);
+                            d = fmaf(v[i][j] * w[which][i][j], rawh[i][j], d);
                         }
                     const float rstd = 1.0f / sqrtf(fmaf(lane_sum<G>(s), inv, eps));
                     const float mean = lane_sum<G>(d) * rstd * inv;
@@ -212,7 +222,7 @@ __global__ __launch_bounds__(BLOCK) void rotary_kernel(RotaryTensor<T, WT> q, Ro
                         {
                             const float m = rawh[i][j] * rstd;
                             gw[which][i][j] = fmaf(v[i][j], m, gw[which][i][j]);
-                            v[i][j] = rstd * (v[i][j] * w[i][j] - m * mean);
+                            v[i][j] = rstd * (v[i][j] * w[which][i][j] - m * mean);
                         }
                 }
                 if (t.out) store_part(t.out + (token * t.x.heads + head) * dim, part, v, streaming);
@@ -255,13 +265,6 @@ __global__ __launch_bounds__(BLOCK) void rotary_kernel(RotaryTensor<T, WT> q, Ro
     }
 }
 
-// Groups of lanes that a launch aims at: 4 waves for each of the 1024 SIMDs.
-static int rotary_splits(int64_t tokens, int heads, int lanes)
-{
-    const int64_t want = 4096 * (int64_t)(WAVE / lanes), s = (want + tokens - 1) / tokens;
-    return (int)(s < 1 ? 1 : s > heads ? heads : s);
-}
-
 template <typename F>
 static hipError_t by_lanes(int lanes, F&& f)
 {
@@ -277,17 +280,22 @@ static hipError_t by_lanes(int lanes, F&& f)
 
 struct RotaryPlan
 {
-    int splits, blocks;
+    int per, splits, blocks;
 };
 
-// Slots of grad_w's partial sums: one a workgroup.
+// Few tokens' rows go to several workgroups, down to one row a group of lanes.
 template <int G>
-static RotaryPlan rotary_plan(int64_t tokens, int heads, int64_t most)
+static RotaryPlan rotary_plan(int64_t tokens, int heads, int pairs, int64_t most)
 {
+    constexpr int64_t ENOUGH = 1024;
     RotaryPlan p;
-    p.splits = rotary_splits(tokens, heads, G);
-    const int64_t groups = tokens * p.splits, blocks = (groups + BLOCK / G - 1) / (BLOCK / G);
-    p.blocks = (int)(blocks < most ? blocks : most);
+    p.per = rotary_tokens(pairs);
+    while (p.per > 1 && (tokens + p.per - 1) / p.per < ENOUGH) p.per = (p.per + 1) / 2;
+    const int64_t blocks = (tokens + p.per - 1) / p.per, rows = ((int64_t)p.per * heads + BLOCK / G - 1) / (BLOCK / G);
+    const int64_t want = (ENOUGH + blocks - 1) / blocks;
+    p.splits = (int)(want < rows ? want : rows);
+    if (p.splits < 1) p.splits = 1;
+    p.blocks = (int)(blocks * p.splits < most ? blocks * p.splits : most);
     return p;
 }
 
@@ -302,8 +310,11 @@ static hipError_t rotary_launch(const RotaryTensor<T, WT>& q, const RotaryTensor
     const bool streaming = streams(values * sizeof(T) * (MODE == NORM_BACKWARD ? 3.0 : 2.0));
     return by_lanes(rotary_lanes(dim, r.pairs), [&](auto g) {
         constexpr int G = decltype(g)::value;
-        const RotaryPlan p = rotary_plan<G>(tokens, heads, MODE == NORM_BACKWARD ? ROTARY_SLOTS : ROTARY_BLOCKS);
-        rotary_kernel<T, WT, G, MODE><<<p.blocks, BLOCK, 0, stream>>>(q, k, tokens, p.splits, dim, r, inverse, eps, gw_part, streaming);
+        const RotaryPlan p = rotary_plan<G>(tokens, heads, r.pairs, MODE == NORM_BACKWARD ? ROTARY_SLOTS : ROTARY_BLOCKS);
+        if (r.interleaved)
+            rotary_kernel<T, WT, G, MODE, true><<<p.blocks, BLOCK, 0, stream>>>(q, k, tokens, p.per, p.splits, dim, r, inverse, eps, gw_part, streaming);
+        else
+            rotary_kernel<T, WT, G, MODE, false><<<p.blocks, BLOCK, 0, stream>>>(q, k, tokens, p.per, p.splits, dim, r, inverse, eps, gw_part, streaming);
         return hipGetLastError();
     });
 }
@@ -329,7 +340,7 @@ static int rotary_slots(int64_t tokens, int heads, int dim, int pairs)
 {
     int slots = 0;
     (void)by_lanes(rotary_lanes(dim, pairs), [&](auto g) {
-        slots = rotary_plan<decltype(g)::value>(tokens, heads, ROTARY_SLOTS).blocks;
+        slots = rotary_plan<decltype(g)::value>(tokens, heads, pairs, ROTARY_SLOTS).blocks;
         return hipSuccess;
     });
     return slots;

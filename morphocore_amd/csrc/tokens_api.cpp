@@ -11,6 +11,8 @@ namespace
 
 // What the lanes of one wave hold of a head's row, and the rows and columns of the state that a workgroup holds.
 constexpr int64_t MAX_ROTARY_DIM = 512, MAX_STATE_DIM = 256, MAX_AXES = 8;
+// Rows of a workgroup's tokens are told apart in float32.
+constexpr int64_t MAX_ROTARY_HEADS = 65536;
 
 int check_types(int dtype, int weight_dtype)
 {
@@ -44,6 +46,11 @@ int check_rotation(const mca_rotation* r, int64_t tokens, int64_t dim)
     if (r->rows < 0 || (tokens > 0 && r->rows == 0)) return mca::api_fail("positions must have rows");
     if (tokens > 0 && (!r->positions || (r->pairs > 0 && !r->frequencies))) return mca::api_fail("positions and frequencies must not be null");
     return MCA_OK;
+}
+
+int check_rotary_heads(const mca_heads* x)
+{
+    return x->heads > MAX_ROTARY_HEADS ? mca::api_fail("Rotations take at most 65536 heads") : MCA_OK;
 }
 
 mca::Rotation rotation_of(const mca_rotation* r)
@@ -205,7 +212,8 @@ extern "C" {
 int mca_axial_rotary(int dtype, const mca_heads* x, void* out, int64_t tokens, int64_t dim, const mca_rotation* rotation, int inverse, void* stream)
 {
     int rc;
-    if ((rc = check_types(dtype, dtype)) || (rc = check_rotation(rotation, tokens, dim)) || (rc = check_heads(x, tokens, dim))) return rc;
+    if ((rc = check_types(dtype, dtype)) || (rc = check_rotation(rotation, tokens, dim)) || (rc = check_heads(x, tokens, dim)) || (rc = check_rotary_heads(x)))
+        return rc;
     if (tokens > 0 && x->heads > 0 && !out) return mca::api_fail("out must not be null");
     return by_type(dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
@@ -220,7 +228,7 @@ int mca_rms_norm_rotary_forward(int dtype, int weight_dtype, const mca_heads* q,
     if ((rc = check_types(dtype, weight_dtype)) || (rc = check_rotation(rotation, tokens, dim)) || (rc = check_heads(q, tokens, dim)) ||
         (rc = check_heads(k, tokens, dim)))
         return rc;
-    if (q->heads + k->heads > INT32_MAX) return mca::api_fail("Too many heads");
+    if ((rc = check_rotary_heads(q)) || (rc = check_rotary_heads(k))) return rc;
     if (!(eps >= 0.0f)) return mca::api_fail("eps must be non negative");
     if (tokens > 0 && ((q->heads > 0 && (!q_weight || !out_q)) || (k->heads > 0 && (!k_weight || !out_k))))
         return mca::api_fail("weights and results must not be null");
@@ -234,7 +242,7 @@ int mca_rms_norm_rotary_forward(int dtype, int weight_dtype, const mca_heads* q,
 
 size_t mca_rms_norm_rotary_backward_workspace_size(int64_t tokens, int64_t heads, int64_t dim, int64_t pairs)
 {
-    if (tokens < 0 || heads < 0 || heads > INT32_MAX || dim < 1 || dim > MAX_ROTARY_DIM || pairs < 0 || 2 * pairs > dim) return 0;
+    if (tokens < 0 || heads < 0 || heads > 2 * MAX_ROTARY_HEADS || dim < 1 || dim > MAX_ROTARY_DIM || pairs < 0 || 2 * pairs > dim) return 0;
     return mca::rms_norm_rotary_backward_workspace(tokens, (int)heads, (int)dim, (int)pairs);
 }
 
@@ -247,7 +255,7 @@ int mca_rms_norm_rotary_backward(int dtype, int weight_dtype, const mca_heads* g
     if ((rc = check_types(dtype, weight_dtype)) || (rc = check_rotation(rotation, tokens, dim)) || (rc = check_heads(grad_out_q, tokens, dim)) ||
         (rc = check_heads(grad_out_k, tokens, dim)) || (rc = check_heads(q, tokens, dim)) || (rc = check_heads(k, tokens, dim)))
         return rc;
-    if (q->heads + k->heads > INT32_MAX) return mca::api_fail("Too many heads");
+    if ((rc = check_rotary_heads(q)) || (rc = check_rotary_heads(k))) return rc;
     if (grad_out_q->heads != q->heads || grad_out_k->heads != k->heads) return mca::api_fail("A gradient must have its tensor's heads");
     if (!(eps >= 0.0f)) return mca::api_fail("eps must be non negative");
     if (tokens > 0 && ((q->heads > 0 && !q_weight) || (k->heads > 0 && !k_weight))) return mca::api_fail("weights must not be null");

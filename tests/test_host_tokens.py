@@ -193,7 +193,8 @@ def test_abi_refuses_rotations():
     refused(norm(eps=float("nan")), "eps")
     refused(norm(qw=None), "must not be null")
     refused(norm(out_k=None), "must not be null")
-    refused(norm(k=heads(2**31 - 1, strides=(0, 0, 0))), "Too many heads")
+    refused(norm(k=heads(65537, strides=(0, 0, 0))), "at most 65536 heads")
+    refused(call(x=heads(65537, strides=(0, 0, 0))), "at most 65536 heads")
     need = lib.mca_rms_norm_rotary_backward_workspace_size(4, 3, 8, 4)
     assert need > 0 and lib.mca_rms_norm_rotary_backward_workspace_size(0, 3, 8, 4) == 0
     assert lib.mca_rms_norm_rotary_backward_workspace_size(4, 3, 513, 4) == 0

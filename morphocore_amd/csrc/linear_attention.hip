@@ -33,7 +33,7 @@ hipError_t sum_shared_heads(const float* part, T* out, int64_t rows, int heads, 
 // the waves, in a fixed order. Rows of the batch that name the same slot are taken by the first of them, in order, the state staying
 // where it is.
 template <typename T, int LC, int R>
-__global__ __launch_bounds__(BLOCK) void attention_step_kernel(TokenRows q, TokenRows k, TokenRows v, const float* __restrict__ log_decay,
+__global__ __launch_bounds__(BLOCK, R <= 16 ? 4 : 2) void attention_step_kernel(TokenRows q, TokenRows k, TokenRows v, const float* __restrict__ log_decay,
                                                                float* __restrict__ states, int64_t slot_stride, int64_t head_stride,
                                                                const void* __restrict__ slot_of, bool wide, int64_t slots, T* __restrict__ out,
                                                                int64_t batch, int heads, int dim, int cols, float scale, int tiles, bool streaming)

@@ -138,7 +138,7 @@ constexpr int ROTARY_TABLE = 256, ROTARY_TOKENS = 16;
 
 inline int rotary_tokens(int pairs) { return pairs * ROTARY_TOKENS <= ROTARY_TABLE ? ROTARY_TOKENS : ROTARY_TABLE / pairs; }
 
-// Workgroup item b: tokens [b / splits * per, ..), every splits-th share of their rows.
+// Workgroup item b: tokens [b / splits * per, ..), every splits-th share of their rows, of one of the tensors.
 template <typename T, typename WT, int G, int MODE, bool INTERLEAVED>
 __global__ __launch_bounds__(BLOCK) void rotary_kernel(RotaryTensor<T, WT> q, RotaryTensor<T, WT> k, int64_t tokens, int per, int splits, int dim,
                                                        Rotation r, bool inverse, float eps, float* __restrict__ gw_part, bool streaming)
@@ -148,13 +148,10 @@ __global__ __launch_bounds__(BLOCK) void rotary_kernel(RotaryTensor<T, WT> q, Ro
     const int lane = threadIdx.x % G, group = threadIdx.x / G;
     const RowPart part = row_part(lane, dim, r);
     const float inv = 1.0f / (float)dim;
-    RawUnit<WT> w[2][2];
-    if constexpr (MODE != ROTATE)
-    {
-        if (q.x.heads > 0) load_part(q.w, part, w[0]);
-        if (k.x.heads > 0) load_part(k.w, part, w[1]);
-    }
-    float gw[2][2][UNIT] = {};
+    const RotaryTensor<T, WT> t = blockIdx.y ? k : q;
+    RawUnit<WT> w[2];
+    if (MODE != ROTATE && t.x.heads > 0) load_part(t.w, part, w);
+    float gw[2][UNIT] = {};
     const int64_t items = (tokens + per - 1) / per * splits;
     for (int64_t item = blockIdx.x; item < items; item += gridDim.x)
     {
@@ -163,11 +160,7 @@ __global__ __launch_bounds__(BLOCK) void rotary_kernel(RotaryTensor<T, WT> q, Ro
         __syncthreads();
         for (int i = threadIdx.x; i < n * r.pairs; i += BLOCK) sine_cosine(r, token0 + i / r.pairs, i % r.pairs, inverse, sines[i], cosines[i]);
         __syncthreads();
-#pragma unroll
-        for (int which = 0; which < 2; ++which)
-        {
-            const RotaryTensor<T, WT>& t = which ? k : q;
-            const float per_head = 1.0f / (float)t.x.heads;
+        const float per_head = 1.0f / (float)t.x.heads;
             for (int i = split * GROUPS + group; i < n * t.x.heads; i += splits * GROUPS)
             {
                 const int at = (int)(((float)i + 0.5f) * per_head), head = i - at * t.x.heads;  // exact below 2^20
@@ -199,7 +192,7 @@ __global__ __launch_bounds__(BLOCK) void rotary_kernel(RotaryTensor<T, WT> q, Ro
 #pragma unroll
                     for (int i = 0; i < 2; ++i)
 #pragma unroll
-                        for (int j = 0; j < UNIT; ++j) v[i][j] = v[i][j] * rstd * w[which][i][j];
+                        for (int j = 0; j < UNIT; ++j) v[i][j] = v[i][j] * rstd * w[i][j];
                 }
                 rotate<INTERLEAVED>(v, turn, part.pairs);
                 if constexpr (MODE == NORM_BACKWARD)
@@ -211,7 +204,7 @@ __global__ __launch_bounds__(BLOCK) void rotary_kernel(RotaryTensor<T, WT> q, Ro
                         for (int j = 0; j < UNIT; ++j)
                         {
                             s = fmaf(rawh[i][j], rawh[i][j], s);
-                            d = fmaf(v[i][j] * w[which][i][j], rawh[i][j], d);
+                            d = fmaf(v[i][j] * w[i][j], rawh[i][j], d);
                         }
                     const float rstd = 1.0f / sqrtf(fmaf(lane_sum<G>(s), inv, eps));
                     const float mean = lane_sum<G>(d) * rstd * inv;
@@ -221,47 +214,38 @@ __global__ __launch_bounds__(BLOCK) void rotary_kernel(RotaryTensor<T, WT> q, Ro
                         for (int j = 0; j < UNIT; ++j)
                         {
                             const float m = rawh[i][j] * rstd;
-                            gw[which][i][j] = fmaf(v[i][j], m, gw[which][i][j]);
-                            v[i][j] = rstd * (v[i][j] * w[which][i][j] - m * mean);
+                            gw[i][j] = fmaf(v[i][j], m, gw[i][j]);
+                            v[i][j] = rstd * (v[i][j] * w[i][j] - m * mean);
                         }
                 }
                 if (t.out) store_part(t.out + (token * t.x.heads + head) * dim, part, v, streaming);
             }
-        }
     }
     if constexpr (MODE == NORM_BACKWARD)
     {
         if (!gw_part) return;
         // Over the groups of a wave, then over the waves, in a fixed order, into the workgroup's slot.
-        __shared__ float sums[NWAVES][2][G][2 * UNIT];
+        __shared__ float sums[NWAVES][G][2 * UNIT];
 #pragma unroll
-        for (int which = 0; which < 2; ++which)
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < UNIT; ++j)
-                {
-                    float s = gw[which][i][j];
-#pragma unroll
-                    for (int d = G; d < WAVE; d *= 2) s += __shfl_xor(s, d);
-                    if (threadIdx.x % WAVE < G) sums[threadIdx.x / WAVE][which][lane][i * UNIT + j] = s;
-                }
-        __syncthreads();
-        float* __restrict__ out = gw_part + (int64_t)blockIdx.x * 2 * dim;
-        for (int which = threadIdx.x / WAVE; which < 2; which += NWAVES)
-            for (int l = threadIdx.x % WAVE; l < G; l += WAVE)
+            for (int j = 0; j < UNIT; ++j)
             {
-                const RowPart p = row_part(l, dim, r);
+                float s = gw[i][j];
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int j = 0; j < UNIT; ++j)
-                        if (j < p.valid[i])
-                        {
-                            const int at = i * UNIT + j;
-                            out[which * dim + p.c[i] + j] = ((sums[0][which][l][at] + sums[1][which][l][at]) + sums[2][which][l][at]) + sums[3][which][l][at];
-                        }
+                for (int d = G; d < WAVE; d *= 2) s += __shfl_xor(s, d);
+                if (threadIdx.x % WAVE < G) sums[threadIdx.x / WAVE][lane][i * UNIT + j] = s;
             }
+        __syncthreads();
+        float* __restrict__ out = gw_part + ((int64_t)blockIdx.x * 2 + blockIdx.y) * dim;
+        for (int i = threadIdx.x; i < G * 2 * UNIT; i += BLOCK)
+        {
+            const int l = i / (2 * UNIT), at = i % (2 * UNIT);
+            const RowPart p = row_part(l, dim, r);
+            const int half = at / UNIT, j = at % UNIT;
+            if (j < (half ? p.valid[1] : p.valid[0]))
+                out[(half ? p.c[1] : p.c[0]) + j] = ((sums[0][l][at] + sums[1][l][at]) + sums[2][l][at]) + sums[3][l][at];
+        }
     }
 }
 
@@ -305,16 +289,16 @@ template <int MODE, typename T, typename WT>
 static hipError_t rotary_launch(const RotaryTensor<T, WT>& q, const RotaryTensor<T, WT>& k, int64_t tokens, int dim, const Rotation& r, bool inverse,
                                 float eps, float* gw_part, hipStream_t stream)
 {
-    const int heads = q.x.heads + k.x.heads;
-    const double values = (double)tokens * heads * dim;
+    const int heads = q.x.heads > k.x.heads ? q.x.heads : k.x.heads, tensors = k.out || gw_part ? 2 : 1;
+    const double values = (double)tokens * ((double)q.x.heads + k.x.heads) * dim;
     const bool streaming = streams(values * sizeof(T) * (MODE == NORM_BACKWARD ? 3.0 : 2.0));
     return by_lanes(rotary_lanes(dim, r.pairs), [&](auto g) {
         constexpr int G = decltype(g)::value;
         const RotaryPlan p = rotary_plan<G>(tokens, heads, r.pairs, MODE == NORM_BACKWARD ? ROTARY_SLOTS : ROTARY_BLOCKS);
         if (r.interleaved)
-            rotary_kernel<T, WT, G, MODE, true><<<p.blocks, BLOCK, 0, stream>>>(q, k, tokens, p.per, p.splits, dim, r, inverse, eps, gw_part, streaming);
+            rotary_kernel<T, WT, G, MODE, true><<<dim3(p.blocks, tensors), BLOCK, 0, stream>>>(q, k, tokens, p.per, p.splits, dim, r, inverse, eps, gw_part, streaming);
         else
-            rotary_kernel<T, WT, G, MODE, false><<<p.blocks, BLOCK, 0, stream>>>(q, k, tokens, p.per, p.splits, dim, r, inverse, eps, gw_part, streaming);
+            rotary_kernel<T, WT, G, MODE, false><<<dim3(p.blocks, tensors), BLOCK, 0, stream>>>(q, k, tokens, p.per, p.splits, dim, r, inverse, eps, gw_part, streaming);
         return hipGetLastError();
     });
 }
@@ -365,7 +349,7 @@ hipError_t rms_norm_rotary_backward(HeadRows<T> gy_q, HeadRows<T> gy_k, HeadRows
         if (err != hipSuccess) return err;
     }
     if (!grad_weights) return hipSuccess;
-    return sum_slots_async<WT>(part, none ? 0 : rotary_slots(tokens, q.heads + k.heads, dim, r.pairs), 2 * (int64_t)dim, grad_weights, stream);
+    return sum_slots_async<WT>(part, none ? 0 : rotary_slots(tokens, q.heads > k.heads ? q.heads : k.heads, dim, r.pairs), 2 * (int64_t)dim, grad_weights, stream);
 }
 
 #define MCA_ROTARY(T, WT)                                                                                                                    \

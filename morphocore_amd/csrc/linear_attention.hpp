@@ -156,9 +156,12 @@ struct Walk
     static constexpr int AB = C * DK * 2, V = C * N * 2, P = C * C * 2;  // bytes of a term's tile
     static constexpr int OUT = C * N * (PL == 3 ? 4 : 2), A = PL * AB > OUT ? PL * AB : OUT;  // a's tile is out's too
     static constexpr int LDS = A + PL * AB + PL * V + PS * P;
+    static constexpr int64_t CUS = 256, CU_LDS = 160 * 1024;
     // Where two workgroups' tiles fit, registers are kept to what lets two run: the next chunk is loaded late.
     static constexpr bool LATE = W == 8 && LDS <= 76 * 1024;
     static constexpr int WAVES = LATE ? 4 : W >= 4 ? 2 : 1;  // a SIMD, at least
+    // Workgroups that a CU runs at once, by their tiles and registers (8 waves a CU, 16 where they are kept to that).
+    static constexpr int64_t BY_LDS = CU_LDS / LDS, BY_WAVES = (LATE ? 16 : 8) / W, TOGETHER = BY_LDS < BY_WAVES ? BY_LDS : BY_WAVES;
 };
 
 // Where unit x (8 values) of row r lies in a tile of U units a row. The 16 lanes that read 16 bytes each at once have rows 0 to 3 and 12 to 15 of unit
@@ -491,6 +494,34 @@ __global__ __launch_bounds__(L::THREADS, L::WAVES) void attention_walk_kernel(Se
         // A sequence without rows has one segment (number 0), which hands its state on.
         if (ONLY ? last || n_all == 0 : n_all == 0 && part.number != 0) continue;
 
+        // Position 0's rows; the rows of later positions follow, or come before it where time runs backwards.
+        const int64_t dir = s ? -1 : 1, t0 = part.q.start + (s ? part.q.length - 1 - part.first : part.first);
+        auto row_base = [&](const TokenRows& r) {
+            return (const T*)r.p + (seq.offsets ? 0 : part.q.batch * r.batch_stride) + t0 * r.token_stride + head / r.share * r.head_stride;
+        };
+        const T* pa = ONLY ? nullptr : row_base(p.a);
+        const T* pb = row_base(p.b);
+        const T* pc = row_base(p.c);
+        const int64_t sa = dir * p.a.token_stride, sb = dir * p.b.token_stride, sc = dir * p.c.token_stride;
+        pa = ONLY ? nullptr : TileLoad<T, L, DK>::begin(pa, sa, 0, p.dim);
+        pb = TileLoad<T, L, DK>::begin(pb, sb, 0, p.dim);
+        pc = TileLoad<T, L, N>::begin(pc + col0, sc, col0, cols - col0);
+        const bool wide = p.dim == DK && col0 + N <= cols;
+        struct Stage
+        {
+            TileLoad<T, L, DK> a, b;
+            TileLoad<T, L, N> c;
+        } stage;
+        const int chunks = (int)((n_all + C - 1) / C), rest = (int)(n_all - (int64_t)(chunks - 1) * C);  // and the last one's rows
+        auto load = [&](Stage& st, int i) {
+            const int n = i + 1 < chunks ? C : rest;
+            const bool whole = wide && n == C;
+            if constexpr (!ONLY) st.a.load(pa, sa, whole, n, 0, p.dim);
+            st.b.load(pb, sb, whole, n, 0, p.dim);
+            st.c.load(pc, sc, whole, n, col0, cols - col0);
+        };
+        if (chunks > 0) load(stage, 0);
+
         const float lg = uniform(log_decay_of(log_decay, head)), lg2 = uniform(lg * 1.4426950408889634f);
         auto power = [&](int n) { return __builtin_amdgcn_exp2f(lg2 * (float)n); };
         const float update = p.update, read = p.read;
@@ -525,36 +556,9 @@ __global__ __launch_bounds__(L::THREADS, L::WAVES) void attention_walk_kernel(Se
             }
         }
 
-        // Position 0's rows; the rows of later positions follow, or come before it where time runs backwards.
-        const int64_t dir = s ? -1 : 1, t0 = part.q.start + (s ? part.q.length - 1 - part.first : part.first);
-        auto row_base = [&](const TokenRows& r) {
-            return (const T*)r.p + (seq.offsets ? 0 : part.q.batch * r.batch_stride) + t0 * r.token_stride + head / r.share * r.head_stride;
-        };
-        const T* pa = ONLY ? nullptr : row_base(p.a);
-        const T* pb = row_base(p.b);
-        const T* pc = row_base(p.c);
-        const int64_t sa = dir * p.a.token_stride, sb = dir * p.b.token_stride, sc = dir * p.c.token_stride;
-        pa = ONLY ? nullptr : TileLoad<T, L, DK>::begin(pa, sa, 0, p.dim);
-        pb = TileLoad<T, L, DK>::begin(pb, sb, 0, p.dim);
-        pc = TileLoad<T, L, N>::begin(pc + col0, sc, col0, cols - col0);
-        const bool wide = p.dim == DK && col0 + N <= cols;
-        struct Stage
-        {
-            TileLoad<T, L, DK> a, b;
-            TileLoad<T, L, N> c;
-        } stage;
-        const int chunks = (int)((n_all + C - 1) / C), rest = (int)(n_all - (int64_t)(chunks - 1) * C);  // and the last one's rows
-        auto load = [&](Stage& st, int i) {
-            const int n = i + 1 < chunks ? C : rest;
-            const bool whole = wide && n == C;
-            if constexpr (!ONLY) st.a.load(pa, sa, whole, n, 0, p.dim);
-            st.b.load(pb, sb, whole, n, 0, p.dim);
-            st.c.load(pc, sc, whole, n, col0, cols - col0);
-        };
         // Where the next chunk's result goes.
         const int64_t out_step = dir * heads * cols;
         int64_t out0 = ((row0 + t0 - part.q.start) * heads + head) * cols + col0;
-        if (chunks > 0) load(stage, 0);
         for (int i0 = 0; i0 < chunks; ++i0)
         {
             const int n = i0 + 1 < chunks ? C : rest;
@@ -861,14 +865,14 @@ __global__ __launch_bounds__(L::THREADS, L::WAVES) void attention_walk_kernel(Se
     }
 }
 
-// Turns the segments' own states into the states after them, sequence by sequence: one value of a tile's state a thread.
+// Turns the segments' own states into the states after them, sequence by sequence: 4 values of a tile's state a thread.
 template <typename L>
 __global__ __launch_bounds__(BLOCK) void attention_join_kernel(Sequences seq, Segments segments, int heads, const float* __restrict__ log_decay,
                                                                Passes passes, int tiles)
 {
-    constexpr int VALUES = (int)state_values<L>(), BLOCKS = (VALUES + BLOCK - 1) / BLOCK;
+    constexpr int QUADS = (int)state_values<L>() / 4, BLOCKS = (QUADS + BLOCK - 1) / BLOCK;
     const Pass& p = passes.p[blockIdx.y];
-    const int64_t spans = seq.offsets ? seq.count : seq.count, work = spans * heads * tiles * BLOCKS;
+    const int64_t work = seq.count * heads * tiles * BLOCKS;
     for (int64_t item = blockIdx.x; item < work; item += gridDim.x)
     {
         const int block = (int)(item % BLOCKS), tile = (int)(item / BLOCKS % tiles), head = (int)(item / BLOCKS / tiles % heads);
@@ -878,33 +882,41 @@ __global__ __launch_bounds__(BLOCK) void attention_join_kernel(Sequences seq, Se
         {
             const int64_t a = offset_at(seq, q), b = offset_at(seq, q + 1);
             length = b > a ? b - a : 0;
+            if (length <= segments.rows) continue;
             at = a / segments.rows + q + 1;
         }
         const int64_t count = (length + segments.rows - 1) / segments.rows - 1;  // all but the last
         const int e = block * BLOCK + threadIdx.x;
-        if (count <= 0 || e >= VALUES) continue;
-        // The value's place: see attention_walk_kernel's workspace.
-        const int r = e % 4, l = e / 4 % WAVE, h = e / 4 / WAVE % 2, u = e / 4 / WAVE / 2 % (L::DK / 32), w = e / 4 / WAVE / 2 / (L::DK / 32);
-        const int d = 32 * u + 8 * (l / 16) + 4 * h + r, c = tile * L::N + 16 * w + l % 16;
-        const Decay decay(log_decay_of(log_decay, head), (double)segments.rows);
-        float x = 0.0f;
-        if (p.first.p && d < p.dim && c < p.cols)
-            x = p.first.p[(q * heads + head) * p.dim * p.cols + d * p.first.row_stride + c * p.first.col_stride];
-        const int64_t stride = (int64_t)heads * tiles * VALUES;
-        float* __restrict__ state = passes.states[blockIdx.y] + ((at * heads + head) * tiles + tile) * VALUES + e;
+        if (e >= QUADS) continue;
+        const int64_t stride = (int64_t)heads * tiles * QUADS;
+        f32x4* __restrict__ state = (f32x4*)passes.states[blockIdx.y] + ((at * heads + head) * tiles + tile) * QUADS + e;
         constexpr int AHEAD = 8;
-        for (int64_t i = 0; i < count; i += AHEAD)
-        {
-            float own[AHEAD];
+        f32x4 own[AHEAD];
 #pragma unroll
-            for (int k = 0; k < AHEAD; ++k) own[k] = state[(i + k < count ? i + k : count - 1) * stride];
+        for (int k = 0; k < AHEAD; ++k) own[k] = state[(k < count ? k : count - 1) * stride];
+        // The values' place: see attention_walk_kernel's workspace.
+        const int l = e % WAVE, h = e / WAVE % 2, u = e / WAVE / 2 % (L::DK / 32), w = e / WAVE / 2 / (L::DK / 32);
+        const int d = 32 * u + 8 * (l / 16) + 4 * h, c = tile * L::N + 16 * w + l % 16;
+        const Decay decay(log_decay_of(log_decay, head), (double)segments.rows);
+        f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (p.first.p && c < p.cols)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (d + r < p.dim) x[r] = p.first.p[(q * heads + head) * p.dim * p.cols + (d + r) * p.first.row_stride + c * p.first.col_stride];
+        for (int64_t i = 0; i < count;)
+        {
 #pragma unroll
             for (int k = 0; k < AHEAD; ++k)
             {
                 if (i + k >= count) break;
-                x = decay.of(x) + own[k];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) x[r] = decay.of(x[r]) + own[k][r];
                 state[(i + k) * stride] = x;
             }
+            i += AHEAD;
+            if (i >= count) break;
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k) own[k] = state[(i + k < count ? i + k : count - 1) * stride];
         }
     }
 }
@@ -913,16 +925,56 @@ __global__ __launch_bounds__(BLOCK) void attention_join_kernel(Sequences seq, Se
 // Launches.
 // ------------------------------------------------------------------------------------------------
 
-// f(the shape of a pass): as few columns as hold the pass's, up to 128 a workgroup.
+template <typename L>
+int tiles_of(const Pass& p)
+{
+    return (p.cols + L::N - 1) / L::N;
+}
+
+// How long sequences are split: the rows of a segment, and an estimate of the time that it takes.
+struct Plan
+{
+    Segments segments;
+    double cost;
+};
+
+// The estimate, in half the time that two workgroups of 128 columns on a CU take for a chunk each: a chunk takes n workgroups of W waves
+// together 0.3 + 0.106 n W, a CU takes its workgroups in rounds of as many as it runs at once, and a workgroup's own cost (its first loads,
+// its state) is that of 2 + W / 2 chunks; where sequences are split, the first launch adds 0.4 of the second's time and the join 2.
+template <typename L>
+Plan plan_of(const Sequences& seq, int heads, const Pass& p)
+{
+    constexpr double OWN = 2.0 + 0.5 * L::W, JOIN = 2.0;
+    auto chunk = [](int64_t workgroups) { return workgroups ? 0.3 + 0.106 * (double)workgroups * L::W : 0.0; };
+    const int64_t walks = (seq.offsets ? 1 : seq.count) * (int64_t)heads * tiles_of<L>(p) * p.together;
+    const int64_t chunks = seq.tokens > 0 ? (seq.tokens + L::C - 1) / L::C : 1;
+    int64_t best = chunks;
+    double least = 1e300;
+    auto consider = [&](int64_t size) {
+        const int64_t parts = (chunks + size - 1) / size, items = walks * (seq.offsets ? parts + seq.count : parts);
+        const int64_t each = (items + L::CUS - 1) / L::CUS, rounds = each / L::TOGETHER, rest = each % L::TOGETHER;
+        const double time = ((double)size + OWN) * ((double)rounds * chunk(L::TOGETHER) + chunk(rest));
+        const double cost = size >= chunks ? time : 1.4 * time + JOIN;
+        if (cost < least) least = cost, best = size;
+    };
+    for (int64_t size = chunks; size > 16; size = size - size / 8) consider(size);
+    for (int64_t size = chunks < 16 ? chunks : 16; size >= 2; --size) consider(size);
+    return Plan{segments_of(seq, best * L::C), least};
+}
+
+// f(the shape of a pass): as few columns a workgroup as hold the pass's. Of more than 64, 128 where two such workgroups don't fit a CU (the
+// scores would be formed twice: 84 us instead of 57, forwards, for 4999 tokens of 6 heads of 96 x 77 in float16), otherwise 128 or 64 by the
+// estimate: 32768 tokens of 32 heads of 128 x 128 in bfloat16 take 547 us by 128 and 568 by 64; 12001 of 41 sequences take 200 and 179.
 template <typename T, typename F>
-hipError_t by_walk(const Pass& p, F&& f)
+hipError_t by_walk(const Sequences& seq, int heads, const Pass& p, F&& f)
 {
 #define MCA_WALK(DK, W) return f(Walk<T, DK, W>())
-#define MCA_WALKS(DK)                    \
-    do                                   \
-    {                                    \
-        if (p.cols <= 64) MCA_WALK(DK, 4); \
-        MCA_WALK(DK, 8);                 \
+#define MCA_WALKS(DK)                                                                                                            \
+    do                                                                                                                           \
+    {                                                                                                                            \
+        if (p.cols <= 64) MCA_WALK(DK, 4);                                                                                       \
+        if (Walk<T, DK, 8>::LATE && plan_of<Walk<T, DK, 4>>(seq, heads, p).cost < plan_of<Walk<T, DK, 8>>(seq, heads, p).cost) MCA_WALK(DK, 4); \
+        MCA_WALK(DK, 8);                                                                                                         \
     } while (0)
     if (p.dim <= 64 && p.cols <= 32)
     {
@@ -942,43 +994,14 @@ hipError_t by_walk(const Pass& p, F&& f)
 #undef MCA_WALK
 }
 
-template <typename L>
-int tiles_of(const Pass& p)
-{
-    return (p.cols + L::N - 1) / L::N;
-}
+inline bool joins(const Sequences& seq, const Segments& s) { return seq.tokens > s.rows; }
 
-// Rows of a segment. Splitting a sequence costs a second read of b and c and its states' way through memory, so it is split only where
-// there are fewer walks than the chip holds, into segments of 8 chunks at least.
+// Bytes of the segments' states of a pass.
 template <typename L>
-Segments plan_segments(const Sequences& seq, int64_t walks)
+size_t walk_states(const Sequences& seq, int heads, const Pass& p)
 {
-    constexpr int64_t TARGET = 512, LEAST = 8;
-    const int64_t chunks = (seq.tokens + L::C - 1) / L::C;
-    // Packed rows may be one sequence.
-    int64_t per = walks >= TARGET ? chunks : (chunks * walks + TARGET - 1) / TARGET;
-    per = per < LEAST ? LEAST : per;
-    if (per >= chunks) per = chunks < 1 ? 1 : chunks;
-    return segments_of(seq, per * L::C);
-}
-
-template <typename L>
-Segments plan_of(const Sequences& seq, int heads, const Pass& p, int count)
-{
-    return plan_segments<L>(seq, (seq.offsets ? 1 : seq.count) * (int64_t)heads * tiles_of<L>(p) * count);
-}
-
-template <typename L>
-bool joins(const Sequences& seq, const Segments& s)
-{
-    return seq.tokens > s.rows;
-}
-
-template <typename L>
-size_t walk_states(const Sequences& seq, int heads, const Pass& p, int count)
-{
-    const Segments s = plan_of<L>(seq, heads, p, count);
-    return joins<L>(seq, s) ? align_up((size_t)(s.count * heads * tiles_of<L>(p) * state_values<L>()) * sizeof(float)) : 0;
+    const Segments s = plan_of<L>(seq, heads, p).segments;
+    return joins(seq, s) ? align_up((size_t)(s.count * heads * tiles_of<L>(p) * state_values<L>()) * sizeof(float)) : 0;
 }
 
 template <typename T>
@@ -986,15 +1009,16 @@ size_t linear_attention_workspace(const Sequences& seq, int heads, const Pass* p
 {
     size_t bytes = 0;
     for (int i = 0; i < count; ++i)
-        (void)by_walk<T>(passes[i], [&](auto walk) {
-            bytes += walk_states<decltype(walk)>(seq, heads, passes[i], count);
+        (void)by_walk<T>(seq, heads, passes[i], [&](auto walk) {
+            bytes += walk_states<decltype(walk)>(seq, heads, passes[i]);
             return hipSuccess;
         });
     return bytes;
 }
 
 template <typename T>
-hipError_t linear_attention(const Sequences& seq, int heads, const float* log_decay, const Pass* passes, int count, void* workspace, hipStream_t stream)
+hipError_t linear_attention(const Sequences& seq, int heads, const float* log_decay, const Pass* passes, int count, void* workspace,
+                            hipStream_t stream)
 {
     if ((seq.offsets ? seq.count + seq.tokens : seq.count) <= 0 || heads <= 0) return hipSuccess;
     char* ws = (char*)workspace;
@@ -1003,25 +1027,25 @@ hipError_t linear_attention(const Sequences& seq, int heads, const float* log_de
         // Passes of the same shape go together.
         int together = 1;
         while (i + together < count && passes[i + together].dim == passes[i].dim && passes[i + together].cols == passes[i].cols) ++together;
-        const hipError_t err = by_walk<T>(passes[i], [&](auto walk) {
+        const hipError_t err = by_walk<T>(seq, heads, passes[i], [&](auto walk) {
             using L = decltype(walk);
-            const Segments s = plan_of<L>(seq, heads, passes[i], count);
+            const Segments s = plan_of<L>(seq, heads, passes[i]).segments;
             const int tiles = tiles_of<L>(passes[i]);
-            const bool split = joins<L>(seq, s);
+            const bool split = joins(seq, s);
             Passes all = {};
             for (int k = 0; k < together; ++k)
             {
                 all.p[k] = passes[i + k];
                 if (!split) continue;
                 all.states[k] = (float*)ws;
-                ws += walk_states<L>(seq, heads, passes[i + k], count);
+                ws += walk_states<L>(seq, heads, passes[i + k]);
             }
             const int64_t work = s.count * heads * tiles, most = 1 << 20;
             const dim3 grid((unsigned)(work < most ? work : most), together);
             if (split)
             {
                 attention_walk_kernel<T, L, true><<<grid, L::THREADS, 0, stream>>>(seq, s, heads, log_decay, all, tiles);
-                const int64_t values = seq.count * heads * tiles * ((state_values<L>() + BLOCK - 1) / BLOCK);
+                const int64_t values = seq.count * heads * tiles * ((state_values<L>() / 4 + BLOCK - 1) / BLOCK);
                 if (values > 0)
                     attention_join_kernel<L><<<dim3((unsigned)(values < most ? values : most), together), BLOCK, 0, stream>>>(seq, s, heads, log_decay, all, tiles);
             }

@@ -82,6 +82,7 @@ struct Pass
     int dim, cols;
     float update, read;
     bool backwards;
+    int together;  // passes of this shape that the whole call has, whichever are asked for: sequences are split by their number
 };
 
 template <typename T>

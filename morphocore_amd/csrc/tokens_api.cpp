@@ -139,6 +139,7 @@ mca::Pass forward_pass(const mca_heads* q, const mca_heads* k, const mca_heads* 
     p.first = states_of(initial, value_dim), p.last = states_of(final, value_dim);
     p.dim = (int)dim, p.cols = (int)value_dim;
     p.update = 1.0f, p.read = scale;
+    p.together = 1;
     return p;
 }
 
@@ -165,6 +166,7 @@ Backward backward_passes(const mca_heads* go, const float* grad_final, const mca
         p.first = transposed(initial, value_dim);
         p.dim = (int)value_dim, p.cols = (int)dim;
         p.update = 1.0f, p.read = scale;
+        p.together = dim == value_dim ? 3 : 2;
         b.pass[b.count++] = p;
     }
     if (grad_k)
@@ -175,6 +177,7 @@ Backward backward_passes(const mca_heads* go, const float* grad_final, const mca
         p.first = transposed(grad_final, value_dim);
         p.dim = (int)value_dim, p.cols = (int)dim;
         p.update = scale, p.read = 1.0f, p.backwards = true;
+        p.together = dim == value_dim ? 3 : 2;
         if (shared) b.part_k = mca::align_up((size_t)(rows * heads * dim) * sizeof(float));
         b.pass[b.count++] = p;
     }
@@ -186,6 +189,7 @@ Backward backward_passes(const mca_heads* go, const float* grad_final, const mca
         p.first = states_of(grad_final, value_dim), p.last = states_of(grad_initial, value_dim);
         p.dim = (int)dim, p.cols = (int)value_dim;
         p.update = scale, p.read = 1.0f, p.backwards = true;
+        p.together = dim == value_dim ? 3 : 1;
         if (shared && grad_v) b.part_v = mca::align_up((size_t)(rows * heads * value_dim) * sizeof(float));
         b.pass[b.count++] = p;
     }

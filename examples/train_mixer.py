@@ -2,12 +2,14 @@
 forward keeps for the backward.
 
     python examples/train_mixer.py [--steps 60] [--size 64] [--batch 4] [--channels 32] [--dtype bfloat16]
+                                   [--attend 4]
 
 The task: the morphological gradient (the range of each pixel's 3x3 neighbourhood) of an image, from the
 image with bright specks and dark holes in it, which an opening and a closing remove. A dilation lifts the
 image to `channels` maps; blocks of a per-channel opening or closing (kept by its input in 8 bits,
 nn.Checkpoint8) and a gated channel mixer (nn.ChannelMixer: norm with the residual, two linear layers and the
-gated activation, kept in 8 bits) follow; a linear layer reads the answer out. Needs a HIP device.
+gated activation, kept in 8 bits) follow; a linear layer reads the answer out. With --attend N each block also mixes
+its pixels with those before them by N heads of linear attention (nn.TokenMixer). Needs a HIP device.
 """
 import argparse
 import os
@@ -19,15 +21,16 @@ import torch.nn as nn
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))  # the package in place, not installed
 
 import morphocore_amd.functional as F
-from morphocore_amd.nn import ChannelMixer, Checkpoint8, Closing, Dilation, Opening, RMSNorm
+from morphocore_amd.nn import ChannelMixer, Checkpoint8, Closing, Dilation, Opening, RMSNorm, TokenMixer
 
 
 class Net(nn.Module):
-    def __init__(self, channels: int, blocks: int, dtype: torch.dtype):
+    def __init__(self, channels: int, blocks: int, dtype: torch.dtype, attend: int = 0):
         super().__init__()
         self.lift = Dilation(1, channels, 3, "sum", dtype=dtype)
         self.morph = nn.ModuleList(Checkpoint8((Opening, Closing)[i % 2](channels, channels, 3, dtype=dtype)) for i in range(blocks))
         self.mix = nn.ModuleList(ChannelMixer(channels, 2 * channels, dtype=dtype) for _ in range(blocks))
+        self.attend = nn.ModuleList(TokenMixer(channels, attend, axes=2, dtype=dtype) for _ in range(blocks if attend else 0))
         self.norm = RMSNorm(channels, dtype=dtype)
         self.read = nn.Parameter(torch.zeros(1, channels, dtype=dtype))
         with torch.no_grad():
@@ -37,9 +40,11 @@ class Net(nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         h = self.lift(x)
         out = None
-        for morph, mix in zip(self.morph, self.mix):
+        for i, (morph, mix) in enumerate(zip(self.morph, self.mix)):
             y = morph(h).permute(0, 2, 3, 1)  # channels last, as the mixer reads them
             out, last = mix(y, h.permute(0, 2, 3, 1))
+            if self.attend:
+                out, last = self.attend[i](out, last)
             h = (out + last).permute(0, 3, 1, 2).contiguous()
         y = self.norm(h.permute(0, 2, 3, 1))
         return F.linear8(y, self.read).permute(0, 3, 1, 2)
@@ -57,11 +62,11 @@ def images(batch: int, size: int, seed: int, device):
 
 
 def train(steps: int = 60, size: int = 64, batch: int = 4, channels: int = 32, blocks: int = 2, dtype: torch.dtype = torch.bfloat16,
-          lr: float = 3e-3, seed: int = 0):
+          lr: float = 3e-3, seed: int = 0, attend: int = 0):
     """Returns the losses of the steps and the bytes that a forward keeps."""
     device = torch.device("cuda")
     torch.manual_seed(seed)
-    net = Net(channels, blocks, dtype).to(device)
+    net = Net(channels, blocks, dtype, attend).to(device)
     opt = torch.optim.Adam(net.parameters(), lr=lr, eps=1e-6)
     losses, kept = [], 0
     for step in range(steps):
@@ -83,8 +88,9 @@ def main():
     ap.add_argument("--batch", type=int, default=4)
     ap.add_argument("--channels", type=int, default=32)
     ap.add_argument("--dtype", choices=["float32", "float16", "bfloat16"], default="bfloat16")
+    ap.add_argument("--attend", type=int, default=0)
     a = ap.parse_args()
-    losses, kept = train(a.steps, a.size, a.batch, a.channels, dtype=getattr(torch, a.dtype))
+    losses, kept = train(a.steps, a.size, a.batch, a.channels, dtype=getattr(torch, a.dtype), attend=a.attend)
     values = a.batch * a.channels * a.size * a.size
     for i in range(0, a.steps, max(1, a.steps // 6)):
         print(f"step {i:4d}  loss {losses[i]:.5f}")

@@ -8,8 +8,9 @@ from .smorph import SMorph
 from .stack import MorphoStack
 from .rms_norm import RMSNorm
 from .channel_mixer import ChannelMixer
+from .token_mixer import TokenMixer
 from .checkpoint8 import Checkpoint8
 from .morpho_module import MorphoModule
 from .alpha_module import AlphaModule
 
-__all__ = ['Dilation', 'Erosion', 'Opening', 'Closing', 'SigmaLayer', 'SMorph', 'MorphoStack', 'RMSNorm', 'ChannelMixer', 'Checkpoint8', 'MorphoModule', 'AlphaModule']
+__all__ = ['Dilation', 'Erosion', 'Opening', 'Closing', 'SigmaLayer', 'SMorph', 'MorphoStack', 'RMSNorm', 'ChannelMixer', 'TokenMixer', 'Checkpoint8', 'MorphoModule', 'AlphaModule']

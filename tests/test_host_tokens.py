@@ -261,3 +261,26 @@ def test_abi_refuses_attention():
     refused(step(slot_stride=-1), "slot_stride")
     refused(step(states=None), "must not be null")
     refused(step(k=heads(3)), "multiple")
+
+
+# ------------------------------------------------------------------------------------------------
+# The module
+# ------------------------------------------------------------------------------------------------
+
+def test_token_mixer():
+    m = mca.nn.TokenMixer(48, 4, axes=3, kv_heads=2, eps=1e-5)
+    shapes = {k: tuple(v.shape) for k, v in m.state_dict().items()}
+    assert shapes == {"norm.weight": (48,), "query_weight": (12,), "key_weight": (12,), "project": (96, 48), "contract": (48, 48), "log_decay": (4,)}
+    assert m.norm.eps == 1e-5 and m.frequencies.shape == (3, 6) and bool((m.frequencies.ne(0).sum(1) == 2).all())
+    # Decays and frequencies are as they were whatever the module's type becomes.
+    decay, frequencies = m.log_decay.clone(), m.frequencies.clone()
+    for t in (torch.bfloat16, torch.float64, torch.float32):
+        m = m.to(t)
+        assert m.project.dtype == t and torch.equal(m.log_decay, decay) and m.log_decay.dtype == torch.float32
+        assert torch.equal(m.frequencies, frequencies) and m.frequencies.dtype == torch.float64
+    assert torch.allclose(-1 / decay, torch.tensor([16.0, 16.0 * 2**(8 / 3), 16.0 * 2**(16 / 3), 4096.0]))
+    assert mca.nn.TokenMixer(8, 1).log_decay.tolist() == [-1 / 16] and mca.nn.TokenMixer(8, 2, dim=7).frequencies.shape == (1, 3)
+    for bad in (lambda: mca.nn.TokenMixer(0, 1), lambda: mca.nn.TokenMixer(8, 0), lambda: mca.nn.TokenMixer(8, 4, kv_heads=3),
+                lambda: mca.nn.TokenMixer(8, 4, axes=2), lambda: mca.nn.TokenMixer(8, 1, axes=0), lambda: mca.nn.TokenMixer(8, 2, kv_heads=0)):
+        with pytest.raises(ValueError):
+            bad()

@@ -23,6 +23,8 @@
 // changes from row to row, so that row and transposing reads both spread over the banks.
 #pragma once
 
+#include <cmath>
+
 #include "block8.hpp"
 #include "launch.hpp"
 #include "tokens.hpp"
@@ -85,17 +87,19 @@ __device__ __forceinline__ int64_t span_start(const Sequences& s, int64_t i)
 }
 
 // Segments. Sequences of one length have the same number each; span i of packed rows has those from span_start(i) / rows + i on, which
-// needs no sum over the spans before it (and leaves some numbers without rows).
+// needs no sum over the spans before it (and leaves some numbers without rows). The state after a segment has a slot in the workspace,
+// unless it is its sequence's last: of packed rows, that of its first row over `rows`, which the row of the next such segment, `rows` rows
+// on at least, can't share. So the workspace doesn't grow with the number of short sequences.
 struct Segments
 {
-    int64_t rows, count, each;
+    int64_t rows, count, each, slots;
 };
 
 inline Segments segments_of(const Sequences& s, int64_t rows)
 {
-    if (s.offsets) return Segments{rows, s.tokens / rows + s.count + 2, 0};
+    if (s.offsets) return Segments{rows, s.tokens / rows + s.count + 2, 0, s.tokens / rows};
     const int64_t each = s.tokens > 0 ? (s.tokens + rows - 1) / rows : 1;
-    return Segments{rows, s.count * each, each};
+    return Segments{rows, s.count * each, each, s.count * each};
 }
 
 struct Segment
@@ -103,6 +107,12 @@ struct Segment
     Rows1 q;
     int64_t first, n, number;  // rows [first, first + n) of the sequence, the number-th segment of it
 };
+
+// The slot of a sequence's first segment; the others' follow.
+__device__ __forceinline__ int64_t first_slot(const Sequences& s, const Segments& g, int64_t sequence, int64_t start)
+{
+    return s.offsets ? start / g.rows : sequence * g.each;
+}
 
 // Every lane of a wave calls it.
 __device__ __forceinline__ Segment segment_at(const Sequences& s, const Segments& g, int64_t at)
@@ -471,7 +481,7 @@ __global__ __launch_bounds__(L::THREADS, L::WAVES) void attention_walk_kernel(Se
         const int tile = (int)(item % tiles), head = (int)(item / tiles % heads);
         const int64_t at = item / tiles / heads;
         const Segment part = segment_at(seq, segments, at);
-        const int64_t n_all = part.n;
+        const int64_t n_all = part.n, slot = first_slot(seq, segments, part.q.batch, part.q.start) + part.number;
         const bool last = part.first + n_all >= part.q.length;
         const int col0 = tile * N, cols = p.cols;
         const int64_t row0 = seq.offsets ? part.q.start : part.q.batch * seq.tokens;
@@ -533,7 +543,7 @@ __global__ __launch_bounds__(L::THREADS, L::WAVES) void attention_walk_kernel(Se
         const int64_t state0 = (part.q.batch * heads + head) * p.dim * cols;
         if (!ONLY && part.number > 0)
         {
-            const float* __restrict__ begin = passes.states[blockIdx.y] + (((at - 1) * heads + head) * tiles + tile) * state_values<L>();
+            const float* __restrict__ begin = passes.states[blockIdx.y] + (((slot - 1) * heads + head) * tiles + tile) * state_values<L>();
 #pragma unroll
             for (int u = 0; u < KD; ++u)
 #pragma unroll
@@ -840,7 +850,7 @@ __global__ __launch_bounds__(L::THREADS, L::WAVES) void attention_walk_kernel(Se
 
         if (ONLY)
         {
-            float* __restrict__ end = passes.states[blockIdx.y] + ((at * heads + head) * tiles + tile) * state_values<L>();
+            float* __restrict__ end = passes.states[blockIdx.y] + ((slot * heads + head) * tiles + tile) * state_values<L>();
 #pragma unroll
             for (int u = 0; u < KD; ++u)
 #pragma unroll
@@ -877,19 +887,19 @@ __global__ __launch_bounds__(BLOCK) void attention_join_kernel(Sequences seq, Se
     {
         const int block = (int)(item % BLOCKS), tile = (int)(item / BLOCKS % tiles), head = (int)(item / BLOCKS / tiles % heads);
         const int64_t q = item / BLOCKS / tiles / heads;
-        int64_t length = seq.tokens, at = q * segments.each;
+        int64_t length = seq.tokens, start = 0;
         if (seq.offsets)
         {
-            const int64_t a = offset_at(seq, q), b = offset_at(seq, q + 1);
-            length = b > a ? b - a : 0;
+            const int64_t end = offset_at(seq, q + 1);
+            start = offset_at(seq, q);
+            length = end > start ? end - start : 0;
             if (length <= segments.rows) continue;
-            at = a / segments.rows + q + 1;
         }
         const int64_t count = (length + segments.rows - 1) / segments.rows - 1;  // all but the last
         const int e = block * BLOCK + threadIdx.x;
         if (e >= QUADS) continue;
         const int64_t stride = (int64_t)heads * tiles * QUADS;
-        f32x4* __restrict__ state = (f32x4*)passes.states[blockIdx.y] + ((at * heads + head) * tiles + tile) * QUADS + e;
+        f32x4* __restrict__ state = (f32x4*)passes.states[blockIdx.y] + ((first_slot(seq, segments, q, start) * heads + head) * tiles + tile) * QUADS + e;
         constexpr int AHEAD = 8;
         f32x4 own[AHEAD];
 #pragma unroll
@@ -940,7 +950,9 @@ struct Plan
 
 // The estimate, in half the time that two workgroups of 128 columns on a CU take for a chunk each: a chunk takes n workgroups of W waves
 // together 0.3 + 0.106 n W, a CU takes its workgroups in rounds of as many as it runs at once, and a workgroup's own cost (its first loads,
-// its state) is that of 2 + W / 2 chunks; where sequences are split, the first launch adds 0.4 of the second's time and the join 2.
+// its state) is that of 2 + W / 2 chunks; where sequences are split, the first launch adds 0.4 of the second's time and the join 2. The
+// lengths of packed sequences are not known here: their mean length, each rounded up to a chunk more, counts for the rounds, and one of 32
+// times the mean for what goes on behind them.
 template <typename L>
 Plan plan_of(const Sequences& seq, int heads, const Pass& p)
 {
@@ -948,12 +960,15 @@ Plan plan_of(const Sequences& seq, int heads, const Pass& p)
     auto chunk = [](int64_t workgroups) { return workgroups ? 0.3 + 0.106 * (double)workgroups * L::W : 0.0; };
     const int64_t walks = (seq.offsets ? 1 : seq.count) * (int64_t)heads * tiles_of<L>(p) * p.together;
     const int64_t chunks = seq.tokens > 0 ? (seq.tokens + L::C - 1) / L::C : 1;
+    const int64_t longest = !seq.offsets || seq.count <= 32 ? chunks : (32 * (chunks / seq.count + 1) < chunks ? 32 * (chunks / seq.count + 1) : chunks);
     int64_t best = chunks;
     double least = 1e300;
     auto consider = [&](int64_t size) {
         const int64_t parts = (chunks + size - 1) / size, items = walks * (seq.offsets ? parts + seq.count : parts);
         const int64_t each = (items + L::CUS - 1) / L::CUS, rounds = each / L::TOGETHER, rest = each % L::TOGETHER;
-        const double time = ((double)size + OWN) * ((double)rounds * chunk(L::TOGETHER) + chunk(rest));
+        const double most = (double)(size < longest ? size : longest);
+        const double mean = seq.offsets ? fmin(most, (double)(chunks + seq.count) / (double)(parts + seq.count)) : most;
+        const double time = (mean + OWN) * ((double)rounds * chunk(L::TOGETHER) + chunk(rest)) + (most - mean) * chunk(rounds > 0 ? L::TOGETHER : rest);
         const double cost = size >= chunks ? time : 1.4 * time + JOIN;
         if (cost < least) least = cost, best = size;
     };
@@ -1001,7 +1016,7 @@ template <typename L>
 size_t walk_states(const Sequences& seq, int heads, const Pass& p)
 {
     const Segments s = plan_of<L>(seq, heads, p).segments;
-    return joins(seq, s) ? align_up((size_t)(s.count * heads * tiles_of<L>(p) * state_values<L>()) * sizeof(float)) : 0;
+    return joins(seq, s) ? align_up((size_t)(s.slots * heads * tiles_of<L>(p) * state_values<L>()) * sizeof(float)) : 0;
 }
 
 template <typename T>

@@ -338,6 +338,25 @@ def test_attention_many_sequences():
     assert (gs - d * (last.double() + 0.5 * q.double().unsqueeze(-1) * go.double().unsqueeze(-2))).abs().max() < 1e-5
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_packed_segments(dtype):
+    """Sequences about a segment's length and several long, which are split and begin where others' segments end."""
+    lengths = [130, 1, 127, 128, 129, 700, 0, 63, 257, 256, 255, 3, 900, 64, 385]
+    heads, kvh, dim, dv = 2, 1, 32, 16
+    q, k, v, first, go, last = inputs(6, (sum(lengths),), heads, kvh, dim, dv, dtype, len(lengths))
+    g = decays(heads)
+    offsets = torch.tensor([0, *np.cumsum(lengths)], device=DEV)
+    names = ["out", "state", "gq", "gk", "gv", "gs"]
+    got = dict(zip(names, attend(q, k, v, first, go, last, g, 0.3, offsets)))
+    for i, n in enumerate(lengths):
+        rows = slice(int(offsets[i]), int(offsets[i + 1]))
+        if n:
+            check_sequence({x: got[x][i] if x in ("state", "gs") else got[x][rows] for x in names}, q[rows], k[rows], v[rows], g, 0.3, first[i], go[rows],
+                           last[i], f"sequence {i}")
+        else:
+            assert torch.equal(got["state"][i], first[i]) and torch.equal(got["gs"][i], last[i])
+
+
 def test_attention_strides():
     """Operands in any order of their dimensions, expanded, and behind 32-bit offsets."""
     q, k, v, first, go, last = inputs(3, (2, 70), 4, 4, 32, 32, torch.bfloat16, 2)

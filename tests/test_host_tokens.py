@@ -263,6 +263,17 @@ def test_abi_refuses_attention():
     refused(step(k=heads(3)), "multiple")
 
 
+def test_attention_workspace_does_not_grow_with_short_sequences():
+    lib = _native.lib()
+    for dtype in range(3):
+        for count, n in [(41, 12001), (10**4, 10**5), (10**6, 10**6), (64, 32768), (3, 10**7)]:
+            size = lib.mca_linear_attention_forward_workspace_size(dtype, sequences(count, n, P), 16, 128, 128)
+            # At most the state of every 64 tokens.
+            assert size <= 16 * 128 * 128 * 4 * (n // 64) + 256, (dtype, count, n)
+            if n <= 100 * count:
+                assert size == 0, (dtype, count, n)
+
+
 # ------------------------------------------------------------------------------------------------
 # The module
 # ------------------------------------------------------------------------------------------------

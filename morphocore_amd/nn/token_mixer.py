@@ -41,8 +41,8 @@ class TokenMixer(nn.Module):
         if channels < 1 or heads < 1 or kv_heads < 1 or heads % kv_heads:
             raise ValueError(f"TokenMixer needs channels and heads that are a multiple of kv_heads, got {channels}, {heads} and {kv_heads}")
         dim = channels // heads if dim is None else dim
-        if axes < 1 or dim // 2 < axes:
-            raise ValueError(f"TokenMixer needs a pair of a head's values for each axis, got {dim} values and {axes} axes")
+        if axes < 1 or axes > 8 or dim // 2 < axes or dim > 256:
+            raise ValueError(f"TokenMixer needs 1 to 8 axes, a pair of a head's values for each, and at most 256 values, got {axes} and {dim}")
         self.heads, self.kv_heads, self.dim, self.axes, self.channels_first = heads, kv_heads, dim, axes, channels_first
         self.norm = RMSNorm(channels, eps, dtype)
         self.query_weight = nn.Parameter(torch.ones(dim, dtype=dtype))

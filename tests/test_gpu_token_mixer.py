@@ -108,6 +108,65 @@ def test_packed_prompts_then_steps(dtype):
         assert (got.float() - w.float()).norm() <= 32 * u * w.float().norm(), f"sequence {i}"
 
 
+def test_inference_and_autocast():
+    """The same bits as otherwise, and a state of either kind written in place."""
+    m = mixer(32, 4, axes=2)
+    x = randn(1, 2, 3, 5, 32)
+    want = m(x, final_state=True)
+    at, state = torch.tensor([[3, 0], [1, 2]], device=DEV), want[2].detach().clone()
+    token = m.step(x[:, 0, 0], state, at)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        got = m(x, final_state=True)
+        other = want[2].detach().clone()
+        assert torch.equal(m.step(x[:, 0, 0], other, at)[0], token[0]) and torch.equal(other, state)
+    assert all(torch.equal(a, b) and a.dtype == b.dtype for a, b in zip(got, want))
+    with torch.inference_mode():
+        got = m(x, final_state=True)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        for other in (want[2].detach().clone(), got[2]):
+            assert torch.equal(m.step(x[:, 0, 0], other, at)[0], token[0]) and torch.equal(other, state)
+
+
+@pytest.mark.parametrize("shape", [(0, 3, 5), (2, 0, 5), (2, 1, 1)])
+def test_no_tokens(shape):
+    m = mixer(32, 4, axes=2)
+    x, s = randn(1, *shape, 32).requires_grad_(), randn(2, shape[0], 4, 8, 8)
+    out, h, last = m(x, state=s, final_state=True)
+    assert out.shape == h.shape == x.shape and last.shape == s.shape
+    if x.numel() == 0:
+        assert torch.equal(last, s)
+    grads = torch.autograd.grad([out, last], [x, *m.parameters()], [torch.ones_like(out), torch.ones_like(last)], allow_unused=True)
+    assert all(g is None or torch.isfinite(g).all() for g in grads)
+
+
+def test_captured_training_step():
+    """A step's forward and backward in a graph, each replay as the eager step."""
+    m = mixer(32, 4, axes=2)
+    x, go = randn(1, 2, 6, 7, 32).requires_grad_(), randn(2, 2, 6, 7, 32)
+
+    def step():
+        out, h = m(x)
+        return [out, *torch.autograd.grad(out, [x, *m.parameters()], go)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for i in range(3):
+        with torch.no_grad():
+            x.copy_(randn(10 + i, 2, 6, 7, 32))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b) or (a - b).norm() <= 1e-6 * b.norm(), f"replay {i}"
+
+
 def test_captured_step():
     m = mixer(32, 4)
     x, cache, at = randn(1, 3, 32), randn(2, 3, 4, 8, 8), torch.tensor([[3], [0], [900]], device=DEV)

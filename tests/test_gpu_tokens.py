@@ -338,6 +338,19 @@ def test_attention_many_sequences():
     assert (gs - d * (last.double() + 0.5 * q.double().unsqueeze(-1) * go.double().unsqueeze(-2))).abs().max() < 1e-5
 
 
+def test_attention_more_sequences_than_workgroups():
+    """Sequences of one token, which a workgroup takes one after another, a value that is not finite among them."""
+    n = 600000
+    q, k, v, *_ = inputs(4, (n,), 2, 1, 3, 2, torch.float32, 0)
+    q, k, v = q.detach(), k.detach(), v.detach().clone()
+    v[123456, 0, 1] = float("inf")
+    out = F.linear_attention(q, k, v, decays(2), offsets=torch.arange(n + 1, device=DEV), scale=0.5)
+    want = 0.5 * (q.double() * k.double()).sum(-1, keepdim=True) * v.double()
+    bad = torch.zeros_like(out, dtype=torch.bool)
+    bad[123456, :, 1] = True
+    assert torch.equal(out.isnan(), bad) and ((out - want)[~bad].abs() <= 2.0**-18 * (q.abs() * k.abs()).sum(-1, keepdim=True).mul(v.abs())[~bad]).all()
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_attention_packed_segments(dtype):
     """Sequences about a segment's length and several long, which are split and begin where others' segments end."""
@@ -486,6 +499,17 @@ def test_step_with_the_same_place_twice(batch):
         rows = (slots == s).nonzero()[:, 0]
         check_sequence(dict(out=out[rows], state=state[s]), q[rows], k[rows], v[rows], g, dim**-0.5, before[s], None, None, f"{s}")
     assert not out[slots < 0].any()
+
+
+def test_step_of_more_states_than_workgroups():
+    batch, heads = 70000, 16
+    q, k, v = randn(1, batch, heads, 2), randn(2, batch, heads, 2), randn(3, batch, heads, 1)
+    state = randn(4, batch, heads, 2, 1)
+    want = k.unsqueeze(-1) * v.unsqueeze(-2) + state  # one rounding apart: what is not lost is added as it is
+    out = F.linear_attention_step(q, k, v, torch.zeros(heads, device=DEV), state, scale=1.0)
+    size = k.abs().unsqueeze(-1) * v.abs().unsqueeze(-2) + 2 * want.abs()
+    assert ((state - want).abs() <= 2.0**-22 * size).all()
+    assert ((out.double() - (q.double().unsqueeze(-1) * state.double()).sum(-2)).abs() <= 2.0**-20 * (q.abs().unsqueeze(-1) * state.abs()).sum(-2)).all()
 
 
 def test_step_strides_and_versions():

@@ -292,6 +292,7 @@ def test_token_mixer():
     assert torch.allclose(-1 / decay, torch.tensor([16.0, 16.0 * 2**(8 / 3), 16.0 * 2**(16 / 3), 4096.0]))
     assert mca.nn.TokenMixer(8, 1).log_decay.tolist() == [-1 / 16] and mca.nn.TokenMixer(8, 2, dim=7).frequencies.shape == (1, 3)
     for bad in (lambda: mca.nn.TokenMixer(0, 1), lambda: mca.nn.TokenMixer(8, 0), lambda: mca.nn.TokenMixer(8, 4, kv_heads=3),
-                lambda: mca.nn.TokenMixer(8, 4, axes=2), lambda: mca.nn.TokenMixer(8, 1, axes=0), lambda: mca.nn.TokenMixer(8, 2, kv_heads=0)):
+                lambda: mca.nn.TokenMixer(8, 4, axes=2), lambda: mca.nn.TokenMixer(8, 1, axes=0), lambda: mca.nn.TokenMixer(8, 2, kv_heads=0),
+                lambda: mca.nn.TokenMixer(257, 1), lambda: mca.nn.TokenMixer(64, 1, axes=9)):
         with pytest.raises(ValueError):
             bad()

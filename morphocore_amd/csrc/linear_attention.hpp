@@ -596,8 +596,10 @@ __global__ __launch_bounds__(L::THREADS, L::WAVES) void attention_walk_kernel(Se
             const int n = i0 + 1 < chunks ? C : rest;
             ++chunk;
             // The lane's places in LDS follow from this copy anew in every chunk: kept from chunk to chunk they would fill the registers.
-            const int l = thread_now<true>() % WAVE, g = l / 16, row_d = row_place<UD>(l), row_c = row_place<UC>(l), column_d = column_place<UD>(l, l & 3);
-            const int column_n = column_place<UN>(l, 2 * wave + ((l >> 1) & 1)) + 8 * (l & 1), score_c = unit_byte<UC>(l % 16, g >> 1) + 8 * (g & 1);
+            // Where registers are few, in each of its parts.
+            const int lane = thread_now<true>() % WAVE;
+            auto lane_now = [&] { return SPARE ? thread_now<true>() % WAVE : lane; };
+            auto column_n_of = [&](int l) { return column_place<UN>(l, 2 * wave + ((l >> 1) & 1)) + 8 * (l & 1); };
             __syncthreads();
             if constexpr (!ONLY) stage.a.store(ta, wide, 0, p.dim);
             stage.b.store(tb, wide, 0, p.dim);
@@ -620,6 +622,7 @@ __global__ __launch_bounds__(L::THREADS, L::WAVES) void attention_walk_kernel(Se
             if constexpr (!ONLY)
             {
                 // Scores, decayed, in terms to LDS: tiles of 16 x 16 on and below the diagonal, by the waves in turn.
+                const int l = lane_now(), g = l / 16, row_d = row_place<UD>(l), score_c = unit_byte<UC>(l % 16, g >> 1) + 8 * (g & 1);
 #pragma unroll
                 for (int t0 = 0; t0 < RT * (RT + 1) / 2; t0 += L::W)
                 {
@@ -665,7 +668,11 @@ __global__ __launch_bounds__(L::THREADS, L::WAVES) void attention_walk_kernel(Se
                         *(bf16x4*)(tp + i * L::P + rt * (256 * UC) + (score_c ^ (32 * ct))) = term_vector<bf16x4>(term, i);
                     __builtin_amdgcn_sched_barrier(0);
                 }
+            }
+            if constexpr (!ONLY)
+            {
                 // a S, with the state's terms as they lie in the lanes.
+                const int l = lane_now(), row_d = row_place<UD>(l);
 #pragma unroll
                 for (int u = 0; u < KD; ++u)
                 {
@@ -704,6 +711,7 @@ __global__ __launch_bounds__(L::THREADS, L::WAVES) void attention_walk_kernel(Se
             if constexpr (!ONLY)
             {
                 // Scores times c, and out.
+                const int l = lane_now(), g = l / 16, row_c = row_place<UC>(l), column_n = column_n_of(l);
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks)
                 {
@@ -804,6 +812,7 @@ __global__ __launch_bounds__(L::THREADS, L::WAVES) void attention_walk_kernel(Se
             __builtin_amdgcn_sched_barrier(0);
 
             // The state after the chunk.
+            const int l = lane_now(), g = l / 16, column_d = column_place<UD>(l, l & 3), column_n = column_n_of(l);
             const bool whole = n == C;
             const Decay decay = kept[i0 + 1 < chunks ? 0 : 1][wave];
 #pragma unroll

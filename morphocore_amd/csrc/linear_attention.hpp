@@ -605,7 +605,7 @@ __global__ __launch_bounds__(L::THREADS, L::WAVES) void attention_walk_kernel(Se
             stage.b.store(tb, wide, 0, p.dim);
             stage.c.store(tc, wide, col0, cols - col0);
             if ((int)stage.b.spoiled() | (int)stage.c.spoiled()) spoiled.any = chunk;
-            if (!L::LATE && i0 + 1 < chunks) load(stage, i0 + 1);
+            if ((ONLY || !L::LATE) && i0 + 1 < chunks) load(stage, i0 + 1);
             __syncthreads();
             const bool spoils = spoiled.any == chunk;
             if (spoils)
@@ -807,9 +807,6 @@ __global__ __launch_bounds__(L::THREADS, L::WAVES) void attention_walk_kernel(Se
                 out0 += C * out_step;
                 __builtin_amdgcn_sched_barrier(0);
             }
-
-            if (ONLY && L::LATE && i0 + 1 < chunks) load(stage, i0 + 1);
-            __builtin_amdgcn_sched_barrier(0);
 
             // The state after the chunk.
             const int l = lane_now(), g = l / 16, column_d = column_place<UD>(l, l & 3), column_n = column_n_of(l);

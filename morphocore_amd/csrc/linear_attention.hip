@@ -31,13 +31,13 @@ hipError_t sum_shared_heads(const float* part, T* out, int64_t rows, int heads, 
 // Bound by HBM: the states are read once and written once, float32. A workgroup has 4 LC columns of one head's state in registers, 4
 // neighbouring values a thread in every RB-th row, all loads in flight at once; q S is summed over a thread's rows, the lanes and
 // the waves, in a fixed order. Rows of the batch that name the same slot are taken by the first of them, in order, the state staying
-// where it is. Measured, 32 heads of 128 x 128 in bfloat16: 256 sequences in 272 us (3.95 TB/s of states read and written in place, where a
-// copy reaches 5.05), one in 5.6 (7.5 with its call).
+// where it is. Measured, 32 heads of 128 x 128 in bfloat16: 256 sequences in 231 us (4.65 TB/s of states read and written in place, where a
+// copy reaches 5.05; stores past the caches are no faster), one in 5.6 (7.5 with its call).
 template <typename T, int LC, int R>
-__global__ __launch_bounds__(BLOCK, R <= 16 ? 4 : 2) void attention_step_kernel(TokenRows q, TokenRows k, TokenRows v, const float* __restrict__ log_decay,
+__global__ __launch_bounds__(BLOCK, 4) void attention_step_kernel(TokenRows q, TokenRows k, TokenRows v, const float* __restrict__ log_decay,
                                                                float* __restrict__ states, int64_t slot_stride, int64_t head_stride,
                                                                const void* __restrict__ slot_of, bool wide, int64_t slots, T* __restrict__ out,
-                                                               int64_t batch, int heads, int dim, int cols, float scale, int tiles, bool streaming)
+                                                               int64_t batch, int heads, int dim, int cols, float scale, int tiles)
 {
     constexpr int RB = BLOCK / LC;
     static_assert(LC <= WAVE);
@@ -143,13 +143,7 @@ __global__ __launch_bounds__(BLOCK, R <= 16 ? 4 : 2) void attention_step_kernel(
             if (row >= dim) continue;
             float* __restrict__ to = state + (int64_t)row * cols;
             if (valid == 4)
-            {
-                typedef f32x4 unaligned __attribute__((aligned(4)));
-                if (streaming)
-                    __builtin_nontemporal_store(s[i], (unaligned*)to);
-                else
-                    *(unaligned*)to = s[i];
-            }
+                __builtin_memcpy(to, &s[i], 16);
             else
 #pragma unroll
                 for (int j = 0; j < 3; ++j)
@@ -164,13 +158,12 @@ hipError_t linear_attention_step(TokenRows q, TokenRows k, TokenRows v, const fl
                                  int cols, float scale, hipStream_t stream)
 {
     if (batch <= 0 || heads <= 0) return hipSuccess;
-    const bool streaming = streams(8.0 * (double)batch * heads * dim * cols);
     auto run = [&](auto lc, auto r) {
         constexpr int LC = decltype(lc)::value, R = decltype(r)::value;
         const int tiles = (cols + 4 * LC - 1) / (4 * LC);
         const int64_t work = batch * heads * tiles, most = 1 << 20;
         attention_step_kernel<T, LC, R><<<(unsigned)(work < most ? work : most), BLOCK, 0, stream>>>(
-            q, k, v, log_decay, states, slot_stride, head_stride, slot_of, wide, slots, out, batch, heads, dim, cols, scale, tiles, streaming);
+            q, k, v, log_decay, states, slot_stride, head_stride, slot_of, wide, slots, out, batch, heads, dim, cols, scale, tiles);
         return hipGetLastError();
     };
     using std::integral_constant;
@@ -184,8 +177,8 @@ hipError_t linear_attention_step(TokenRows q, TokenRows k, TokenRows v, const fl
         if (dim <= RB * (MOST / 2)) return run(lc, integral_constant<int, MOST / 2>());
         return run(lc, integral_constant<int, MOST>());
     };
-    // Whole rows of the state at once, up to 512 bytes, where there are workgroups enough; parts of 128 bytes otherwise.
-    if (cols > 64 && batch * heads >= 512) return by_rows(integral_constant<int, 32>());
+    // Parts of 256 bytes of the state's rows where there are workgroups enough (256 states of 32 heads of 128 x 128 in 230 us, by whole rows of
+    // 512 bytes in 272); of 128 bytes otherwise.
     if (cols > 32 && batch * heads >= 256) return by_rows(integral_constant<int, 16>());
     if (cols > 16) return by_rows(integral_constant<int, 8>());
     return by_rows(integral_constant<int, 4>());

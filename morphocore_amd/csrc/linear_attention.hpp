@@ -408,11 +408,12 @@ struct TileLoad
         return any;
     }
 
-    __device__ __forceinline__ void store(char* tile, bool whole, int c0, int left)
+    // full: no unit is partial.
+    __device__ __forceinline__ void store(char* tile, bool full, int c0, int left)
     {
         constexpr int BYTES = L::C * COLS * 2;
         const int thread = thread_now<SPARE>();
-        if (!whole)
+        if (!full)
         {
             const int n = down(thread, c0, left);
 #pragma unroll
@@ -538,7 +539,7 @@ __global__ __launch_bounds__(L::THREADS, L::WAVES) void attention_walk_kernel(Se
         pa = ONLY ? nullptr : TileLoad<T, L, DK, SPARE>::begin(pa, sa, 0, p.dim);
         pb = TileLoad<T, L, DK, SPARE>::begin(pb, sb, 0, p.dim);
         pc = TileLoad<T, L, N, SPARE>::begin(pc + col0, sc, col0, cols - col0);
-        const bool wide = p.dim == DK && col0 + N <= cols;
+        const bool wide = p.dim == DK && col0 + N <= cols, full = p.dim % UNIT == 0, full_c = col0 + N <= cols || (cols - col0) % UNIT == 0;
         struct Stage
         {
             TileLoad<T, L, DK, SPARE> a, b;
@@ -601,9 +602,9 @@ __global__ __launch_bounds__(L::THREADS, L::WAVES) void attention_walk_kernel(Se
             auto lane_now = [&] { return SPARE ? thread_now<true>() % WAVE : lane; };
             auto column_n_of = [&](int l) { return column_place<UN>(l, 2 * wave + ((l >> 1) & 1)) + 8 * (l & 1); };
             __syncthreads();
-            if constexpr (!ONLY) stage.a.store(ta, wide, 0, p.dim);
-            stage.b.store(tb, wide, 0, p.dim);
-            stage.c.store(tc, wide, col0, cols - col0);
+            if constexpr (!ONLY) stage.a.store(ta, full, 0, p.dim);
+            stage.b.store(tb, full, 0, p.dim);
+            stage.c.store(tc, full_c, col0, cols - col0);
             if ((int)stage.b.spoiled() | (int)stage.c.spoiled()) spoiled.any = chunk;
             if ((ONLY || !L::LATE) && i0 + 1 < chunks) load(stage, i0 + 1);
             __syncthreads();

@@ -62,6 +62,14 @@ class TokenMixer(nn.Module):
             setattr(self, name, moved if moved.dtype == value.dtype else value.to(moved.device))
         return self
 
+    def _normed(self, x: torch.Tensor, residual: Optional[torch.Tensor]):
+        """The norm, its 8-bit form where a backward may read it, and the sum with the residual."""
+        if torch.is_grad_enabled():
+            y, packed, h = rms_norm8(x, self.norm.weight, residual, self.norm.eps)
+            return y, packed, x if h is None else h
+        y = rms_norm(x, self.norm.weight, residual, self.norm.eps)
+        return (y, None, x) if residual is None else (y[0], None, y[1])
+
     def _rotated(self, y: torch.Tensor, packed, positions: torch.Tensor):
         qkv = linear8(y, self.project, packed).unflatten(-1, (self.heads + 2 * self.kv_heads, self.dim))
         q, k, v = qkv.split((self.heads, self.kv_heads, self.kv_heads), -2)
@@ -77,8 +85,7 @@ class TokenMixer(nn.Module):
             x = x.movedim(1, -1)
             residual = residual.movedim(1, -1) if residual is not None else None
         places = x.shape[1:-1]
-        y, packed, h = rms_norm8(x, self.norm.weight, residual, self.norm.eps)
-        h = x if h is None else h
+        y, packed, h = self._normed(x, residual)
         if positions is None:
             positions = grid_positions(places, x.device)
         if offsets is None:  # places of all axes become one dimension
@@ -97,7 +104,7 @@ class TokenMixer(nn.Module):
     def step(self, x: torch.Tensor, state: torch.Tensor, positions: torch.Tensor, residual: torch.Tensor = None, slots: torch.Tensor = None):
         if x.dim() != 2:
             raise ValueError(f"TokenMixer.step expects [batch, channels], got {list(x.shape)}")
-        y, h = rms_norm(x, self.norm.weight, residual, self.norm.eps) if residual is not None else (rms_norm(x, self.norm.weight, None, self.norm.eps), x)
+        y, _, h = self._normed(x, residual)
         q, k, v = self._rotated(y, None, positions)
         out = linear_attention_step(q, k, v, self.log_decay, state, slots)
         return linear8(out.flatten(-2), self.contract), h

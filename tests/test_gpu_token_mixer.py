@@ -120,6 +120,10 @@ def test_inference_and_autocast():
         other = want[2].detach().clone()
         assert torch.equal(m.step(x[:, 0, 0], other, at)[0], token[0]) and torch.equal(other, state)
     assert all(torch.equal(a, b) and a.dtype == b.dtype for a, b in zip(got, want))
+    r = randn(2, 2, 3, 5, 32)
+    with torch.no_grad():
+        got = m(x, final_state=True), m(x, r)
+    assert all(torch.equal(a, b) for a, b in zip((*got[0], *got[1]), (*want, *m(x, r))))
     with torch.inference_mode():
         got = m(x, final_state=True)
         assert all(torch.equal(a, b) for a, b in zip(got, want))
@@ -146,7 +150,7 @@ def test_captured_training_step():
 
     def step():
         out, h = m(x)
-        return [out, *torch.autograd.grad(out, [x, *m.parameters()], go)]
+        return [out.detach(), *torch.autograd.grad(out, [x, *m.parameters()], go)]
 
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())

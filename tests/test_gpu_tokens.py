@@ -636,6 +636,29 @@ def test_captured_steps():
         assert torch.equal(out[0], serve(other)[0]) and torch.equal(cache, other), f"replay {i}"
 
 
+def test_captured_packed_sequences():
+    """Offsets are read on the device: a replay takes those that are there then."""
+    heads, kvh, dim, dv, n = 2, 1, 32, 16, 1500
+    q, k, v, first, go, last = inputs(9, (n,), heads, kvh, dim, dv, torch.bfloat16, 4)
+    g = decays(heads)
+    cuts = [[0, 0, 700, 1300, 1500], [3, 900, 900, 1100, 1499], [0, 1500, 1500, 1500, 1500], [500, 501, 502, 503, 504]]
+    offsets = torch.tensor(cuts[0], device=DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        attend(q, k, v, first, go, last, g, 0.3, offsets)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = attend(q, k, v, first, go, last, g, 0.3, offsets)
+    for cut in cuts[1:] + cuts:
+        offsets.copy_(torch.tensor(cut))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, attend(q, k, v, first, go, last, g, 0.3, offsets))), cut
+
+
 def test_on_another_stream():
     t = inputs(8, (2, 700), 4, 2, 64, 64, torch.bfloat16, 2)
     g = decays(4)

@@ -87,7 +87,8 @@ int mca_linear_attention_backward(int dtype, const mca_sequences* sequences, con
                                   void* workspace, size_t workspace_bytes, void* stream);
 
 /* One token for each of `batch` sequences. Sequence b's state, [heads, dim, value_dim] at states + slot * slot_stride (heads head_stride
- * apart, dense within), is updated in place; its slot is slot_of[b], of 32 or (wide) 64 bits, or b without slot_of. A slot outside
+ * apart, dense within), is updated in place; its slot is slot_of[b], of 32 or (wide) 64 bits, or b without slot_of. States of different
+ * slots and heads must not share memory: one of the two strides reaches over all that the other one spans. A slot outside
  * [0, slots) stands for no sequence: its row of out is zero. Rows that name the same slot are taken one after another. The
  * rows' token_stride is read, their batch_stride is not. */
 int mca_linear_attention_step(int dtype, const mca_heads* q, const mca_heads* k, const mca_heads* v, const float* log_decay, float* states,

@@ -16,7 +16,7 @@
 // of c, which are float32, are split into three, so that nothing is rounded to fewer bits before the result. (With two terms for scores and
 // states, 2^-16 of each, one bfloat16 result in a hundred was its neighbour, 1.0e-4 of the results by norm instead of 4.3e-5; 32768 tokens of 32
 // heads took 480 us instead of 515, 4 x 4096 of 16 with their gradients 500 instead of 550.) Products of terms whose places add up to more than
-// 2 are left out: 2^-23 of the magnitudes at most.
+// 2 are left out: below 2^-22 of the magnitudes at the very most.
 //
 // Layouts. Of a 16 x 16 x 32 product lane l gives the first operand's row l % 16 and the second's column l % 16 with 8 values
 // of the summed axis from 8 (l / 16) on, and gets column l % 16, rows 4 (l / 16) to + 3. The transposing LDS read takes a row's 4-value

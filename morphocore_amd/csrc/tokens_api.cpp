@@ -126,6 +126,14 @@ mca::TokenRows token_rows(const mca_heads* x, int64_t heads)
     return mca::TokenRows{x->data, x->batch_stride, x->token_stride, x->head_stride, x->heads > 0 ? (int)(heads / x->heads) : 1};
 }
 
+// Whether no two of slots x heads states of `extent` values share memory: neither stride is less than a state, and one of them reaches over
+// all that the other one spans.
+bool apart(int64_t slots, int64_t slot_stride, int64_t heads, int64_t head_stride, int64_t extent)
+{
+    if ((slots > 1 && slot_stride < extent) || (heads > 1 && head_stride < extent)) return false;
+    return slots <= 1 || heads <= 1 || (slot_stride - extent) / head_stride >= heads - 1 || (head_stride - extent) / slot_stride >= slots - 1;
+}
+
 // A state as it lies, and transposed.
 mca::States states_of(const float* p, int64_t value_dim) { return mca::States{(float*)p, value_dim, 1}; }
 mca::States transposed(const float* p, int64_t value_dim) { return mca::States{(float*)p, 1, value_dim}; }
@@ -369,6 +377,7 @@ int mca_linear_attention_step(int dtype, const mca_heads* q, const mca_heads* k,
         return rc;
     if (k->heads != v->heads) return mca::api_fail("Keys and values must have the same heads");
     if (slots < 0 || slot_stride < 0 || head_stride < dim * value_dim) return mca::api_fail("slots and slot_stride must be non negative, head_stride at least dim * value_dim");
+    if (!apart(slots, slot_stride, q->heads, head_stride, dim * value_dim)) return mca::api_fail("States must not share memory");
     if (!slot_of && slots < batch) return mca::api_fail("Without slot_of there must be a slot for every sequence");
     if (batch > 0 && q->heads > 0 && (!log_decay || !out || (slots > 0 && !states))) return mca::api_fail("log_decay, states and out must not be null");
     return by_type(dtype, [&](auto* t) {

@@ -7,8 +7,6 @@
 // an error, never a fallback.
 #include "ops.hpp"
 
-#include <ATen/MemoryOverlap.h>
-
 #include "../../include/morphocore_amd_tokens.h"
 
 namespace
@@ -385,12 +383,14 @@ Tensor linear_attention_step(const Tensor& query, const Tensor& key, const Tenso
     }
     else
         TORCH_CHECK(state.size(0) == batch, name, ": without slots state must have ", batch, " entries, got ", state.size(0));
-    // It is written in place: no copy may stand in for it, and no two entries may share memory.
+    // It is written in place, by workgroups that don't wait for each other: no copy may stand in for it, and no two of its entries may share memory.
+    // One of the strides of slots and heads reaches over all that the other one spans.
     const bool dense = (value_dim == 1 || state.stride(3) == 1) && (dim == 1 || state.stride(2) == value_dim);
-    const int64_t head_stride = heads > 1 ? state.stride(1) : dim * value_dim, slot_stride = state.size(0) > 1 ? state.stride(0) : 0;
-    TORCH_CHECK(dense && head_stride >= dim * value_dim && (state.size(0) <= 1 || slot_stride >= dim * value_dim) &&
-                    at::has_internal_overlap(state) != at::MemOverlap::Yes,
-                name, ": a head's state must be dense, got strides ", state.strides());
+    const int64_t places = state.size(0), extent = dim * value_dim;
+    const int64_t head_stride = heads > 1 ? state.stride(1) : extent, slot_stride = places > 1 ? state.stride(0) : 0;
+    TORCH_CHECK(dense && head_stride >= extent && (places <= 1 || slot_stride >= extent) &&
+                    (places <= 1 || heads <= 1 || slot_stride >= (heads - 1) * head_stride + extent || head_stride >= (places - 1) * slot_stride + extent),
+                name, ": a head's state must be dense and share no memory with another, got strides ", state.strides());
     check_device(name, query, {key, value, log_decay, state});
     if (at.defined()) check_device(name, query, {at});
     const c10::DeviceGuard guard(query.device());

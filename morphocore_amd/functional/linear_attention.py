@@ -33,7 +33,7 @@ def linear_attention_step(query: torch.Tensor, key: torch.Tensor, value: torch.T
     [batch, heads, value_dim]. Not differentiable.
 
     query, key, value : [batch, heads, dim], [batch, kv_heads, dim], [batch, kv_heads, value_dim].
-    state : [slots, heads, dim, value_dim] float32, each head's dense.
+    state : [slots, heads, dim, value_dim] float32, each head's dense; no two of them may share memory.
     slots : [batch] int32 or int64, the sequences' places in ``state``; without it they are the batch's. A place outside it stands for
         no sequence (a padded batch) and gets zeros. Tokens that name the same place are taken one after another.
     """

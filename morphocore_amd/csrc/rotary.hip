@@ -96,26 +96,25 @@ __device__ __forceinline__ void sine_cosine(const Rotation& r, int64_t token, in
     if (inverse) sine = -sine;
 }
 
-__device__ __forceinline__ void turn_pair(float& a, float& b, float c, float s)
+// `there`: values behind the pairs are chosen, not turned by 0, which would spread an infinity among them.
+__device__ __forceinline__ void turn_pair(float& a, float& b, float c, float s, bool there)
 {
-    const float x = a * c - b * s;
-    b = b * c + a * s;
-    a = x;
+    const float x = a * c - b * s, y = b * c + a * s;
+    a = there ? x : a;
+    b = there ? y : b;
 }
 
 // Of a unit's pairs those that are there.
 template <bool INTERLEAVED>
 __device__ __forceinline__ void rotate(float (&v)[2][UNIT], const Turn& t, int pairs)
 {
-    if constexpr (INTERLEAVED)
-    {
 #pragma unroll
-        for (int e = 0; e < UNIT; ++e) turn_pair(v[e / 4][2 * e % UNIT], v[e / 4][2 * e % UNIT + 1], e < pairs ? t.cos[e] : 1.0f, e < pairs ? t.sin[e] : 0.0f);
-    }
-    else
+    for (int e = 0; e < UNIT; ++e)
     {
-#pragma unroll
-        for (int e = 0; e < UNIT; ++e) turn_pair(v[0][e], v[1][e], e < pairs ? t.cos[e] : 1.0f, e < pairs ? t.sin[e] : 0.0f);
+        if constexpr (INTERLEAVED)
+            turn_pair(v[e / 4][2 * e % UNIT], v[e / 4][2 * e % UNIT + 1], t.cos[e], t.sin[e], e < pairs);
+        else
+            turn_pair(v[0][e], v[1][e], t.cos[e], t.sin[e], e < pairs);
     }
 }
 

@@ -7,6 +7,8 @@
 // an error, never a fallback.
 #include "ops.hpp"
 
+#include <c10/core/InferenceMode.h>
+
 #include "../../include/morphocore_amd_tokens.h"
 
 namespace
@@ -391,6 +393,7 @@ Tensor linear_attention_step(const Tensor& query, const Tensor& key, const Tenso
     TORCH_CHECK(dense && head_stride >= extent && (places <= 1 || slot_stride >= extent) &&
                     (places <= 1 || heads <= 1 || slot_stride >= (heads - 1) * head_stride + extent || head_stride >= (places - 1) * slot_stride + extent),
                 name, ": a head's state must be dense and share no memory with another, got strides ", state.strides());
+    TORCH_CHECK(!state.is_inference() || c10::InferenceMode::is_enabled(), name, ": state is an inference tensor, which is written to in inference mode alone");
     check_device(name, query, {key, value, log_decay, state});
     if (at.defined()) check_device(name, query, {at});
     const c10::DeviceGuard guard(query.device());

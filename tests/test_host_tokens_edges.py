@@ -48,3 +48,13 @@ def test_abi_step_refuses_states_that_share_memory():
     for slot, head in SHARED + [(2**40, 2**40), (2**62, 2**62), (2**62, 2**61)]:
         rc, message = call(slot, head)
         assert rc == 1 and ("share memory" in message or "head_stride" in message), (slot, head, message)
+
+
+def test_step_refuses_an_inference_tensor_outside_of_inference_mode():
+    """Before anything is launched: the state would be updated, and the result lost in the error."""
+    with torch.inference_mode():
+        state = torch.zeros(3, 4, 8, 6)
+        with pytest.raises(RuntimeError, match="runs on AMD GPUs"):
+            step(state)
+    with pytest.raises(RuntimeError, match="inference tensor"):
+        step(state)

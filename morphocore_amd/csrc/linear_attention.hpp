@@ -365,7 +365,13 @@ struct TileLoad
         {
 #pragma unroll
             for (int i = 0; i < COUNT; ++i, at += STEP * stride)
-                if (UNITS % L::THREADS == 0 || thread_now<SPARE>() < UNITS) __builtin_memcpy(raw[i].d, at, sizeof(raw[i].d));
+            {
+                if (UNITS % L::THREADS == 0 || thread_now<SPARE>() < UNITS)
+                    __builtin_memcpy(raw[i].d, at, sizeof(raw[i].d));
+                else  // a thread without a unit, which spoiled() asks too
+#pragma unroll
+                    for (int k = 0; k < RawUnit<T>::DWORDS; ++k) raw[i].d[k] = 0;
+            }
         }
         else
         {

@@ -1017,14 +1017,17 @@ Plan plan_of(const Sequences& seq, int heads, const Pass& p)
         const double cost = size >= chunks ? time : 1.4 * time + JOIN;
         if (cost < least) least = cost, best = size;
     };
-    for (int64_t size = chunks; size > 16; size = size - size / 8) consider(size);
-    for (int64_t size = chunks < 16 ? chunks : 16; size >= 2; --size) consider(size);
+    consider(chunks);
+    for (int64_t size = chunks - chunks / 8; size > 16; size = size - size / 8) consider(size);
+    for (int64_t size = chunks <= 16 ? chunks - 1 : 16; size >= 2; --size) consider(size);
     return Plan{segments_of(seq, best * L::C), least};
 }
 
 // f(the shape of a pass): as few columns a workgroup as hold the pass's. Of more than 64, 128 where two such workgroups don't fit a CU (the
-// scores would be formed twice: 84 us instead of 57, forwards, for 4999 tokens of 6 heads of 96 x 77 in float16), otherwise 128 or 64 by the
-// estimate: 32768 tokens of 32 heads of 128 x 128 in bfloat16 take 492 us by 128 and 568 by 64; 12001 of 41 sequences take 200 and 166.
+// scores would be formed twice: 84 us instead of 57, forwards, for 4999 tokens of 6 heads of 96 x 77 in float16) and for sequences of one chunk, whose
+// scores are most of the work (500 of 33 tokens of 8 heads of 64 x 128 in bfloat16: 84 us by 128, 125 by 64; 2000 of 60 of 16 heads of 128 x 128: 1100
+// and 1190), otherwise 128 or 64 by the estimate: 32768 tokens of 32 heads of 128 x 128 in bfloat16 take 492 us by 128 and 568 by 64; 12001 of 41
+// sequences take 200 and 166.
 template <typename T, typename F>
 hipError_t by_walk(const Sequences& seq, int heads, const Pass& p, F&& f)
 {
@@ -1033,7 +1036,9 @@ hipError_t by_walk(const Sequences& seq, int heads, const Pass& p, F&& f)
     do                                                                                                                           \
     {                                                                                                                            \
         if (p.cols <= 64) MCA_WALK(DK, 4);                                                                                       \
-        if (Walk<T, DK, 8>::LATE && plan_of<Walk<T, DK, 4>>(seq, heads, p).cost < plan_of<Walk<T, DK, 8>>(seq, heads, p).cost) MCA_WALK(DK, 4); \
+        if (Walk<T, DK, 8>::LATE && seq.tokens > Walk<T, DK, 8>::C &&                                                            \
+            plan_of<Walk<T, DK, 4>>(seq, heads, p).cost < plan_of<Walk<T, DK, 8>>(seq, heads, p).cost)                           \
+            MCA_WALK(DK, 4);                                                                                                     \
         MCA_WALK(DK, 8);                                                                                                         \
     } while (0)
     if (p.dim <= 64 && p.cols <= 32)

@@ -6,6 +6,8 @@ import subprocess
 
 import pytest
 
+from tests import walk_cases
+
 HERE = os.path.dirname(os.path.abspath(__file__))
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
@@ -40,3 +42,18 @@ def test_sequences_of_one_chunk_form_their_scores_once(plans):
     rows = [(t, packed, 9, n, 8, d, c, 1) for t in range(3) for packed in (0, 1) for n in (1, 32) for d in (32, 64, 128, 256) for c in (65, 128, 200)]
     assert all(p[1] == 8 for p in plans(rows))
     assert all(p[1] == 4 for p in plans([(t, 0, 9, 32, 8, 64, 64, 1) for t in range(3)]))
+
+
+def test_the_cases_reach_every_walk(plans):
+    """tests/walk_cases.py, which the GPU's tests run: every shape of every type, split and not; those that two workgroups a CU take
+    forwards and backwards."""
+    reached = {}
+    for c in walk_cases.CASES:
+        for kind in c["types"]:
+            for part, (dk, w, late, _, _, split, _) in zip(("forward", "backward", "backward"), plans(walk_cases.passes(c, kind))):
+                reached.setdefault((kind, dk, w, split, late), set()).add(part)
+    shapes = {(dk, w) for dk in (32, 64, 128, 256) for w in (4, 8)} | {(dk, w) for dk in (32, 64) for w in (1, 2)}
+    assert {r[:4] for r in reached} == {(kind, *s, split) for kind in range(3) for s in shapes for split in (0, 1)}
+    late = {r[:4] for r in reached if r[4]}
+    assert late == {(kind, dk, 8, split) for kind, dks in ((0, (32, 64)), (2, (32, 64, 128))) for dk in dks for split in (0, 1)}
+    assert all(reached[(*r, 1)] == {"forward", "backward"} for r in late)

@@ -26,7 +26,8 @@ class TokenMixer(nn.Module):
     shared out among the axes, the first ones' first. The buffers keep their types where the module's is changed.
 
     ``forward(x, residual=None, positions=None, state=None, offsets=None, final_state=False)``: x is [batch, places of each axis ...,
-    channels], with ``channels_first`` [batch, channels, places of each axis ...], and ``positions`` the places by default; with
+    channels], with ``channels_first`` [batch, channels, places of each axis ...], and ``positions`` the places by default, otherwise
+    [places of each axis ..., axes] or [places, axes] with all of them in one dimension, either with the batch in front; with
     ``offsets`` it is [tokens, channels], sequences one after another, with their ``positions`` [tokens, axes]. Returns (out, h), with
     ``final_state`` (out, h, last states), which ``state`` of a later call goes on from.
 
@@ -88,6 +89,8 @@ class TokenMixer(nn.Module):
         y, packed, h = self._normed(x, residual)
         if positions is None:
             positions = grid_positions(places, x.device)
+        elif offsets is None and positions.shape[-1 - self.axes:-1] == places:
+            positions = positions.flatten(-1 - self.axes, -2)
         if offsets is None:  # places of all axes become one dimension
             y, packed = y.flatten(1, -2), type(packed)(*(t.flatten(1, -2) for t in packed)) if packed is not None else None
         q, k, v = self._rotated(y, packed, positions)

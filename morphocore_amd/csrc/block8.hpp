@@ -1,5 +1,5 @@
 // Rows of values in units and 8-bit blocks, shared by the channel-mixing kernels (norm.hip, gated.hip,
-// weight8.hip).
+// weight8.hip); the token-mixing ones (rotary.hip, linear_attention.hpp) take the units.
 //
 // A lane holds a unit of 8 consecutive values of a row in float32; 4 consecutive lanes hold a block of 32.
 // A block is kept in 8 bits as 32 codes and one scale byte b: value = e4m3(code) * 2^(b - 127). The

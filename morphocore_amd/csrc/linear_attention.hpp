@@ -24,11 +24,11 @@
 // results are 8 neighbouring rows: the first operand of a S, with no exchange between lanes. Rows of the staged tiles are units of 8 values whose order
 // changes from row to row, so that row and transposing reads both spread over the banks.
 //
-// Measured, bfloat16, heads of 128 x 128. 32768 tokens of 32 heads, 128 columns a workgroup, two a CU: 147 us for the segments' states, 12
-// for the join and 340 to 360 for the results, where reading and writing alone take 255 and the instructions alone 295, of which 100 matrix and
-// about 700 vector ones a wave and chunk, which hardly overlap on a SIMD. 4 x 4096 tokens of 16 heads, 64 columns a workgroup: 47, 7 and 114
-// us; the backward's three passes in one launch 380, not split. float32 goes by chunks of 32 rows: 8 x 4096 tokens of 4 heads of 16 x 16 take
-// 12, 6 and 22 us, bound by the 3 us that one chunk's steps take after another.
+// Measured, bfloat16, heads of 128 x 128. 32768 tokens of 32 heads, 128 columns a workgroup, two a CU: 150 us for the segments' states, 12
+// for the join and 350 to 360 for the results, where reading and writing alone take 255 and the instructions alone 328, of which 122 matrix and
+// about 800 vector ones a wave and chunk, which hardly overlap on a SIMD. 4 x 4096 tokens of 16 heads, 64 columns a workgroup: 44, 7 and 124
+// us; the backward's three passes in one launch 419, not split. float32 goes by chunks of 32 rows: 8 x 4096 tokens of 4 heads of 16 x 16 take
+// 12, 6 and 21 us, bound by the 3 us that one chunk's steps take after another.
 #pragma once
 
 #include <cmath>
@@ -298,7 +298,7 @@ struct Spoiled
 };
 
 // The thread's number, anew at each call where registers are few (SPARE): what follows from it would be kept through the walk otherwise, and
-// spilled. 32768 tokens of 32 heads take 350 us instead of 445 so; where they aren't, forming it anew costs 2 to 5%.
+// spilled. 32768 tokens of 32 heads take 523 us instead of 577 so; where they aren't, forming it anew costs 2 to 5%.
 template <bool SPARE>
 __device__ __forceinline__ int thread_now()
 {
@@ -1024,10 +1024,10 @@ Plan plan_of(const Sequences& seq, int heads, const Pass& p)
 }
 
 // f(the shape of a pass): as few columns a workgroup as hold the pass's. Of more than 64, 128 where two such workgroups don't fit a CU (the
-// scores would be formed twice: 84 us instead of 57, forwards, for 4999 tokens of 6 heads of 96 x 77 in float16) and for sequences of one chunk, whose
+// scores would be formed twice: 88 us instead of 67, forwards, for 4999 tokens of 6 heads of 96 x 77 in float16) and for sequences of one chunk, whose
 // scores are most of the work (500 of 33 tokens of 8 heads of 64 x 128 in bfloat16: 84 us by 128, 125 by 64; 2000 of 60 of 16 heads of 128 x 128: 1100
-// and 1190), otherwise 128 or 64 by the estimate: 32768 tokens of 32 heads of 128 x 128 in bfloat16 take 492 us by 128 and 568 by 64; 12001 of 41
-// sequences take 200 and 166.
+// and 1190), otherwise 128 or 64 by the estimate: 32768 tokens of 32 heads of 128 x 128 in bfloat16 take 516 us by 128 and 612 by 64; 12001 of 41
+// sequences take 185 and 182.
 template <typename T, typename F>
 hipError_t by_walk(const Sequences& seq, int heads, const Pass& p, F&& f)
 {

@@ -6,10 +6,10 @@
 //
 // Bound by HBM: every row is read once and written once. A lane holds 8 pairs (their two halves apart, or side by
 // side) or 16 values behind the last pair, so the lanes of a row exchange only the norm's sums. A workgroup takes a few
-// tokens: it forms their sines and cosines once, in LDS, then all their heads, of queries and keys, in the order in which they lie in
-// memory. Few tokens' heads are spread over several workgroups. Measured, bfloat16: 65536 tokens of 16 heads of 64 rotated in 54 us
-// (5.0 TB/s, a large copy's rate); 16384 tokens of 32 and 8 heads of 128, normed and rotated in 60 us (5.6 TB/s, partly cached), their
-// gradients in 104 (4.9 TB/s) and 7 for the weights' slots; one token of those in 4.0.
+// tokens of one tensor: it forms their sines and cosines once, in LDS, then all their heads, in the order in which they lie in
+// memory (queries and keys each form their own). Few tokens' heads are spread over several workgroups. Measured, bfloat16: 65536 tokens
+// of 16 heads of 64 rotated in 54 us (5.0 TB/s, a large copy's rate); 16384 tokens of 32 and 8 heads of 128, normed and rotated in
+// 59 us (5.7 TB/s, partly cached), their gradients in 105 (4.8 TB/s) and 7 for the weights' slots; one token of those in 4.1.
 //
 // Angles are float64 up to a fraction of a turn: in float32 a position of 100000 would be off by 0.004 radians. What is
 // left of a turn goes through float32 sine and cosine, the rounding of a result.
@@ -162,65 +162,65 @@ __global__ __launch_bounds__(BLOCK) void rotary_kernel(RotaryTensor<T, WT> q, Ro
         for (int i = threadIdx.x; i < n * r.pairs; i += BLOCK) sine_cosine(r, token0 + i / r.pairs, i % r.pairs, inverse, sines[i], cosines[i]);
         __syncthreads();
         const float per_head = 1.0f / (float)t.x.heads;
-            for (int i = split * GROUPS + group; i < n * t.x.heads; i += splits * GROUPS)
-            {
-                const int at = (int)(((float)i + 0.5f) * per_head), head = i - at * t.x.heads;  // exact below 2^20
-                const int64_t token = token0 + at;
-                RawUnit<T> raw[2], rawh[2];
-                load_part(t.x.x + token * t.x.token_stride + head * t.x.head_stride, part, raw);
-                if (MODE == NORM_BACKWARD) load_part(t.h.x + token * t.h.token_stride + head * t.h.head_stride, part, rawh);
-                Turn turn;
+        for (int row = split * GROUPS + group; row < n * t.x.heads; row += splits * GROUPS)
+        {
+            const int at = (int)(((float)row + 0.5f) * per_head), head = row - at * t.x.heads;  // exact below 2^20
+            const int64_t token = token0 + at;
+            RawUnit<T> raw[2], rawh[2];
+            load_part(t.x.x + token * t.x.token_stride + head * t.x.head_stride, part, raw);
+            if (MODE == NORM_BACKWARD) load_part(t.h.x + token * t.h.token_stride + head * t.h.head_stride, part, rawh);
+            Turn turn;
 #pragma unroll
-                for (int e = 0; e < UNIT; ++e)
-                {
-                    // (A partial unit's further ones are other pairs', or what lies behind the table, for values that are not there.)
-                    turn.cos[e] = cosines[min(at * r.pairs + part.pair, ROTARY_TABLE) + e];
-                    turn.sin[e] = sines[min(at * r.pairs + part.pair, ROTARY_TABLE) + e];
-                }
-                float v[2][UNIT];
+            for (int e = 0; e < UNIT; ++e)
+            {
+                // (A partial unit's further ones are other pairs', or what lies behind the table, for values that are not there.)
+                turn.cos[e] = cosines[min(at * r.pairs + part.pair, ROTARY_TABLE) + e];
+                turn.sin[e] = sines[min(at * r.pairs + part.pair, ROTARY_TABLE) + e];
+            }
+            float v[2][UNIT];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < UNIT; ++j) v[i][j] = raw[i][j];
+            if constexpr (MODE == NORM_FORWARD)
+            {
+                float s = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int j = 0; j < UNIT; ++j) v[i][j] = raw[i][j];
-                if constexpr (MODE == NORM_FORWARD)
-                {
-                    float s = 0.0f;
+                    for (int j = 0; j < UNIT; ++j) s = fmaf(v[i][j], v[i][j], s);
+                const float rstd = 1.0f / sqrtf(fmaf(lane_sum<G>(s), inv, eps));
 #pragma unroll
-                    for (int i = 0; i < 2; ++i)
+                for (int i = 0; i < 2; ++i)
 #pragma unroll
-                        for (int j = 0; j < UNIT; ++j) s = fmaf(v[i][j], v[i][j], s);
-                    const float rstd = 1.0f / sqrtf(fmaf(lane_sum<G>(s), inv, eps));
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)
-#pragma unroll
-                        for (int j = 0; j < UNIT; ++j) v[i][j] = v[i][j] * rstd * w[i][j];
-                }
-                rotate<INTERLEAVED>(v, turn, part.pairs);
-                if constexpr (MODE == NORM_BACKWARD)
-                {
-                    float s = 0.0f, d = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)
-#pragma unroll
-                        for (int j = 0; j < UNIT; ++j)
-                        {
-                            s = fmaf(rawh[i][j], rawh[i][j], s);
-                            d = fmaf(v[i][j] * w[i][j], rawh[i][j], d);
-                        }
-                    const float rstd = 1.0f / sqrtf(fmaf(lane_sum<G>(s), inv, eps));
-                    const float mean = lane_sum<G>(d) * rstd * inv;
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)
-#pragma unroll
-                        for (int j = 0; j < UNIT; ++j)
-                        {
-                            const float m = rawh[i][j] * rstd;
-                            gw[i][j] = fmaf(v[i][j], m, gw[i][j]);
-                            v[i][j] = rstd * (v[i][j] * w[i][j] - m * mean);
-                        }
-                }
-                if (t.out) store_part(t.out + (token * t.x.heads + head) * dim, part, v, streaming);
+                    for (int j = 0; j < UNIT; ++j) v[i][j] = v[i][j] * rstd * w[i][j];
             }
+            rotate<INTERLEAVED>(v, turn, part.pairs);
+            if constexpr (MODE == NORM_BACKWARD)
+            {
+                float s = 0.0f, d = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < UNIT; ++j)
+                    {
+                        s = fmaf(rawh[i][j], rawh[i][j], s);
+                        d = fmaf(v[i][j] * w[i][j], rawh[i][j], d);
+                    }
+                const float rstd = 1.0f / sqrtf(fmaf(lane_sum<G>(s), inv, eps));
+                const float mean = lane_sum<G>(d) * rstd * inv;
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < UNIT; ++j)
+                    {
+                        const float m = rawh[i][j] * rstd;
+                        gw[i][j] = fmaf(v[i][j], m, gw[i][j]);
+                        v[i][j] = rstd * (v[i][j] * w[i][j] - m * mean);
+                    }
+            }
+            if (t.out) store_part(t.out + (token * t.x.heads + head) * dim, part, v, streaming);
+        }
     }
     if constexpr (MODE == NORM_BACKWARD)
     {
